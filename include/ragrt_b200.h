@@ -36,6 +36,10 @@ extern "C" {
 #define RAGRT_MAX_PROBE        128  /* nprobe (nc) per query token                            */
 #define RAGRT_MAX_CANDIDATES 16384  /* ndocs (k_candidates) per query and shard               */
 
+/* Element types of the entry points that take either 16-bit floating type. */
+#define RAGRT_F16                0
+#define RAGRT_BF16               1
+
 typedef struct ragrt_index ragrt_index;
 
 /*
@@ -273,6 +277,8 @@ const char* ragrt_last_error(void);
  * gave up a bounded wait (a tensor-core pipeline stage that never completed), 2 a code
  * outside [0, num_centroids) was met (the centroid row was not read), 3 the self-test below,
  * 4 a token id outside the vocabulary (ragrt_enc_embed);
+ * 5 a position outside the rotary table (ragrt_enc_qk_norm_rope);
+ * 6 a sequence table that is not ascending (ragrt_enc_packed_attention);
  * <0 on error.  Synchronises with the device's error flag.  reset != 0 clears it.
  */
 int ragrt_device_error(int32_t reset);
@@ -356,6 +362,66 @@ int ragrt_enc_embed(const int64_t* d_ids, const void* d_word, const void* d_pos,
  */
 int ragrt_enc_attention(const void* d_qkv, const int64_t* d_mask, void* d_ctx, int32_t B, int32_t L, int32_t heads,
                         int32_t dim, void* stream);
+
+/* ------------------------------------------------------------------------------------ *
+ * Layer operators of encoders with packed rows, rotary positions, grouped heads and gated
+ * feed-forward blocks, beside the fixed-shape ones above.  No counterpart in the reference,
+ * whose encoder is BERT on [B, 32] tokens.  dtype is RAGRT_F16 or RAGRT_BF16 for all 16-bit
+ * operands of a call; strides are in elements, multiples of 8; operands are 16-byte aligned;
+ * sums are fp32.  Outputs do not overlap inputs unless an entry point says so.
+ * ------------------------------------------------------------------------------------ */
+
+/*
+ * Attention over B packed sequences: rows d_cu_seqlens[b] .. d_cu_seqlens[b + 1] - 1 (int32
+ * [B + 1] on the device, ascending, within [0, T]) of d_q [T, heads, head_dim], d_k and d_v
+ * [T, kv_heads, head_dim] are sequence b; row strides let them be column blocks of one
+ * projection.  Query head h reads key head h / (heads / kv_heads).  causal != 0: row t sees the rows
+ * up to t of its sequence, else all of it.  d_out [T, heads, head_dim] = softmax(scale q k^T) v.
+ * A sequence may be empty; rows outside every sequence are not read as queries and not written.
+ * What no row may see (other sequences, later rows) does not reach its output, NaN and infinities
+ * included.  A table that is not ascending within [0, T] sets the device error flag to 6 and
+ * leaves the rows it cannot place unwritten.  head_dim a multiple of 8 up to 128.
+ */
+int ragrt_enc_packed_attention(const void* d_q, const void* d_k, const void* d_v, const int32_t* d_cu_seqlens,
+                               void* d_out, int32_t T, int32_t B, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                               int64_t q_stride, int64_t k_stride, int64_t v_stride, int64_t out_stride, float scale,
+                               int32_t causal, int32_t dtype, void* stream);
+
+/*
+ * RMS norm of every query and key head (over head_dim, weights d_q_weight / d_k_weight [head_dim]; a
+ * NULL weight leaves those heads as they are), then the rotation of their first rot_dim values by
+ * d_cos / d_sin [max_pos, rot_dim / 2] f32 at row d_pos[t] (int32 or int64: pos_bytes 4 or 8): pairs
+ * (i, i + rot_dim / 2), or neighbours (2 i, 2 i + 1) with interleaved != 0.  d_q [T, heads, head_dim],
+ * d_k [T, kv_heads, head_dim] (kv_heads may be 0); d_q_out may be d_q with the same stride, d_k_out
+ * likewise.  A position outside [0, max_pos) reads row 0 and sets the device error flag to 5.
+ * head_dim a multiple of 8 in [16, 256], rot_dim a multiple of 16 up to head_dim.
+ */
+int ragrt_enc_qk_norm_rope(const void* d_q, const void* d_k, const void* d_q_weight, const void* d_k_weight,
+                           const float* d_cos, const float* d_sin, const void* d_pos, int32_t pos_bytes,
+                           void* d_q_out, void* d_k_out, int32_t T, int32_t heads, int32_t kv_heads,
+                           int32_t head_dim, int32_t rot_dim, int32_t max_pos, int64_t q_stride, int64_t k_stride,
+                           int64_t q_out_stride, int64_t k_out_stride, float eps, int32_t interleaved, int32_t dtype,
+                           void* stream);
+
+/*
+ * d_h [M, F] = act(d_x . d_w_gate^T) * (d_x . d_w_up^T), d_x [M, K], weights [F, K] (the halves of a
+ * stacked [2 F, K] matrix will do): both projections, the activation and the product in one
+ * kernel.  act 0: silu, 1: gelu (erf form), 2: gelu (tanh form).  d_gate / d_up [M, F] (or both NULL)
+ * keep the two products for ragrt_enc_gated_ffn_backward.  F and K multiples of 8.
+ */
+int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const void* d_w_up, void* d_h, void* d_gate,
+                        void* d_up, int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype, void* stream);
+
+/*
+ * Gradients of ragrt_enc_gated_ffn from d_dh [M, F] and the kept d_gate / d_up: d_dgate, d_dup [M, F]
+ * (the gradients of the two products; always written, they may be d_gate and d_up themselves),
+ * d_dx [M, K] (may be NULL), d_dw_gate and d_dw_up [F, K] (may both be NULL).  Overwrites, does
+ * not add to, its outputs; the order of every sum is fixed.  M = 0 gives zero weight gradients.
+ */
+int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* d_w_gate, const void* d_w_up,
+                                 const void* d_gate, const void* d_up, void* d_dgate, void* d_dup, void* d_dx,
+                                 void* d_dw_gate, void* d_dw_up, int32_t M, int32_t F, int32_t K, int32_t act,
+                                 int32_t dtype, void* stream);
 
 /* Library version string. */
 const char* ragrt_version(void);

@@ -64,6 +64,12 @@ _SIGS = {
     "ragrt_enc_layernorm": (I32, [P, P, P, C.c_float, P, I32, I32, P]),
     "ragrt_enc_embed": (I32, [P, P, P, P, P, P, C.c_float, I32, I32, I32, I32, P, P]),
     "ragrt_enc_attention": (I32, [P, P, P, I32, I32, I32, I32, P]),
+    "ragrt_enc_packed_attention": (I32, [P, P, P, P, P, I32, I32, I32, I32, I32, I64, I64, I64, I64, C.c_float, I32,
+                                         I32, P]),
+    "ragrt_enc_qk_norm_rope": (I32, [P, P, P, P, P, P, P, I32, P, P, I32, I32, I32, I32, I32, I32, I64, I64, I64, I64,
+                                     C.c_float, I32, I32, P]),
+    "ragrt_enc_gated_ffn": (I32, [P, P, P, P, P, P, I32, I32, I32, I32, I32, P]),
+    "ragrt_enc_gated_ffn_backward": (I32, [P, P, P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, P]),
 }
 
 _lib = None

@@ -18,13 +18,10 @@
 //   enc_attention  two warps per (query, head): 32 tokens x head_dim 64; scores, masked
 //                  softmax and the weighted sum in fp32 (the 32 x 32 products are too small
 //                  for the tensor cores to pay).
-#include <cuda.h>
-
 #include <algorithm>
 #include <atomic>
-#include <utility>
 
-#include "common.cuh"
+#include "enc_common.cuh"
 #include "tc.cuh"
 
 namespace ragrt {
@@ -46,15 +43,6 @@ struct EncCfg {
     static constexpr uint32_t kTmemCols = 2 * BN;       // two accumulator buffers
 };
 
-// Programmatic dependent launch: every encoder kernel is launched so that it may start while
-// its predecessor in the stream drains; it does its own set-up, then waits for the
-// predecessor's results (griddepcontrol.wait returns at once for a normal launch) and lets
-// its own successor start early.
-__device__ __forceinline__ void pdl_wait_then_release() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 enum EncEpilogue : int { kEpiBias = 0, kEpiBiasGelu = 1, kEpiBiasGeluTanh = 2, kEpiBiasResidual = 3, kEpiNorm = 4 };
 
 struct EncGemmParams {
@@ -66,12 +54,6 @@ struct EncGemmParams {
     int ksplit;               // > 1: each unit sums a slice of K into partial[slice][M][N] (fp32)
     float* partial;
 };
-
-__device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
-__device__ __forceinline__ float gelu_tanh(float x) {
-    const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
-    return 0.5f * x * (1.0f + tanhf(u));
-}
 
 // Persistent: CTA c takes tiles c, c + grid, ... (N-tile index fastest, so neighbouring CTAs
 // share the A row block).  The TMA ring runs across tile boundaries; the MMA warp alternates
@@ -637,59 +619,6 @@ enc_attention(const __half* __restrict__ qkv, const int64_t* __restrict__ mask, 
     }
 }
 
-// Launch with programmatic stream serialisation (see pdl_wait_then_release).
-template <typename... KArgs, typename... Args>
-int enc_launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        return fail(RAGRT_ERR_CUDA, "encoder kernel launch: %s", cudaGetErrorString(e));
-    }
-    count_launch();
-    return RAGRT_OK;
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn enc_encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (EncodeTiledFn)f;
-    }
-    return fn;
-}
-
-// fp16 [rows, cols] row-major, box [box_rows x 64 cols], 128-byte swizzle (out-of-range rows read 0)
-int enc_make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int box_rows) {
-    EncodeTiledFn fn = enc_encode_fn();
-    if (!fn) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-    const cuuint32_t box[2] = {(cuuint32_t)kEK, (cuuint32_t)box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return RAGRT_OK;
-}
-
 }  // namespace
 }  // namespace ragrt
 
@@ -699,8 +628,8 @@ template <int BN>
 static int enc_gemm_launch(const void* d_A, const void* d_W, int32_t M, int32_t N, int32_t K, const EncGemmParams& p,
                            cudaStream_t stream) {
     CUtensorMap tA, tW;
-    int rc = enc_make_map(&tA, d_A, M, K, kEM);
-    if (rc || (rc = enc_make_map(&tW, d_W, N, K, BN))) return rc;
+    int rc = enc_map_2d(&tA, RAGRT_F16, d_A, M, K, K, kEM);
+    if (rc || (rc = enc_map_2d(&tW, RAGRT_F16, d_W, N, K, K, BN))) return rc;
     // the shared-memory attribute is per device: set it once for each device used
     static std::atomic<uint64_t> attr_set{0};
     int dev = 0;

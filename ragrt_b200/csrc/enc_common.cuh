@@ -1,0 +1,121 @@
+// enc_common.cuh -- what the encoder's kernels share: programmatic dependent launch, TMA tensor
+// maps, 16-bit vectors of either floating type, activations.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include <utility>
+
+#include "common.cuh"
+
+namespace ragrt {
+
+// Programmatic dependent launch: every encoder kernel is launched so that it may start while
+// its predecessor in the stream drains; it does its own set-up, then waits for the
+// predecessor's results (griddepcontrol.wait returns at once for a normal launch) and lets
+// its own successor start early.
+__device__ __forceinline__ void pdl_wait_then_release() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Launch with programmatic stream serialisation (see pdl_wait_then_release).
+template <typename... KArgs, typename... Args>
+int enc_launch(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(RAGRT_ERR_CUDA, "encoder kernel launch: %s", cudaGetErrorString(e));
+    }
+    count_launch();
+    return RAGRT_OK;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn enc_encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    if (!fn) {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiledFn)f;
+    }
+    return fn;
+}
+
+// 16-bit [rows, cols] matrix whose rows lie `stride` elements apart (a multiple of 8), box
+// [box_rows x 64 cols], 128-byte swizzle; what lies outside reads 0.
+inline int enc_map_2d(CUtensorMap* m, int dtype, const void* base, int64_t rows, int64_t cols, int64_t stride,
+                      int box_rows) {
+    EncodeTiledFn fn = enc_encode_fn();
+    if (!fn) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(m, dtype == RAGRT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                    const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return RAGRT_OK;
+}
+
+// ------------------------------------------------------------------ 16-bit vectors
+template <typename T>
+struct Pair16;
+template <>
+struct Pair16<__half> {
+    typedef __half2 type;
+    static __device__ __forceinline__ float2 up(__half2 v) { return __half22float2(v); }
+    static __device__ __forceinline__ __half2 down(float a, float b) { return __floats2half2_rn(a, b); }
+};
+template <>
+struct Pair16<__nv_bfloat16> {
+    typedef __nv_bfloat162 type;
+    static __device__ __forceinline__ float2 up(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+    static __device__ __forceinline__ __nv_bfloat162 down(float a, float b) { return __floats2bfloat162_rn(a, b); }
+};
+
+// 8 values of 16 bits <-> 8 floats
+template <typename T>
+__device__ __forceinline__ void up8(const uint4& u, float (&f)[8]) {
+    const typename Pair16<T>::type* h = reinterpret_cast<const typename Pair16<T>::type*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = Pair16<T>::up(h[i]);
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 down8(const float (&f)[8]) {
+    uint4 u;
+    typename Pair16<T>::type* h = reinterpret_cast<typename Pair16<T>::type*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = Pair16<T>::down(f[2 * i], f[2 * i + 1]);
+    return u;
+}
+
+// ------------------------------------------------------------------ activations
+__device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+__device__ __forceinline__ float gelu_tanh(float x) {
+    const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
+    return 0.5f * x * (1.0f + tanhf(u));
+}
+
+}  // namespace ragrt

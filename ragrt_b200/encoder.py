@@ -15,6 +15,14 @@ normalisation fused, LayerNorm and the 32-token attention as their own kernels.
                                  (fast_encoder.py:80-125); `checkpoint` needs .query_tokenizer,
                                  .linear and a BERT model (.bert, .model.bert or .model.LM)
 
+Layer operators for encoders with packed rows, rotary positions, grouped heads and gated
+feed-forward blocks (fp16 or bf16, no counterpart in the reference):
+
+  packed_attention(q, k, v, cu_seqlens, causal)      attention over packed sequences
+  qk_norm_rope(q, k, cos, sin, positions, ...)       per-head RMS norm + rotary positions
+  gated_ffn(x, w_gate, w_up, act)                    act(x w_gate^T) * (x w_up^T)
+  gated_ffn_backward(dh, x, w_gate, w_up, ...)       its gradients
+
 The token ids, [Q] marker and [MASK] padding come from the checkpoint's own tokenizer, as in
 the reference; `encode_ids` takes already-tokenized input.
 """
@@ -132,6 +140,181 @@ def flat_forward(W, ids, mask):
     out = torch.empty(M, W["linear"].shape[0], dtype=torch.float16, device=dev)
     _gemm(x, W["linear"], None, out, EPI_NORM, ws=ws)
     return out.view(B, L, -1)
+
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+def _dtype16(*ts):
+    """Type code of a call's 16-bit tensors (None for an absent one), which must agree."""
+    ts = [t for t in ts if t is not None]
+    if ts[0].dtype not in _DTYPES or any(t.dtype != ts[0].dtype for t in ts):
+        raise RuntimeError(f"the operands must all be fp16 or all bf16; got {[t.dtype for t in ts]}")
+    return _DTYPES[ts[0].dtype]
+
+
+def _rows_ok(t):
+    """Whether [T, H, D] rows can be read in place: heads side by side, rows apart by a multiple of
+    16 bytes that holds them all, 16-byte aligned."""
+    T, H, D = t.shape
+    return ((t.stride(2) == 1 or D == 1) and (t.stride(1) == D or H <= 1) and t.data_ptr() % 16 == 0 and
+            (T <= 1 or (t.stride(0) >= H * D and t.stride(0) % 8 == 0)))
+
+
+def _rows(t):
+    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _solid(t):
+    """Contiguous and 16-byte aligned (a copy where it is not)."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _span(t):
+    """(first byte, row pitch in bytes, bytes of a row, rows) of a tensor whose rows are solid."""
+    row = t[0].numel() * t.element_size()
+    pitch = t.stride(0) * t.element_size() if t.shape[0] > 1 else row
+    return t.data_ptr(), pitch, row, t.shape[0]
+
+
+def _overlap(a, b):
+    """Whether the bytes of two tensors with solid rows can meet.  Column blocks of one matrix
+    interleave without meeting."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (pa, sa, wa, na), (pb, sb, wb, nb) = _span(a), _span(b)
+    if pa + (na - 1) * sa + wa <= pb or pb + (nb - 1) * sb + wb <= pa:
+        return False
+    if sa == sb:
+        d = (pb - pa) % sa                                    # b's rows begin d bytes into a's pitch
+        return d < wa or d + wb > sa
+    return True
+
+
+def _same(a, b):
+    return a.data_ptr() == b.data_ptr() and _row_stride(a) == _row_stride(b) and a.shape == b.shape
+
+
+def _output(out, shape, like, inputs, in_place_of=None):
+    """`out` checked (shape, like's type, rows in place, apart from the inputs), or a new contiguous one."""
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if out.shape != shape or out.dtype != like.dtype:
+        raise RuntimeError(f"out must be {tuple(shape)} {like.dtype}; got {tuple(out.shape)} {out.dtype}")
+    if not (_rows_ok(out) if out.dim() == 3 else out.is_contiguous() and out.data_ptr() % 16 == 0):
+        raise RuntimeError("out must be written in place: solid rows, 16-byte aligned, strides in multiples of 8")
+    for t in inputs:
+        if t is not None and _overlap(out, t) and not (t is in_place_of and _same(out, t)):
+            raise RuntimeError("out overlaps an input")
+    return out
+
+
+def packed_attention(q, k, v, cu_seqlens, causal=False, scale=None, out=None):
+    """Attention over packed sequences: q [T, H, D], k and v [T, KV, D] (fp16 or bf16; views of one
+    projection are read in place), sequence b in rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32
+    [B + 1], ascending) -> out [T, H, D].  Head h reads key head h // (H // KV); causal: a row sees
+    its sequence up to itself.  scale defaults to D ** -0.5.  Rows outside every sequence are not
+    written (undefined in a new `out`).  D a multiple of 8 up to 128.  A bad table raises the
+    device error flag (6) and leaves rows unwritten.  Not differentiable."""
+    _need_cuda(q, k, v, cu_seqlens, out)
+    dt = _dtype16(q, k, v)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise RuntimeError(f"q [T, H, D], k and v [T, KV, D] wanted; got {tuple(q.shape)}, {tuple(k.shape)}, "
+                           f"{tuple(v.shape)}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("cu_seqlens must be int32 [B + 1]")
+    cu = cu_seqlens.to(torch.int32).contiguous()
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    T, H, D = q.shape
+    out = _output(out, q.shape, q, (q, k, v))
+    _lib.check(_lib.lib().ragrt_enc_packed_attention(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(cu), _ptr(out), T, cu.shape[0] - 1, H, k.shape[1], D, _row_stride(q),
+        _row_stride(k), _row_stride(v), _row_stride(out), float(D ** -0.5 if scale is None else scale),
+        int(bool(causal)), dt, _stream()))
+    return out
+
+
+def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e-6, interleaved=False, q_out=None,
+                 k_out=None):
+    """RMS norm of each query and key head (skipped where its weight is None), then the rotation by
+    cos / sin [max_pos, R / 2] f32 at positions [T] (int32 or int64) of each head's first R values:
+    pairs (i, i + R / 2), or neighbours with `interleaved`.  q [T, H, D], k [T, KV, D] fp16 or bf16 ->
+    (q_out, k_out), which may be q and k themselves.  D a multiple of 8 in [16, 256], R a multiple
+    of 16.  A position outside the table reads its row 0 and raises the device error flag (5)."""
+    _need_cuda(q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out)
+    dt = _dtype16(q, k, q_weight, k_weight)
+    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise RuntimeError(f"q [T, H, D] and k [T, KV, D] wanted; got {tuple(q.shape)}, {tuple(k.shape)}")
+    T, H, D = q.shape
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise RuntimeError("cos and sin must be f32 [max_pos, R / 2]")
+    if positions.shape != (T,) or positions.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"positions must be int32 or int64 [{T}]")
+    for w in (q_weight, k_weight):
+        if w is not None and w.shape != (D,):
+            raise RuntimeError(f"a norm weight must be [{D}]; got {tuple(w.shape)}")
+    qi, ki = _rows(q), _rows(k)
+    cos, sin, qw, kw, pos = _solid(cos), _solid(sin), _solid(q_weight), _solid(k_weight), positions.contiguous()
+    q_out = _output(q_out, q.shape, q, (qi, ki), in_place_of=qi)
+    k_out = _output(k_out, k.shape, k, (qi, ki, q_out), in_place_of=ki)
+    _lib.check(_lib.lib().ragrt_enc_qk_norm_rope(
+        _ptr(qi), _ptr(ki), _ptr(qw), _ptr(kw), _ptr(cos), _ptr(sin), _ptr(pos), pos.element_size(), _ptr(q_out),
+        _ptr(k_out), T, H, k.shape[1], D, 2 * cos.shape[1], cos.shape[0], _row_stride(qi), _row_stride(ki),
+        _row_stride(q_out), _row_stride(k_out), float(eps), int(bool(interleaved)), dt, _stream()))
+    return q_out, k_out
+
+
+def _ffn_args(x, w_gate, w_up, act):
+    if act not in _ACTS:
+        raise RuntimeError(f"unknown activation {act!r}: one of {sorted(_ACTS)}")
+    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[1]:
+        raise RuntimeError(f"x [M, K], w_gate and w_up [F, K] wanted; got {tuple(x.shape)}, {tuple(w_gate.shape)}, "
+                           f"{tuple(w_up.shape)}")
+    return x.shape[0], w_gate.shape[0], x.shape[1]
+
+
+def gated_ffn(x, w_gate, w_up, act="silu", keep=False, out=None):
+    """h [M, F] = act(x w_gate^T) * (x w_up^T) in one kernel: x [M, K], weights [F, K] (the halves of
+    a stacked [2 F, K] matrix are read in place), fp16 or bf16, F and K multiples of 8; act "silu",
+    "gelu" (erf form) or "gelu_tanh".  keep=True returns (h, gate, up) with the two products that
+    gated_ffn_backward wants.  Not tracked by autograd."""
+    _need_cuda(x, w_gate, w_up, out)
+    dt = _dtype16(x, w_gate, w_up)
+    M, F, K = _ffn_args(x, w_gate, w_up, act)
+    x, wg, wu = _solid(x), _solid(w_gate), _solid(w_up)
+    h = _output(out, (M, F), x, (x, wg, wu))
+    gate = up = None
+    if keep:
+        gate, up = x.new_empty(M, F), x.new_empty(M, F)
+    _lib.check(_lib.lib().ragrt_enc_gated_ffn(_ptr(x), _ptr(wg), _ptr(wu), _ptr(h), _ptr(gate), _ptr(up), M, F, K,
+                                              _ACTS[act], dt, _stream()))
+    return (h, gate, up) if keep else h
+
+
+def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu", need_dx=True, need_dw=True):
+    """Gradients of gated_ffn from dh [M, F] and the kept gate and up: (dx [M, K], dw_gate [F, K],
+    dw_up [F, K]) in the inputs' type, None for what is not needed.  Sums run in a fixed order."""
+    _need_cuda(dh, x, w_gate, w_up, gate, up)
+    dt = _dtype16(dh, x, w_gate, w_up, gate, up)
+    M, F, K = _ffn_args(x, w_gate, w_up, act)
+    if dh.shape != (M, F) or gate.shape != (M, F) or up.shape != (M, F):
+        raise RuntimeError(f"dh, gate and up must be {(M, F)}; got {tuple(dh.shape)}, {tuple(gate.shape)}, "
+                           f"{tuple(up.shape)}")
+    dh, x, wg, wu, gate, up = (_solid(t) for t in (dh, x, w_gate, w_up, gate, up))
+    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
+    dx = torch.empty_like(x) if need_dx else None
+    dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_dw else (None, None)
+    _lib.check(_lib.lib().ragrt_enc_gated_ffn_backward(
+        _ptr(dh), _ptr(x), _ptr(wg), _ptr(wu), _ptr(gate), _ptr(up), _ptr(dgate), _ptr(dup), _ptr(dx), _ptr(dwg),
+        _ptr(dwu), M, F, K, _ACTS[act], dt, _stream()))
+    return dx, dwg, dwu
 
 
 class FastQueryEncoder:
