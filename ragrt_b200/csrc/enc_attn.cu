@@ -5,10 +5,20 @@
 // over the keys j of t's own sequence (with causal set: those up to t).  The sequences lie one behind
 // the other in the rows of q, k, v; cu_seqlens names where each begins.
 //
-//   packed_attn_simt   a warp per (row, head): 32 keys per step, scores, running maximum and sum in fp32.
+//   packed_attn_mma    a CTA per 256 packed rows (two tiles of 128) and head.  The tiles run over the rows
+//                      as they lie, whatever sequences they belong to: a tile walks the keys of the
+//                      sequences that it touches, and each row masks what is not its own.  Short sequences
+//                      thus share a tile, and no tile is padded but the last.  Warp 0 streams Q and the
+//                      128-key blocks of K and V by TMA, warp 1 issues the products (S = Q K^T and
+//                      O += P V, P from tensor memory), and per tile four warps run the softmax, a
+//                      thread per row.
+//   attn_row           one row of one head by a warp, in fp32.  A weight of zero does not keep a NaN or
+//                      an infinity in a masked row of V out of a matrix product: rows that come out
+//                      of it not finite are computed once more by this, over their own keys alone.
 #include <algorithm>
 
 #include "enc_common.cuh"
+#include "tc.cuh"
 
 namespace ragrt {
 
@@ -104,18 +114,317 @@ __device__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi, floa
         if (lane + 32 * c < p.dim) dst[lane + 32 * c] = (T)(o[c] / l);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) packed_attn_simt(const AttnParams p) {
-    __shared__ float sq[8][128];
+constexpr int kAM = 128;                       // rows per tile, keys per block
+constexpr int kATiles = 2;
+constexpr int kAThreads = 64 + kATiles * 128;  // TMA warp, MMA warp, four softmax warps per tile
+constexpr uint32_t kAWaitLimit = 1u << 26;
+// The reference maximum of a row moves only when it is exceeded by 2^8: until then the weights are
+// at most 256, well inside either type, and the accumulator is not rescaled.
+constexpr float kARescale = 8.0f;
+
+template <int DP>
+struct AttnCfg {
+    static constexpr int kTile = kAM * DP * 2;                    // bytes of a Q tile, a K or a V block
+    static constexpr int kStages = DP == 128 ? 4 : 8;             // K and V blocks in flight
+    static constexpr int kSmem = 1024 + (kATiles + kStages) * kTile + 512;
+    static constexpr uint32_t kO = kATiles * kAM;                 // first accumulator column: S and P lie before
+};
+
+struct AttnMaps {
+    CUtensorMap q, k, v;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
+    using Cfg = AttnCfg<DP>;
+    constexpr int S = Cfg::kStages;
+    extern __shared__ uint8_t attn_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)attn_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* sQ = sm;
+    uint8_t* sKV = sm + kATiles * Cfg::kTile;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sKV + S * Cfg::kTile);
+    uint64_t* empty = full + S;
+    uint64_t* qfull = empty + S;
+    uint64_t* sfull = qfull + 1;             // [2] scores ready (MMA -> softmax)
+    uint64_t* pready = sfull + kATiles;      // [2] weights written (softmax -> MMA)
+    uint64_t* ofull = pready + kATiles;      // [2] last product done
+    uint64_t* drain = ofull + kATiles;
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
+    int* swlo = reinterpret_cast<int*>(tslot + 2);                // [8] key range of each softmax warp's rows
+    int* swhi = swlo + 4 * kATiles;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the tiles of a causal sequence grow along it: the longest go first
+    const int tiles = (p.T + kATiles * kAM - 1) / (kATiles * kAM);
+    const int h = blockIdx.x % p.heads;
+    const int row0 = (tiles - 1 - (int)(blockIdx.x / p.heads)) * kATiles * kAM;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            tc::mbar_init(full + s, 1);
+            tc::mbar_init(empty + s, 1);
+        }
+        tc::mbar_init(qfull, 1);
+        tc::mbar_init(drain, 1);
+        for (int t = 0; t < kATiles; ++t) {
+            tc::mbar_init(sfull + t, 1);
+            tc::mbar_init(pready + t, 4);
+            tc::mbar_init(ofull + t, 1);
+        }
+        *abort = 0;
+        tc::mbar_fence_init();
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(tslot, 512);
+        tc::tmem_relinquish();
+    }
     pdl_wait_then_release();
     attn_check_table(p);
-    const int warp = threadIdx.x >> 5;
-    const int64_t unit = (int64_t)blockIdx.x * 8 + warp;
-    if (unit >= (int64_t)p.T * p.heads) return;
-    const int t = (int)(unit / p.heads), h = (int)(unit % p.heads);
-    int lo, hi;
-    attn_range(p, t, lo, hi);
-    if (lo < hi) attn_row<T>(p, t, h, lo, hi, sq[warp]);
+    const int tile = (warp - 2) >> 2, quad = warp & 3;
+    int lo = 0, hi = 0;
+    const int row = row0 + tile * kAM + quad * 32 + lane;         // of a softmax thread
+    if (warp >= 2) {
+        attn_range(p, row, lo, hi);
+        const int wl = __reduce_min_sync(0xFFFFFFFFu, lo < hi ? lo : 0x7FFFFFFF);
+        const int wh = __reduce_max_sync(0xFFFFFFFFu, hi);
+        if (lane == 0) {
+            swlo[warp - 2] = wl;
+            swhi[warp - 2] = wh;
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tbase = *tslot;
+    // the keys that each tile walks, in blocks of 128 from the first key of either
+    int kv0 = 0x7FFFFFFF, kv1 = 0, jb[kATiles], je[kATiles];
+#pragma unroll
+    for (int t = 0; t < kATiles; ++t) {
+        jb[t] = 0x7FFFFFFF;
+        je[t] = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            jb[t] = min(jb[t], swlo[4 * t + w]);
+            je[t] = max(je[t], swhi[4 * t + w]);
+        }
+        kv0 = min(kv0, jb[t]);
+        kv1 = max(kv1, je[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < kATiles; ++t) {
+        const bool any = je[t] > 0;
+        jb[t] = any ? (jb[t] - kv0) / kAM : 0;
+        je[t] = any ? (je[t] - kv0 + kAM - 1) / kAM : 0;
+    }
+    const int n = max(je[0], je[1]);
+    bool failed = false;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0 && n > 0) {
+            const int g = h / (p.heads / p.kv_heads);
+            tc::mbar_arrive_expect_tx(qfull, kATiles * Cfg::kTile);
+            for (int t = 0; t < kATiles; ++t)
+                for (int c = 0; c < DP / 64; ++c)
+                    tc::tma_load_3d(sQ + t * Cfg::kTile + c * kAM * 128, &maps.q, 64 * c, h, row0 + t * kAM, qfull);
+            int i = 0;
+            for (; i < 2 * n; ++i) {                              // K0, V0, K1, V1, ...
+                const int s = i % S;
+                if (i >= S && !tc::mbar_wait_or_abort(empty + s, ((i / S) - 1) & 1, abort, kAWaitLimit)) {
+                    failed = true;
+                    break;
+                }
+                tc::mbar_arrive_expect_tx(full + s, Cfg::kTile);
+                for (int c = 0; c < DP / 64; ++c)
+                    tc::tma_load_3d(sKV + s * Cfg::kTile + c * kAM * 128, i & 1 ? &maps.v : &maps.k, 64 * c, g,
+                                    kv0 + (i >> 1) * kAM, full + s);
+            }
+            if (failed) {                                         // copies in flight end before the CTA does
+                (void)tc::mbar_wait_bounded(qfull, 0, kAWaitLimit);
+                for (int k = max(0, i - S); k < i; ++k)
+                    (void)tc::mbar_wait_bounded(full + k % S, (k / S) & 1, kAWaitLimit);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t idS = tc::idesc_f16_f32(kAM, kAM) | idesc_type<T>();
+            constexpr uint32_t idO = tc::idesc_f16_f32(kAM, DP) | idesc_type<T>() | kIdescBMn;
+            failed = !tc::mbar_wait_or_abort(qfull, 0, abort, kAWaitLimit);
+            for (int j = -1; j < n && !failed; ++j) {
+                const int vi = 2 * j + 1, ki = 2 * j + 2;
+                if (j >= 0) failed = !tc::mbar_wait_or_abort(full + vi % S, (vi / S) & 1, abort, kAWaitLimit);
+                if (!failed && j + 1 < n) failed = !tc::mbar_wait_or_abort(full + ki % S, (ki / S) & 1, abort, kAWaitLimit);
+                if (failed) break;
+                tc::fence_after();
+                const uint32_t v = tc::smem_u32(sKV + (vi % S) * Cfg::kTile), k = tc::smem_u32(sKV + (ki % S) * Cfg::kTile);
+#pragma unroll
+                for (int t = 0; t < kATiles; ++t) {
+                    if (j >= jb[t] && j < je[t]) {
+                        if (!tc::mbar_wait_or_abort(pready + t, (j - jb[t]) & 1, abort, kAWaitLimit)) {
+                            failed = true;
+                            break;
+                        }
+                        tc::fence_after();
+#pragma unroll
+                        for (int c = 0; c < kAM / 16; ++c)
+                            tc::mma_ts(tbase + Cfg::kO + t * DP, tbase + t * kAM + 8 * c,
+                                       tc::sw128_mnmajor_desc(v + 2048 * c, kAM * 128), idO, j > jb[t] || c > 0);
+                        if (j == je[t] - 1) tc::mma_commit(ofull + t);
+                    }
+                    if (j + 1 >= jb[t] && j + 1 < je[t]) {
+                        // S takes the columns of the P that the product just issued reads: the tensor
+                        // pipe runs them one behind the other
+                        const uint32_t q = tc::smem_u32(sQ + t * Cfg::kTile);
+#pragma unroll
+                        for (int c = 0; c < DP / 16; ++c) {
+                            const uint32_t at = (c >> 2) * kAM * 128 + (c & 3) * 32;
+                            tc::mma_ss(tbase + t * kAM, tc::sw128_kmajor_desc(q + at), tc::sw128_kmajor_desc(k + at), idS,
+                                       c > 0);
+                        }
+                        tc::mma_commit(sfull + t);
+                    }
+                }
+                if (failed) break;
+                if (j >= 0) tc::mma_commit(empty + vi % S);
+                if (j + 1 < n) tc::mma_commit(empty + ki % S);
+            }
+            if (failed) {                                         // the last products read shared memory
+                tc::mma_commit(drain);
+                (void)tc::mbar_wait_bounded(drain, 0, kAWaitLimit);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ softmax, a thread per row
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const uint32_t ts = tbase + lanes + (uint32_t)(tile * kAM), to = tbase + lanes + Cfg::kO + (uint32_t)(tile * DP);
+        const float scale2 = p.scale * 1.4426950408889634f;       // weights are powers of two
+        const int b0 = tile == 0 ? jb[0] : jb[1], b1 = tile == 0 ? je[0] : je[1];
+        float m = -INFINITY, l = 0.f;
+        for (int j = b0; j < b1; ++j) {
+            const bool ok = tc::mbar_wait_or_abort(sfull + tile, (j - b0) & 1, abort, kAWaitLimit);
+            if (!__all_sync(0xFFFFFFFFu, ok)) {
+                failed = true;
+                break;
+            }
+            tc::fence_after();
+            float s[128];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+            tc::wait_ld();
+            const int first = kv0 + j * kAM;
+            if (!__all_sync(0xFFFFFFFFu, lo <= first && first + kAM <= hi)) {
+                const int c0 = lo - first, c1 = hi - first;
+#pragma unroll
+                for (int c = 0; c < 128; ++c) s[c] = c >= c0 && c < c1 ? s[c] : -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+            const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+            if (__any_sync(0xFFFFFFFFu, bm > m + kARescale)) {
+                // the scores of this block came behind the product with the last weights, so the
+                // accumulator is at rest
+                const float mn = fmaxf(m, bm);
+                const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+                l *= alpha;
+                m = mn;
+                if (j > b0) {
+#pragma unroll 1
+                    for (int c = 0; c < DP / 32; ++c) {
+                        uint32_t r[32];
+                        tc::ld32x32(to + 32 * c, r);
+                        tc::wait_ld();
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * alpha);
+                        tc::st32x32(to + 32 * c, r);
+                    }
+                }
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t w[32];
+#pragma unroll
+                for (int q = 0; q < 32; ++q) {
+                    const float a = ex2(fmaf(s[64 * c + 2 * q], scale2, -ref));
+                    const float b = ex2(fmaf(s[64 * c + 2 * q + 1], scale2, -ref));
+                    sum[(2 * q) & 3] += a;
+                    sum[(2 * q + 1) & 3] += b;
+                    const typename Pair16<T>::type ab = Pair16<T>::down(a, b);
+                    w[q] = *reinterpret_cast<const uint32_t*>(&ab);
+                }
+                tc::st32x32(ts + 32 * c, w);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(pready + tile);
+        }
+        if (!failed && b1 > b0) {
+            const bool ok = tc::mbar_wait_or_abort(ofull + tile, 0, abort, kAWaitLimit);
+            failed = !__all_sync(0xFFFFFFFFu, ok);
+        }
+        if (!failed && b1 > b0) {
+            tc::fence_after();
+            const float inv = 1.0f / l;
+            float o[DP];
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) tc::ld32x32(to + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o + 32 * c));
+            tc::wait_ld();
+            float odd = 0.f;
+#pragma unroll
+            for (int c = 0; c < DP; ++c) {
+                o[c] *= inv;
+                odd = fmaf(o[c], 0.f, odd);                       // NaN as soon as one is not finite
+            }
+            const bool mine = lo < hi, bad = mine && !(odd == 0.f);
+            if (mine && !bad) {
+                T* dst = static_cast<T*>(p.out) + row * p.out_stride + (int64_t)h * p.dim;
+#pragma unroll
+                for (int c = 0; c < DP; c += 8)
+                    if (c < p.dim) *reinterpret_cast<uint4*>(dst + c) = down8<T>(*reinterpret_cast<float(*)[8]>(o + c));
+            }
+            // Q is no longer read by any product of this tile: its place serves attn_row
+            float* sq = reinterpret_cast<float*>(sQ + tile * Cfg::kTile) + 128 * ((warp - 2) & 3);
+            for (unsigned left = __ballot_sync(0xFFFFFFFFu, bad); left; left &= left - 1) {
+                const int src = __ffs(left) - 1;
+                attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), h, __shfl_sync(0xFFFFFFFFu, lo, src),
+                            __shfl_sync(0xFFFFFFFFu, hi, src), sq);
+            }
+        }
+    }
+    if (failed && lane == 0) atomicExch(p.err, 1);
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc::fence_after();
+        tc::tmem_dealloc(tbase, 512);
+    }
+}
+
+template <typename T, int DP>
+int attn_launch(int dtype, const AttnParams& p, cudaStream_t stream) {
+    static std::atomic<uint64_t> done{0};
+    int rc = enc_allow_smem(packed_attn_mma<T, DP>, AttnCfg<DP>::kSmem, done);
+    if (rc) return rc;
+    AttnMaps m;
+    if ((rc = enc_map_heads(&m.q, dtype, p.q, p.T, p.heads, p.dim, p.q_stride, kAM)) ||
+        (rc = enc_map_heads(&m.k, dtype, p.k, p.T, p.kv_heads, p.dim, p.k_stride, kAM)) ||
+        (rc = enc_map_heads(&m.v, dtype, p.v, p.T, p.kv_heads, p.dim, p.v_stride, kAM)))
+        return rc;
+    const int64_t blocks = ceil_div(p.T, kATiles * kAM) * p.heads;
+    if (blocks > 0x7FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many rows x heads");
+    return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)blocks), dim3(kAThreads), AttnCfg<DP>::kSmem, stream, m, p);
 }
 
 }  // namespace
@@ -150,10 +459,9 @@ extern "C" int ragrt_enc_packed_attention(const void* d_q, const void* d_k, cons
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
     AttnParams p{d_q, d_k, d_v, d_out, d_cu_seqlens, q_stride, k_stride, v_stride, out_stride, T, B, heads, kv_heads,
                  head_dim, causal != 0, scale, err};
-    const int64_t blocks = ceil_div((int64_t)T * heads, 8);
-    RAGRT_REQUIRE(blocks <= 0x7FFFFFFF, "too many rows x heads");
-    return dtype == RAGRT_BF16 ? enc_launch(packed_attn_simt<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), 0,
-                                            (cudaStream_t)stream_, p)
-                               : enc_launch(packed_attn_simt<__half>, dim3((unsigned)blocks), dim3(256), 0,
-                                            (cudaStream_t)stream_, p);
+    cudaStream_t stream = (cudaStream_t)stream_;
+    if (dtype == RAGRT_BF16)
+        return head_dim <= 64 ? attn_launch<__nv_bfloat16, 64>(dtype, p, stream)
+                              : attn_launch<__nv_bfloat16, 128>(dtype, p, stream);
+    return head_dim <= 64 ? attn_launch<__half, 64>(dtype, p, stream) : attn_launch<__half, 128>(dtype, p, stream);
 }

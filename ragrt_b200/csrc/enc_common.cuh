@@ -4,6 +4,8 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <atomic>
+#include <type_traits>
 #include <utility>
 
 #include "common.cuh"
@@ -74,6 +76,44 @@ inline int enc_map_2d(CUtensorMap* m, int dtype, const void* base, int64_t rows,
     if (r != CUDA_SUCCESS) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return RAGRT_OK;
 }
+
+// 16-bit [rows, heads, dim] tensor, rows `stride` elements apart, box [box_rows x 1 x 64]: one head's
+// columns of box_rows rows; columns behind dim and rows behind the last read 0.
+inline int enc_map_heads(CUtensorMap* m, int dtype, const void* base, int64_t rows, int heads, int dim, int64_t stride,
+                         int box_rows) {
+    EncodeTiledFn fn = enc_encode_fn();
+    if (!fn) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)dim * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64u, 1u, (cuuint32_t)box_rows};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(m, dtype == RAGRT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                    const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return RAGRT_OK;
+}
+
+// The shared-memory attribute of a kernel is per device: set once for each device used.
+template <typename K>
+int enc_allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    RAGRT_CUDA_TRY(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(done.load() & bit)) {
+        RAGRT_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        done.fetch_or(bit);
+    }
+    return RAGRT_OK;
+}
+
+// tcgen05 instruction-descriptor bits of an operand pair of type T (0 = fp16, 1 = bf16)
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_type() {
+    return std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+}
+constexpr uint32_t kIdescAMn = 1u << 15, kIdescBMn = 1u << 16;      // operand is MN-major
 
 // ------------------------------------------------------------------ 16-bit vectors
 template <typename T>

@@ -54,19 +54,6 @@ struct FfnParams {
     int* err;
 };
 
-// MN-major operand in 128-byte-swizzle atoms: 64 values of the row / column index side by side
-// (128 B), 8 contraction steps per 1024-byte group (stride byte offset); the next 64 row / column
-// values follow `mn_bytes` later (leading byte offset).
-__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t addr, uint32_t mn_bytes) {
-    uint64_t d = 0;
-    d |= (uint64_t)((addr >> 4) & 0x3FFF);
-    d |= (uint64_t)(mn_bytes >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
 
 // act(x); gelu's tanh form is x * sigmoid(2 u)
@@ -198,8 +185,8 @@ __global__ void __launch_bounds__(kFThreads, 1) ffn_mma(const __grid_constant__ 
                     const uint32_t a = tc::smem_u32(sA + s * kFTileA), bb = tc::smem_u32(sB + s * kFTileB);
 #pragma unroll
                     for (int k = 0; k < kFK / 16; ++k)
-                        tc::mma_ss(d, kAMn ? sw128_mnmajor_desc(a + 2048 * k, 8192) : tc::sw128_kmajor_desc(a + 32 * k),
-                                   kBMn ? sw128_mnmajor_desc(bb + 2048 * k, 8192) : tc::sw128_kmajor_desc(bb + 32 * k),
+                        tc::mma_ss(d, kAMn ? tc::sw128_mnmajor_desc(a + 2048 * k, 8192) : tc::sw128_kmajor_desc(a + 32 * k),
+                                   kBMn ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192) : tc::sw128_kmajor_desc(bb + 32 * k),
                                    idesc, (i | k) != 0 ? 1u : 0u);
                     tc::mma_commit(empty + s);
                     issued_g = g;

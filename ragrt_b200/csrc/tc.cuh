@@ -31,6 +31,20 @@ __device__ __forceinline__ uint64_t sw128_kmajor_desc(uint32_t addr) {
     return d;
 }
 
+// MN-major operand in 128-byte-swizzle atoms: 64 values of the row / column index side by side
+// (128 B), 8 contraction steps per 1024-byte group (stride byte offset); the next 64 row / column
+// values follow `mn_bytes` later (leading byte offset).  `addr` may be advanced by 2048 B per
+// 16 contraction steps.
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t addr, uint32_t mn_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((addr >> 4) & 0x3FFF);
+    d |= (uint64_t)(mn_bytes >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N) {
     return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
@@ -154,6 +168,14 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, int x, 
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
             "r"(smem_u32(dst)), "l"(tmap), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+// The same of a 3-D tensor.
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(smem_u32(dst)),
+        "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
 }
 // Asynchronous 16-byte copy global -> shared (per thread; completion per commit group).
