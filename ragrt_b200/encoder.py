@@ -148,33 +148,38 @@ _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 def _dtype16(*ts):
     """Type code of a call's 16-bit tensors (None for an absent one), which must agree."""
-    ts = [t for t in ts if t is not None]
-    if ts[0].dtype not in _DTYPES or any(t.dtype != ts[0].dtype for t in ts):
-        raise RuntimeError(f"the operands must all be fp16 or all bf16; got {[t.dtype for t in ts]}")
-    return _DTYPES[ts[0].dtype]
+    want = ts[0].dtype
+    for t in ts:
+        if t is not None and t.dtype is not want:
+            raise RuntimeError(f"the operands must all be fp16 or all bf16; got {want} and {t.dtype}")
+    if want not in _DTYPES:
+        raise RuntimeError(f"the operands must be fp16 or bf16; got {want}")
+    return _DTYPES[want]
 
 
-def _rows_ok(t):
-    """Whether [T, H, D] rows can be read in place: heads side by side, rows apart by a multiple of
-    16 bytes that holds them all, 16-byte aligned."""
+def _row_stride(t):
+    """Row stride in elements of [T, H, D] rows that can be used in place (heads side by side, rows
+    apart by a multiple of 16 bytes that holds them all, 16-byte aligned); 0 if they cannot."""
     T, H, D = t.shape
-    return ((t.stride(2) == 1 or D == 1) and (t.stride(1) == D or H <= 1) and t.data_ptr() % 16 == 0 and
-            (T <= 1 or (t.stride(0) >= H * D and t.stride(0) % 8 == 0)))
+    s = t.stride()
+    if (s[2] != 1 and D > 1) or (s[1] != D and H > 1) or t.data_ptr() & 15:
+        return 0
+    if T <= 1:
+        return H * D
+    return s[0] if s[0] >= H * D and not s[0] & 7 else 0
 
 
 def _rows(t):
-    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+    """(t, its row stride), or a copy of it where it cannot be read in place."""
+    s = _row_stride(t)
+    return (t, s) if s else (t.clone(memory_format=torch.contiguous_format), t.shape[1] * t.shape[2])
 
 
 def _solid(t):
     """Contiguous and 16-byte aligned (a copy where it is not)."""
-    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+    if t is None or (t.is_contiguous() and not t.data_ptr() & 15):
         return t
     return t.clone(memory_format=torch.contiguous_format)
-
-
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
 def _span(t):
@@ -198,22 +203,18 @@ def _overlap(a, b):
     return True
 
 
-def _same(a, b):
-    return a.data_ptr() == b.data_ptr() and _row_stride(a) == _row_stride(b) and a.shape == b.shape
-
-
-def _output(out, shape, like, inputs, in_place_of=None):
-    """`out` checked (shape, like's type, rows in place, apart from the inputs), or a new contiguous one."""
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    if out.shape != shape or out.dtype != like.dtype:
-        raise RuntimeError(f"out must be {tuple(shape)} {like.dtype}; got {tuple(out.shape)} {out.dtype}")
-    if not (_rows_ok(out) if out.dim() == 3 else out.is_contiguous() and out.data_ptr() % 16 == 0):
+def _check_output(out, shape, dtype, inputs, in_place_of=None):
+    """`out` has the shape and type, can be written in place and is apart from the inputs."""
+    if out.shape != shape or out.dtype != dtype:
+        raise RuntimeError(f"out must be {tuple(shape)} {dtype}; got {tuple(out.shape)} {out.dtype}")
+    if not (_row_stride(out) if out.dim() == 3 else out.is_contiguous() and not out.data_ptr() & 15):
         raise RuntimeError("out must be written in place: solid rows, 16-byte aligned, strides in multiples of 8")
     for t in inputs:
-        if t is not None and _overlap(out, t) and not (t is in_place_of and _same(out, t)):
-            raise RuntimeError("out overlaps an input")
-    return out
+        if not _overlap(out, t):
+            continue
+        if t is in_place_of and out.data_ptr() == t.data_ptr() and _row_stride(out) == _row_stride(t):
+            continue
+        raise RuntimeError("out overlaps an input")
 
 
 def packed_attention(q, k, v, cu_seqlens, causal=False, scale=None, out=None):
@@ -230,14 +231,18 @@ def packed_attention(q, k, v, cu_seqlens, causal=False, scale=None, out=None):
                            f"{tuple(v.shape)}")
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise RuntimeError("cu_seqlens must be int32 [B + 1]")
-    cu = cu_seqlens.to(torch.int32).contiguous()
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    if cu_seqlens.dtype is not torch.int32 or not cu_seqlens.is_contiguous():
+        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
     T, H, D = q.shape
-    out = _output(out, q.shape, q, (q, k, v))
+    if out is None:
+        out, os = q.new_empty((T, H, D)), H * D
+    else:
+        _check_output(out, q.shape, q.dtype, (q, k, v))
+        os = _row_stride(out)
     _lib.check(_lib.lib().ragrt_enc_packed_attention(
-        _ptr(q), _ptr(k), _ptr(v), _ptr(cu), _ptr(out), T, cu.shape[0] - 1, H, k.shape[1], D, _row_stride(q),
-        _row_stride(k), _row_stride(v), _row_stride(out), float(D ** -0.5 if scale is None else scale),
-        int(bool(causal)), dt, _stream()))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr(), T, cu_seqlens.shape[0] - 1, H,
+        k.shape[1], D, qs, ks, vs, os, D ** -0.5 if scale is None else scale, bool(causal), dt, _stream()))
     return out
 
 
@@ -253,21 +258,30 @@ def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise RuntimeError(f"q [T, H, D] and k [T, KV, D] wanted; got {tuple(q.shape)}, {tuple(k.shape)}")
     T, H, D = q.shape
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    KV = k.shape[1]
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise RuntimeError("cos and sin must be f32 [max_pos, R / 2]")
     if positions.shape != (T,) or positions.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"positions must be int32 or int64 [{T}]")
     for w in (q_weight, k_weight):
         if w is not None and w.shape != (D,):
             raise RuntimeError(f"a norm weight must be [{D}]; got {tuple(w.shape)}")
-    qi, ki = _rows(q), _rows(k)
+    (q, qs), (k, ks) = _rows(q), _rows(k)
     cos, sin, qw, kw, pos = _solid(cos), _solid(sin), _solid(q_weight), _solid(k_weight), positions.contiguous()
-    q_out = _output(q_out, q.shape, q, (qi, ki), in_place_of=qi)
-    k_out = _output(k_out, k.shape, k, (qi, ki, q_out), in_place_of=ki)
+    if q_out is None:
+        q_out, qos = q.new_empty((T, H, D)), H * D
+    else:
+        _check_output(q_out, q.shape, q.dtype, (q, k), in_place_of=q)
+        qos = _row_stride(q_out)
+    if k_out is None:
+        k_out, kos = k.new_empty((T, KV, D)), KV * D
+    else:
+        _check_output(k_out, k.shape, k.dtype, (q, k, q_out), in_place_of=k)
+        kos = _row_stride(k_out)
     _lib.check(_lib.lib().ragrt_enc_qk_norm_rope(
-        _ptr(qi), _ptr(ki), _ptr(qw), _ptr(kw), _ptr(cos), _ptr(sin), _ptr(pos), pos.element_size(), _ptr(q_out),
-        _ptr(k_out), T, H, k.shape[1], D, 2 * cos.shape[1], cos.shape[0], _row_stride(qi), _row_stride(ki),
-        _row_stride(q_out), _row_stride(k_out), float(eps), int(bool(interleaved)), dt, _stream()))
+        q.data_ptr(), k.data_ptr(), qw if qw is None else qw.data_ptr(), kw if kw is None else kw.data_ptr(),
+        cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), pos.element_size(), q_out.data_ptr(), k_out.data_ptr(), T, H,
+        KV, D, 2 * cos.shape[1], cos.shape[0], qs, ks, qos, kos, eps, bool(interleaved), dt, _stream()))
     return q_out, k_out
 
 
@@ -289,13 +303,17 @@ def gated_ffn(x, w_gate, w_up, act="silu", keep=False, out=None):
     dt = _dtype16(x, w_gate, w_up)
     M, F, K = _ffn_args(x, w_gate, w_up, act)
     x, wg, wu = _solid(x), _solid(w_gate), _solid(w_up)
-    h = _output(out, (M, F), x, (x, wg, wu))
+    if out is None:
+        out = x.new_empty((M, F))
+    else:
+        _check_output(out, (M, F), x.dtype, (x, wg, wu))
     gate = up = None
     if keep:
-        gate, up = x.new_empty(M, F), x.new_empty(M, F)
-    _lib.check(_lib.lib().ragrt_enc_gated_ffn(_ptr(x), _ptr(wg), _ptr(wu), _ptr(h), _ptr(gate), _ptr(up), M, F, K,
-                                              _ACTS[act], dt, _stream()))
-    return (h, gate, up) if keep else h
+        gate, up = x.new_empty((M, F)), x.new_empty((M, F))
+    _lib.check(_lib.lib().ragrt_enc_gated_ffn(
+        x.data_ptr(), wg.data_ptr(), wu.data_ptr(), out.data_ptr(), gate.data_ptr() if keep else None,
+        up.data_ptr() if keep else None, M, F, K, _ACTS[act], dt, _stream()))
+    return (out, gate, up) if keep else out
 
 
 def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu", need_dx=True, need_dw=True):
@@ -308,9 +326,9 @@ def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu", need_dx=True, 
         raise RuntimeError(f"dh, gate and up must be {(M, F)}; got {tuple(dh.shape)}, {tuple(gate.shape)}, "
                            f"{tuple(up.shape)}")
     dh, x, wg, wu, gate, up = (_solid(t) for t in (dh, x, w_gate, w_up, gate, up))
-    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
-    dx = torch.empty_like(x) if need_dx else None
-    dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_dw else (None, None)
+    dgate, dup = gate.new_empty((M, F)), up.new_empty((M, F))
+    dx = x.new_empty((M, K)) if need_dx else None
+    dwg, dwu = (wg.new_empty((F, K)), wu.new_empty((F, K))) if need_dw else (None, None)
     _lib.check(_lib.lib().ragrt_enc_gated_ffn_backward(
         _ptr(dh), _ptr(x), _ptr(wg), _ptr(wu), _ptr(gate), _ptr(up), _ptr(dgate), _ptr(dup), _ptr(dx), _ptr(dwg),
         _ptr(dwu), M, F, K, _ACTS[act], dt, _stream()))

@@ -19,7 +19,8 @@ RERANK_MODES = {"tc": 1, "wmma": 1, "simt": 0}
 
 
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # torch's current stream of the current device, without building a Stream object around it
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _ptr(t):
@@ -34,14 +35,15 @@ def _need_cuda(*ts):
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError("ragrt_b200 runs on CUDA tensors only (there is no CPU path)")
+        i = t.get_device()                                   # -1: not on a CUDA device
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"tensors of one call are on {dev} and {t.device}: all must be on one device")
-    if dev is not None and dev.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensors are on {dev} but the current device is cuda:{torch.cuda.current_device()}")
+            dev = i
+        if i < 0 or not t.is_cuda:
+            raise RuntimeError("ragrt_b200 runs on CUDA tensors only (there is no CPU path)")
+        if i != dev:
+            raise RuntimeError(f"tensors of one call are on cuda:{dev} and {t.device}: all must be on one device")
+    if dev is not None and dev != torch.cuda.current_device():
+        raise RuntimeError(f"tensors are on cuda:{dev} but the current device is cuda:{torch.cuda.current_device()}")
 
 
 def _c(t, dtype):
