@@ -31,7 +31,7 @@ struct AttnParams {
     void* out;
     const int32_t* cu;
     int64_t q_stride, k_stride, v_stride, out_stride;
-    int T, B, heads, kv_heads, dim, causal;
+    int T, B, heads, kv_heads, dim, causal, per_cta;
     float scale;
     int* err;
 };
@@ -61,30 +61,29 @@ __device__ __forceinline__ void attn_check_table(const AttnParams& p) {
     }
 }
 
-// One row of one head by one warp.  sq: dim floats of shared memory of this warp's own.
+// One row of one head by one warp.
 template <typename T>
-__device__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi, float* sq) {
+__device__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi) {
     const int lane = threadIdx.x & 31;
     const int g = h / (p.heads / p.kv_heads);
     const T* q = static_cast<const T*>(p.q) + t * p.q_stride + (int64_t)h * p.dim;
     const T* k = static_cast<const T*>(p.k) + (int64_t)g * p.dim;
     const T* v = static_cast<const T*>(p.v) + (int64_t)g * p.dim;
-    __syncwarp();
-    for (int d = lane; d < p.dim; d += 32) sq[d] = (float)q[d] * p.scale;
-    __syncwarp();
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};         // dims lane, lane + 32, ...
     for (int base = lo; base < hi; base += 32) {
         const int j = base + lane;
         float s = -INFINITY;
         if (j < hi) {
-            const uint4* kr = reinterpret_cast<const uint4*>(k + j * p.k_stride);
+            const T* kr = k + j * p.k_stride;
             s = 0.f;
-            for (int c = 0; c < p.dim / 8; ++c) {
-                float f[8];
-                up8<T>(__ldg(kr + c), f);
+            for (int c = 0; c < p.dim; c += 8) {
+                float f[8], a[8];
+                up8<T>(__ldg(reinterpret_cast<const uint4*>(kr + c)), f);
+                up8<T>(__ldg(reinterpret_cast<const uint4*>(q + c)), a);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s = fmaf(f[e], sq[8 * c + e], s);
+                for (int e = 0; e < 8; ++e) s = fmaf(f[e], a[e], s);
             }
+            s *= p.scale;
         }
         float mx = s;
 #pragma unroll
@@ -116,7 +115,11 @@ __device__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi, floa
 
 constexpr int kAM = 128;                       // rows per tile, keys per block
 constexpr int kATiles = 2;
-constexpr int kAThreads = 64 + kATiles * 128;  // TMA warp, MMA warp, four softmax warps per tile
+constexpr int kAFirst = 4;                    // first softmax warp: TMA, MMA and two idle warps before them
+constexpr int kAThreads = 32 * (kAFirst + 4 * kATiles);
+// The launch's 384 x 168 registers, dealt out anew: a softmax thread holds its row of 128 scores.
+constexpr int kARegsFew = 88, kARegsMany = 208;
+static_assert(128 * kARegsFew + 256 * kARegsMany <= kAThreads * 168, "more registers than the launch holds");
 constexpr uint32_t kAWaitLimit = 1u << 26;
 // The reference maximum of a row moves only when it is exceeded by 2^8: until then the weights are
 // at most 256, well inside either type, and the accumulator is not rescaled.
@@ -125,8 +128,9 @@ constexpr float kARescale = 8.0f;
 template <int DP>
 struct AttnCfg {
     static constexpr int kTile = kAM * DP * 2;                    // bytes of a Q tile, a K or a V block
+    static constexpr int kQ = DP == 128 ? 1 : 2;                  // heads whose Q is in shared memory
     static constexpr int kStages = DP == 128 ? 4 : 8;             // K and V blocks in flight
-    static constexpr int kSmem = 1024 + (kATiles + kStages) * kTile + 512;
+    static constexpr int kSmem = 1024 + (kQ * kATiles + kStages) * kTile + 512;
     static constexpr uint32_t kO = kATiles * kAM;                 // first accumulator column: S and P lie before
 };
 
@@ -139,21 +143,46 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// two fp32 values side by side, one instruction for both
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
     using Cfg = AttnCfg<DP>;
-    constexpr int S = Cfg::kStages;
+    constexpr int S = Cfg::kStages, NQ = Cfg::kQ;
     extern __shared__ uint8_t attn_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)attn_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sQ = sm;
-    uint8_t* sKV = sm + kATiles * Cfg::kTile;
+    uint8_t* sKV = sm + NQ * kATiles * Cfg::kTile;
     uint64_t* full = reinterpret_cast<uint64_t*>(sKV + S * Cfg::kTile);
     uint64_t* empty = full + S;
     uint64_t* qfull = empty + S;
-    uint64_t* sfull = qfull + 1;             // [2] scores ready (MMA -> softmax)
+    uint64_t* qempty = qfull + NQ;           // both tiles' last scores of a head are done
+    uint64_t* sfull = qempty + NQ;           // [2] scores ready (MMA -> softmax)
     uint64_t* pready = sfull + kATiles;      // [2] weights written (softmax -> MMA)
-    uint64_t* ofull = pready + kATiles;      // [2] last product done
+    uint64_t* ofull = pready + kATiles;      // [2] last product of a head done
     uint64_t* drain = ofull + kATiles;
     uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
@@ -161,17 +190,22 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
     int* swhi = swlo + 4 * kATiles;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // a CTA takes per_cta heads of its rows, one behind the other
+    const int shares = (p.heads + p.per_cta - 1) / p.per_cta;
+    const int h0 = (int)(blockIdx.x % shares) * p.per_cta, nh = min(p.per_cta, p.heads - h0);
     // the tiles of a causal sequence grow along it: the longest go first
     const int tiles = (p.T + kATiles * kAM - 1) / (kATiles * kAM);
-    const int h = blockIdx.x % p.heads;
-    const int row0 = (tiles - 1 - (int)(blockIdx.x / p.heads)) * kATiles * kAM;
+    const int row0 = (tiles - 1 - (int)(blockIdx.x / shares)) * kATiles * kAM;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             tc::mbar_init(full + s, 1);
             tc::mbar_init(empty + s, 1);
         }
-        tc::mbar_init(qfull, 1);
+        for (int s = 0; s < NQ; ++s) {
+            tc::mbar_init(qfull + s, 1);
+            tc::mbar_init(qempty + s, 1);
+        }
         tc::mbar_init(drain, 1);
         for (int t = 0; t < kATiles; ++t) {
             tc::mbar_init(sfull + t, 1);
@@ -187,16 +221,16 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
     }
     pdl_wait_then_release();
     attn_check_table(p);
-    const int tile = (warp - 2) >> 2, quad = warp & 3;
-    int lo = 0, hi = 0;
+    const int tile = (warp - kAFirst) >> 2, quad = warp & 3;
+    int lo = 0, hi = 0, wlo = 0, whi = 0;                         // this row's keys, and its warp's
     const int row = row0 + tile * kAM + quad * 32 + lane;         // of a softmax thread
-    if (warp >= 2) {
+    if (warp >= kAFirst) {
         attn_range(p, row, lo, hi);
-        const int wl = __reduce_min_sync(0xFFFFFFFFu, lo < hi ? lo : 0x7FFFFFFF);
-        const int wh = __reduce_max_sync(0xFFFFFFFFu, hi);
+        wlo = __reduce_min_sync(0xFFFFFFFFu, lo < hi ? lo : 0x7FFFFFFF);
+        whi = __reduce_max_sync(0xFFFFFFFFu, hi);
         if (lane == 0) {
-            swlo[warp - 2] = wl;
-            swhi[warp - 2] = wh;
+            swlo[warp - kAFirst] = wlo;
+            swhi[warp - kAFirst] = whi;
         }
     }
     tc::fence_before();
@@ -204,7 +238,7 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
     tc::fence_after();
     const uint32_t tbase = *tslot;
     // the keys that each tile walks, in blocks of 128 from the first key of either
-    int kv0 = 0x7FFFFFFF, kv1 = 0, jb[kATiles], je[kATiles];
+    int kv0 = 0x7FFFFFFF, jb[kATiles], je[kATiles];
 #pragma unroll
     for (int t = 0; t < kATiles; ++t) {
         jb[t] = 0x7FFFFFFF;
@@ -215,7 +249,6 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
             je[t] = max(je[t], swhi[4 * t + w]);
         }
         kv0 = min(kv0, jb[t]);
-        kv1 = max(kv1, je[t]);
     }
 #pragma unroll
     for (int t = 0; t < kATiles; ++t) {
@@ -223,33 +256,45 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
         jb[t] = any ? (jb[t] - kv0) / kAM : 0;
         je[t] = any ? (je[t] - kv0 + kAM - 1) / kAM : 0;
     }
-    const int n = max(je[0], je[1]);
+    const int n = max(je[0], je[1]);                              // blocks per head
     bool failed = false;
 
+    if (warp < kAFirst) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kARegsFew));
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
         if (lane == 0 && n > 0) {
-            const int g = h / (p.heads / p.kv_heads);
-            tc::mbar_arrive_expect_tx(qfull, kATiles * Cfg::kTile);
-            for (int t = 0; t < kATiles; ++t)
-                for (int c = 0; c < DP / 64; ++c)
-                    tc::tma_load_3d(sQ + t * Cfg::kTile + c * kAM * 128, &maps.q, 64 * c, h, row0 + t * kAM, qfull);
-            int i = 0;
-            for (; i < 2 * n; ++i) {                              // K0, V0, K1, V1, ...
-                const int s = i % S;
-                if (i >= S && !tc::mbar_wait_or_abort(empty + s, ((i / S) - 1) & 1, abort, kAWaitLimit)) {
+            const int per = p.heads / p.kv_heads;
+            int i = 0, hh = 0;
+            for (; hh < nh && !failed; ++hh) {
+                const int b = hh % NQ;
+                if (hh >= NQ && !tc::mbar_wait_or_abort(qempty + b, (hh / NQ - 1) & 1, abort, kAWaitLimit)) {
                     failed = true;
                     break;
                 }
-                tc::mbar_arrive_expect_tx(full + s, Cfg::kTile);
-                for (int c = 0; c < DP / 64; ++c)
-                    tc::tma_load_3d(sKV + s * Cfg::kTile + c * kAM * 128, i & 1 ? &maps.v : &maps.k, 64 * c, g,
-                                    kv0 + (i >> 1) * kAM, full + s);
+                tc::mbar_arrive_expect_tx(qfull + b, kATiles * Cfg::kTile);
+                for (int t = 0; t < kATiles; ++t)
+                    for (int c = 0; c < DP / 64; ++c)
+                        tc::tma_load_3d(sQ + (b * kATiles + t) * Cfg::kTile + c * kAM * 128, &maps.q, 64 * c, h0 + hh,
+                                        row0 + t * kAM, qfull + b);
+                const int g = (h0 + hh) / per;
+                for (int k = 0; k < 2 * n; ++k, ++i) {            // K0, V0, K1, V1, ...
+                    const int s = i % S;
+                    if (i >= S && !tc::mbar_wait_or_abort(empty + s, ((i / S) - 1) & 1, abort, kAWaitLimit)) {
+                        failed = true;
+                        break;
+                    }
+                    tc::mbar_arrive_expect_tx(full + s, Cfg::kTile);
+                    for (int c = 0; c < DP / 64; ++c)
+                        tc::tma_load_3d(sKV + s * Cfg::kTile + c * kAM * 128, k & 1 ? &maps.v : &maps.k, 64 * c, g,
+                                        kv0 + (k >> 1) * kAM, full + s);
+                }
             }
             if (failed) {                                         // copies in flight end before the CTA does
-                (void)tc::mbar_wait_bounded(qfull, 0, kAWaitLimit);
+                for (int k = max(0, hh - NQ); k < min(hh + 1, nh); ++k)
+                    (void)tc::mbar_wait_bounded(qfull + k % NQ, (k / NQ) & 1, 1u << 16);
                 for (int k = max(0, i - S); k < i; ++k)
-                    (void)tc::mbar_wait_bounded(full + k % S, (k / S) & 1, kAWaitLimit);
+                    (void)tc::mbar_wait_bounded(full + k % S, (k / S) & 1, 1u << 16);
             }
         }
     } else if (warp == 1) {
@@ -257,21 +302,31 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
         if (lane == 0 && n > 0) {
             constexpr uint32_t idS = tc::idesc_f16_f32(kAM, kAM) | idesc_type<T>();
             constexpr uint32_t idO = tc::idesc_f16_f32(kAM, DP) | idesc_type<T>() | kIdescBMn;
-            failed = !tc::mbar_wait_or_abort(qfull, 0, abort, kAWaitLimit);
-            for (int j = -1; j < n && !failed; ++j) {
-                const int vi = 2 * j + 1, ki = 2 * j + 2;
-                if (j >= 0) failed = !tc::mbar_wait_or_abort(full + vi % S, (vi / S) & 1, abort, kAWaitLimit);
-                if (!failed && j + 1 < n) failed = !tc::mbar_wait_or_abort(full + ki % S, (ki / S) & 1, abort, kAWaitLimit);
+            // step u: the product with V of block u, and the scores of block u + 1, over all heads' blocks
+            const int total = nh * n;
+            uint32_t pph[kATiles] = {0u, 0u};                     // pready phases used
+            int j = -1;                                           // u % n
+            for (int u = -1, hq = 0; u < total && !failed; ++u) {
+                const int vi = 2 * u + 1, ki = 2 * u + 2;
+                const int jn = j + 1 == n ? 0 : j + 1;            // block of u + 1, and
+                const bool next = u + 1 < total;                  // whether there is one
+                if (u >= 0) failed = !tc::mbar_wait_or_abort(full + vi % S, (vi / S) & 1, abort, kAWaitLimit);
+                if (!failed && next) failed = !tc::mbar_wait_or_abort(full + ki % S, (ki / S) & 1, abort, kAWaitLimit);
+                if (!failed && next && jn == 0) {                 // u + 1 begins head hq
+                    failed = !tc::mbar_wait_or_abort(qfull + hq % NQ, (hq / NQ) & 1, abort, kAWaitLimit);
+                    ++hq;
+                }
                 if (failed) break;
                 tc::fence_after();
                 const uint32_t v = tc::smem_u32(sKV + (vi % S) * Cfg::kTile), k = tc::smem_u32(sKV + (ki % S) * Cfg::kTile);
 #pragma unroll
                 for (int t = 0; t < kATiles; ++t) {
-                    if (j >= jb[t] && j < je[t]) {
-                        if (!tc::mbar_wait_or_abort(pready + t, (j - jb[t]) & 1, abort, kAWaitLimit)) {
+                    if (u >= 0 && j >= jb[t] && j < je[t]) {
+                        if (!tc::mbar_wait_or_abort(pready + t, pph[t] & 1, abort, kAWaitLimit)) {
                             failed = true;
                             break;
                         }
+                        ++pph[t];
                         tc::fence_after();
 #pragma unroll
                         for (int c = 0; c < kAM / 16; ++c)
@@ -279,10 +334,10 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
                                        tc::sw128_mnmajor_desc(v + 2048 * c, kAM * 128), idO, j > jb[t] || c > 0);
                         if (j == je[t] - 1) tc::mma_commit(ofull + t);
                     }
-                    if (j + 1 >= jb[t] && j + 1 < je[t]) {
+                    if (next && jn >= jb[t] && jn < je[t]) {
                         // S takes the columns of the P that the product just issued reads: the tensor
                         // pipe runs them one behind the other
-                        const uint32_t q = tc::smem_u32(sQ + t * Cfg::kTile);
+                        const uint32_t q = tc::smem_u32(sQ + (((hq - 1) % NQ) * kATiles + t) * Cfg::kTile);
 #pragma unroll
                         for (int c = 0; c < DP / 16; ++c) {
                             const uint32_t at = (c >> 2) * kAM * 128 + (c & 3) * 32;
@@ -293,113 +348,151 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
                     }
                 }
                 if (failed) break;
-                if (j >= 0) tc::mma_commit(empty + vi % S);
-                if (j + 1 < n) tc::mma_commit(empty + ki % S);
+                if (u >= 0) tc::mma_commit(empty + vi % S);
+                if (next) {
+                    tc::mma_commit(empty + ki % S);
+                    if (jn == n - 1) tc::mma_commit(qempty + (hq - 1) % NQ);
+                }
+                j = jn;
             }
             if (failed) {                                         // the last products read shared memory
                 tc::mma_commit(drain);
-                (void)tc::mbar_wait_bounded(drain, 0, kAWaitLimit);
+                (void)tc::mbar_wait_bounded(drain, 0, 1u << 16);
             }
         }
+    }
     } else {
         // ------------------------------------------------------------ softmax, a thread per row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kARegsMany));
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const uint32_t ts = tbase + lanes + (uint32_t)(tile * kAM), to = tbase + lanes + Cfg::kO + (uint32_t)(tile * DP);
         const float scale2 = p.scale * 1.4426950408889634f;       // weights are powers of two
+        const uint64_t scale22 = pack2(scale2, scale2);
         const int b0 = tile == 0 ? jb[0] : jb[1], b1 = tile == 0 ? je[0] : je[1];
-        float m = -INFINITY, l = 0.f;
-        for (int j = b0; j < b1; ++j) {
-            const bool ok = tc::mbar_wait_or_abort(sfull + tile, (j - b0) & 1, abort, kAWaitLimit);
-            if (!__all_sync(0xFFFFFFFFu, ok)) {
-                failed = true;
-                break;
-            }
-            tc::fence_after();
-            float s[128];
+        uint32_t sph = 0;
+        for (int hh = 0; hh < nh && b0 < b1 && !failed; ++hh) {
+            float m = -INFINITY, l = 0.f;
+            for (int j = b0; j < b1; ++j, ++sph) {
+                const bool ok = tc::mbar_wait_or_abort(sfull + tile, sph & 1, abort, kAWaitLimit);
+                if (!__all_sync(0xFFFFFFFFu, ok)) {
+                    failed = true;
+                    break;
+                }
+                tc::fence_after();
+                const int first = kv0 + j * kAM;
+                // most blocks lie inside every row's range; in the others, 32-key steps that no row of
+                // the warp sees are left out
+                const bool whole = __all_sync(0xFFFFFFFFu, lo <= first && first + kAM <= hi);
+                float s[128];
+                if (whole) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
-            tc::wait_ld();
-            const int first = kv0 + j * kAM;
-            if (!__all_sync(0xFFFFFFFFu, lo <= first && first + kAM <= hi)) {
-                const int c0 = lo - first, c1 = hi - first;
+                    for (int c = 0; c < 4; ++c) tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+                    tc::wait_ld();
+                } else {
+                    const int c0 = lo - first, c1 = hi - first;
 #pragma unroll
-                for (int c = 0; c < 128; ++c) s[c] = c >= c0 && c < c1 ? s[c] : -INFINITY;
-            }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
+                    for (int c = 0; c < 4; ++c) {
+                        if (first + 32 * c < whi && first + 32 * c + 32 > wlo) {
+                            tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+                            tc::wait_ld();
 #pragma unroll
-            for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-            const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
-            if (__any_sync(0xFFFFFFFFu, bm > m + kARescale)) {
-                // the scores of this block came behind the product with the last weights, so the
-                // accumulator is at rest
-                const float mn = fmaxf(m, bm);
-                const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
-                l *= alpha;
-                m = mn;
-                if (j > b0) {
-#pragma unroll 1
-                    for (int c = 0; c < DP / 32; ++c) {
-                        uint32_t r[32];
-                        tc::ld32x32(to + 32 * c, r);
-                        tc::wait_ld();
+                            for (int q = 32 * c; q < 32 * c + 32; ++q) s[q] = q >= c0 && q < c1 ? s[q] : -INFINITY;
+                        } else {
 #pragma unroll
-                        for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * alpha);
-                        tc::st32x32(to + 32 * c, r);
+                            for (int q = 32 * c; q < 32 * c + 32; ++q) s[q] = -INFINITY;
+                        }
                     }
                 }
-            }
-            const float ref = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                float mx[4];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t w[32];
+                for (int c = 0; c < 4; ++c) mx[c] = fmaxf(s[c], s[c + 4]);
 #pragma unroll
-                for (int q = 0; q < 32; ++q) {
-                    const float a = ex2(fmaf(s[64 * c + 2 * q], scale2, -ref));
-                    const float b = ex2(fmaf(s[64 * c + 2 * q + 1], scale2, -ref));
-                    sum[(2 * q) & 3] += a;
-                    sum[(2 * q + 1) & 3] += b;
-                    const typename Pair16<T>::type ab = Pair16<T>::down(a, b);
-                    w[q] = *reinterpret_cast<const uint32_t*>(&ab);
+                for (int c = 8; c < 128; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + e + 4]);
+                const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+                if (__any_sync(0xFFFFFFFFu, bm > m + kARescale)) {
+                    // the scores of this block came behind the product with the last weights, so the
+                    // accumulator is at rest
+                    const float mn = fmaxf(m, bm);
+                    const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+                    l *= alpha;
+                    m = mn;
+                    if (j > b0) {
+#pragma unroll 1
+                        for (int c = 0; c < DP / 32; ++c) {
+                            uint32_t r[32];
+                            tc::ld32x32(to + 32 * c, r);
+                            tc::wait_ld();
+#pragma unroll
+                            for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * alpha);
+                            tc::st32x32(to + 32 * c, r);
+                        }
+                    }
                 }
-                tc::st32x32(ts + 32 * c, w);
+                const float ref = m == -INFINITY ? 0.f : m;
+                const uint64_t ref2 = pack2(-ref, -ref);
+                uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+                    if (whole || (first + 32 * c < whi && first + 32 * c + 32 > wlo)) {
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) {
+                            float a, b;
+                            unpack2(fma2(pack2(s[32 * c + 2 * q], s[32 * c + 2 * q + 1]), scale22, ref2), a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                            sum[q & 1] = add2(sum[q & 1], pack2(a, b));
+                            const typename Pair16<T>::type ab = Pair16<T>::down(a, b);
+                            w[q] = *reinterpret_cast<const uint32_t*>(&ab);
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) w[q] = 0u;
+                    }
+                    tc::st32x16(ts + 16 * c, w);
+                }
+                float sa, sb;
+                unpack2(add2(sum[0], sum[1]), sa, sb);
+                l += sa + sb;
+                tc::wait_st();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(pready + tile);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tc::wait_st();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(pready + tile);
-        }
-        if (!failed && b1 > b0) {
-            const bool ok = tc::mbar_wait_or_abort(ofull + tile, 0, abort, kAWaitLimit);
-            failed = !__all_sync(0xFFFFFFFFu, ok);
-        }
-        if (!failed && b1 > b0) {
+            if (!failed) {
+                const bool ok = tc::mbar_wait_or_abort(ofull + tile, hh & 1, abort, kAWaitLimit);
+                failed = !__all_sync(0xFFFFFFFFu, ok);
+            }
+            if (failed) break;
             tc::fence_after();
+            // The next head's weights are announced behind these loads, so that its first product finds
+            // the accumulator read.
             const float inv = 1.0f / l;
+            const int h = h0 + hh;
+            const bool mine = lo < hi;
+            T* dst = static_cast<T*>(p.out) + row * p.out_stride + (int64_t)h * p.dim;
+            float odd = 0.f;
             float o[DP];
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) tc::ld32x32(to + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o + 32 * c));
             tc::wait_ld();
-            float odd = 0.f;
 #pragma unroll
             for (int c = 0; c < DP; ++c) {
                 o[c] *= inv;
                 odd = fmaf(o[c], 0.f, odd);                       // NaN as soon as one is not finite
             }
-            const bool mine = lo < hi, bad = mine && !(odd == 0.f);
+            const bool bad = mine && !(odd == 0.f);
             if (mine && !bad) {
-                T* dst = static_cast<T*>(p.out) + row * p.out_stride + (int64_t)h * p.dim;
 #pragma unroll
                 for (int c = 0; c < DP; c += 8)
                     if (c < p.dim) *reinterpret_cast<uint4*>(dst + c) = down8<T>(*reinterpret_cast<float(*)[8]>(o + c));
             }
-            // Q is no longer read by any product of this tile: its place serves attn_row
-            float* sq = reinterpret_cast<float*>(sQ + tile * Cfg::kTile) + 128 * ((warp - 2) & 3);
             for (unsigned left = __ballot_sync(0xFFFFFFFFu, bad); left; left &= left - 1) {
                 const int src = __ffs(left) - 1;
                 attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), h, __shfl_sync(0xFFFFFFFFu, lo, src),
-                            __shfl_sync(0xFFFFFFFFu, hi, src), sq);
+                            __shfl_sync(0xFFFFFFFFu, hi, src));
             }
         }
     }
@@ -413,7 +506,7 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
 }
 
 template <typename T, int DP>
-int attn_launch(int dtype, const AttnParams& p, cudaStream_t stream) {
+int attn_launch(int dtype, AttnParams p, cudaStream_t stream) {
     static std::atomic<uint64_t> done{0};
     int rc = enc_allow_smem(packed_attn_mma<T, DP>, AttnCfg<DP>::kSmem, done);
     if (rc) return rc;
@@ -422,7 +515,11 @@ int attn_launch(int dtype, const AttnParams& p, cudaStream_t stream) {
         (rc = enc_map_heads(&m.k, dtype, p.k, p.T, p.kv_heads, p.dim, p.k_stride, kAM)) ||
         (rc = enc_map_heads(&m.v, dtype, p.v, p.T, p.kv_heads, p.dim, p.v_stride, kAM)))
         return rc;
-    const int64_t blocks = ceil_div(p.T, kATiles * kAM) * p.heads;
+    // Several heads per CTA save its set-up (barriers, tensor memory, the bisection of the table), as
+    // long as eight CTAs remain for each SM to even out their lengths.
+    const int64_t pairs = ceil_div(p.T, kATiles * kAM);
+    p.per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(p.heads, pairs * p.heads / (8 * (int64_t)num_sms())));
+    const int64_t blocks = pairs * ceil_div(p.heads, p.per_cta);
     if (blocks > 0x7FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many rows x heads");
     return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)blocks), dim3(kAThreads), AttnCfg<DP>::kSmem, stream, m, p);
 }
@@ -458,7 +555,7 @@ extern "C" int ragrt_enc_packed_attention(const void* d_q, const void* d_k, cons
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
     AttnParams p{d_q, d_k, d_v, d_out, d_cu_seqlens, q_stride, k_stride, v_stride, out_stride, T, B, heads, kv_heads,
-                 head_dim, causal != 0, scale, err};
+                 head_dim, causal != 0, 1, scale, err};
     cudaStream_t stream = (cudaStream_t)stream_;
     if (dtype == RAGRT_BF16)
         return head_dim <= 64 ? attn_launch<__nv_bfloat16, 64>(dtype, p, stream)
