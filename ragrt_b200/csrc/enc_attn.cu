@@ -5,13 +5,15 @@
 // over the keys j of t's own sequence (with causal set: those up to t).  The sequences lie one behind
 // the other in the rows of q, k, v; cu_seqlens names where each begins.
 //
-//   packed_attn_mma    a CTA per 256 packed rows (two tiles of 128) and head.  The tiles run over the rows
-//                      as they lie, whatever sequences they belong to: a tile walks the keys of the
-//                      sequences that it touches, and each row masks what is not its own.  Short sequences
-//                      thus share a tile, and no tile is padded but the last.  Warp 0 streams Q and the
-//                      128-key blocks of K and V by TMA, warp 1 issues the products (S = Q K^T and
-//                      O += P V, P from tensor memory), and per tile four warps run the softmax, a
-//                      thread per row.
+//   packed_attn_mma    persistent; an item is 256 packed rows (two tiles of 128) of one head.  The tiles run
+//                      over the rows as they lie, whatever sequences they belong to: a tile walks the
+//                      keys of the sequences that it touches, and each row masks what is not its own.
+//                      Short sequences thus share a tile, and no tile is padded but the last.  Warp 0
+//                      streams Q and the 64-key blocks of K and V by TMA, warps 1 and 3 issue a tile's
+//                      products each (S = Q K^T and O += P V, P from tensor memory), warp 2 finds the
+//                      coming items' key ranges, and per tile four warps run the softmax, a thread per row.
+//                      Each tile has two score buffers, so that the scores of the block after next are
+//                      computed while a block's weights are: no role waits for a whole turn of another.
 //   attn_row           one row of one head by a warp, in fp32.  A weight of zero does not keep a NaN or
 //                      an infinity in a masked row of V out of a matrix product: rows that come out
 //                      of it not finite are computed once more by this, over their own keys alone.
@@ -31,35 +33,51 @@ struct AttnParams {
     void* out;
     const int32_t* cu;
     int64_t q_stride, k_stride, v_stride, out_stride;
-    int T, B, heads, kv_heads, dim, causal, per_cta;
+    int T, B, heads, kv_heads, dim, causal, items;
     float scale;
     int* err;
 };
 
-// The keys [lo, hi) that row t sees; empty for rows outside every sequence.  The last begin <= t is
-// found by bisection; what a table that is not ascending names outside [0, T] gives an empty range.
-__device__ __forceinline__ void attn_range(const AttnParams& p, int t, int& lo, int& hi) {
-    lo = hi = 0;
-    if (t >= p.T) return;
-    int a = 0, b = p.B;                              // cu[a] <= t (or a == 0), cu[b] > t (or b == B)
-    while (b - a > 1) {
-        const int m = (a + b) >> 1;
-        if (__ldg(p.cu + m) <= t) a = m; else b = m;
+// The keys [lo, hi) that rows t, t + 32, ... see; empty for rows outside every sequence.  The last begin
+// <= t is found by bisection, for N rows side by side; what a table that is not ascending names outside
+// [0, T] gives an empty range.
+template <int N>
+__device__ __forceinline__ void attn_ranges(const AttnParams& p, int t, int (&lo)[N], int (&hi)[N]) {
+    int a[N], b[N];                                  // cu[a] <= t (or a == 0), cu[b] > t (or b == B)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        a[i] = 0;
+        b[i] = p.B;
     }
-    const int begin = __ldg(p.cu + a), end = __ldg(p.cu + a + 1);
-    if (begin < 0 || end > p.T) return;              // a bad table
-    if (t < begin || t >= end) return;               // before the first or behind the last sequence
-    lo = begin;
-    hi = p.causal ? t + 1 : end;
+    for (int size = p.B; size > 1; size = (size + 1) >> 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int m = (a[i] + b[i]) >> 1;
+            if (b[i] - a[i] > 1) {
+                if (__ldg(p.cu + m) <= t + 32 * i) a[i] = m; else b[i] = m;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int row = t + 32 * i, begin = __ldg(p.cu + a[i]), end = __ldg(p.cu + a[i] + 1);
+        // behind T, a bad table, before the first or behind the last sequence
+        const bool none = row >= p.T || begin < 0 || end > p.T || row < begin || row >= end;
+        lo[i] = none ? 0 : begin;
+        hi[i] = none ? 0 : p.causal ? row + 1 : end;
+    }
 }
 
 // Every entry of the table is looked at by one thread of the grid: bisection alone does not see them all.
-__device__ __forceinline__ void attn_check_table(const AttnParams& p) {
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < p.B; i += (int64_t)gridDim.x * blockDim.x) {
+__device__ __forceinline__ void attn_check_table(const AttnParams& p, int lane) {
+    for (int64_t i = (int64_t)blockIdx.x * 32 + lane; i < p.B; i += (int64_t)gridDim.x * 32) {
         const int begin = __ldg(p.cu + i), end = __ldg(p.cu + i + 1);
         if (begin < 0 || end < begin || end > p.T) atomicExch(p.err, 6);
     }
 }
+
+// bits below n of a word, n of any size
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 
 // One row of one head by one warp.
 template <typename T>
@@ -113,29 +131,97 @@ __device__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi) {
         if (lane + 32 * c < p.dim) dst[lane + 32 * c] = (T)(o[c] / l);
 }
 
-constexpr int kAM = 128;                       // rows per tile, keys per block
+constexpr int kAM = 128;                       // rows per tile
+constexpr int kAN = 64;                        // keys per block
 constexpr int kATiles = 2;
-constexpr int kAFirst = 4;                    // first softmax warp: TMA, MMA and two idle warps before them
+constexpr int kAFirst = 4;                     // first softmax warp: TMA, two MMA and the range warp before them
 constexpr int kAThreads = 32 * (kAFirst + 4 * kATiles);
-// The launch's 384 x 168 registers, dealt out anew: a softmax thread holds its row of 128 scores.
+constexpr int kARanges = 4;                    // items whose key ranges are in shared memory
+constexpr uint32_t kAWaitLimit = 1u << 26;
+// The launch's 384 x 168 registers, dealt out anew: a softmax thread holds its row of scores.
 constexpr int kARegsFew = 88, kARegsMany = 208;
 static_assert(128 * kARegsFew + 256 * kARegsMany <= kAThreads * 168, "more registers than the launch holds");
-constexpr uint32_t kAWaitLimit = 1u << 26;
 // The reference maximum of a row moves only when it is exceeded by 2^8: until then the weights are
 // at most 256, well inside either type, and the accumulator is not rescaled.
 constexpr float kARescale = 8.0f;
 
 template <int DP>
 struct AttnCfg {
-    static constexpr int kTile = kAM * DP * 2;                    // bytes of a Q tile, a K or a V block
-    static constexpr int kQ = DP == 128 ? 1 : 2;                  // heads whose Q is in shared memory
-    static constexpr int kStages = DP == 128 ? 4 : 8;             // K and V blocks in flight
-    static constexpr int kSmem = 1024 + (kQ * kATiles + kStages) * kTile + 512;
-    static constexpr uint32_t kO = kATiles * kAM;                 // first accumulator column: S and P lie before
+    static constexpr int kTileQ = kAM * DP * 2;                   // bytes of a Q tile
+    static constexpr int kTileK = kAN * DP * 2;                   // bytes of a K or a V block
+    static constexpr int kQ = DP == 128 ? 1 : 2;                  // items whose Q is in shared memory
+    static constexpr int kStage = 2 * kTileK;                     // the V of a block, the K of the one after next
+    static constexpr int kStages = DP == 128 ? 4 : 6;
+    static constexpr int kShared = kARanges * 8 * kATiles * kAM + 1024;      // at least sizeof(AttnShared)
+    static constexpr int kSmem = 1024 + kQ * kATiles * kTileQ + kStages * kStage + kShared;
+    static constexpr uint32_t kO = 2 * kATiles * kAN;             // first accumulator column: S and P lie before
 };
 
 struct AttnMaps {
     CUtensorMap q, k, v;
+};
+
+// What the roles hand one another, behind the tiles in shared memory.
+template <int DP>
+struct AttnShared {
+    int lo[kARanges][kATiles * kAM], hi[kARanges][kATiles * kAM];     // keys [lo, hi) of each row
+    int tlo[kARanges][kATiles], thi[kARanges][kATiles];               // of each tile; [1, 0) where it has none
+    int row0[kARanges], head[kARanges];                               // row0 < 0: no more items
+    uint64_t full[AttnCfg<DP>::kStages], empty[AttnCfg<DP>::kStages];
+    uint64_t qfull[AttnCfg<DP>::kQ], qempty[AttnCfg<DP>::kQ];
+    uint64_t rfull[kARanges], rempty[kARanges];
+    uint64_t sfull[kATiles][2];              // scores ready (MMA -> softmax)
+    uint64_t pready[kATiles][2];             // weights written (softmax -> MMA)
+    uint64_t odone[kATiles][2];              // product with V done, even and odd blocks
+    uint64_t drain[kATiles];
+    uint32_t tmem;
+    int abort;
+};
+
+// The blocks of an item: 64-key blocks 0 .. n - 1 from key kv0 on, tile t takes [jb[t], je[t]) of them.
+struct AttnBlocks {
+    int row0 = -1, head, kv0, n = 0, jb[kATiles], je[kATiles];
+    __device__ __forceinline__ int lo(int t) const { return t == 0 ? jb[0] : jb[1]; }
+    __device__ __forceinline__ int hi(int t) const { return t == 0 ? je[0] : je[1]; }
+    template <int DP>
+    __device__ __forceinline__ void get(const AttnShared<DP>* sh, int r) {
+        row0 = sh->row0[r];
+        head = sh->head[r];
+        kv0 = 0x7FFFFFFF;
+        n = 0;
+#pragma unroll
+        for (int t = 0; t < kATiles; ++t)
+            if (sh->thi[r][t] > 0) kv0 = min(kv0, sh->tlo[r][t]);
+#pragma unroll
+        for (int t = 0; t < kATiles; ++t) {
+            const bool any = sh->thi[r][t] > 0;
+            jb[t] = any ? (sh->tlo[r][t] - kv0) / kAN : 0;
+            je[t] = any ? (sh->thi[r][t] - kv0 + kAN - 1) / kAN : 0;
+            n = max(n, je[t]);
+        }
+    }
+};
+
+// A walk of a thread or a whole warp over the blocks of its CTA's items.  The last of a role's walks
+// gives the items' ranges back behind itself (by the lane with `lead` set).
+template <int DP, bool kRelease>
+struct AttnWalk {
+    AttnBlocks b;
+    int rec = -1, j = 0;
+    bool lead = true;
+    // On to the next block; 1: there is one, 0: no more, -1: gave up waiting.
+    __device__ __forceinline__ int next(AttnShared<DP>* sh) {
+        if (j + 1 < b.n) {
+            ++j;
+            return 1;
+        }
+        if (kRelease && rec >= 0 && lead) tc::mbar_arrive(&sh->rempty[rec % kARanges]);
+        ++rec;
+        if (!tc::mbar_wait_or_abort(&sh->rfull[rec % kARanges], (rec / kARanges) & 1, &sh->abort, kAWaitLimit)) return -1;
+        b.get(sh, rec % kARanges);
+        j = 0;
+        return b.row0 >= 0;
+    }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -175,258 +261,318 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
     extern __shared__ uint8_t attn_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)attn_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sQ = sm;
-    uint8_t* sKV = sm + NQ * kATiles * Cfg::kTile;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sKV + S * Cfg::kTile);
-    uint64_t* empty = full + S;
-    uint64_t* qfull = empty + S;
-    uint64_t* qempty = qfull + NQ;           // both tiles' last scores of a head are done
-    uint64_t* sfull = qempty + NQ;           // [2] scores ready (MMA -> softmax)
-    uint64_t* pready = sfull + kATiles;      // [2] weights written (softmax -> MMA)
-    uint64_t* ofull = pready + kATiles;      // [2] last product of a head done
-    uint64_t* drain = ofull + kATiles;
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
-    volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
-    int* swlo = reinterpret_cast<int*>(tslot + 2);                // [8] key range of each softmax warp's rows
-    int* swhi = swlo + 4 * kATiles;
+    uint8_t* sKV = sm + NQ * kATiles * Cfg::kTileQ;
+    AttnShared<DP>* sh = reinterpret_cast<AttnShared<DP>*>(sKV + S * Cfg::kStage);
+    static_assert(sizeof(AttnShared<DP>) <= Cfg::kShared, "shared memory of the roles");
+    volatile int* abort = &sh->abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // a CTA takes per_cta heads of its rows, one behind the other
-    const int shares = (p.heads + p.per_cta - 1) / p.per_cta;
-    const int h0 = (int)(blockIdx.x % shares) * p.per_cta, nh = min(p.per_cta, p.heads - h0);
-    // the tiles of a causal sequence grow along it: the longest go first
-    const int tiles = (p.T + kATiles * kAM - 1) / (kATiles * kAM);
-    const int row0 = (tiles - 1 - (int)(blockIdx.x / shares)) * kATiles * kAM;
-
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
-            tc::mbar_init(full + s, 1);
-            tc::mbar_init(empty + s, 1);
+            tc::mbar_init(&sh->full[s], 1);
+            tc::mbar_init(&sh->empty[s], kATiles);
         }
         for (int s = 0; s < NQ; ++s) {
-            tc::mbar_init(qfull + s, 1);
-            tc::mbar_init(qempty + s, 1);
+            tc::mbar_init(&sh->qfull[s], 1);
+            tc::mbar_init(&sh->qempty[s], kATiles);
         }
-        tc::mbar_init(drain, 1);
+        for (int r = 0; r < kARanges; ++r) {
+            tc::mbar_init(&sh->rfull[r], 1);
+            tc::mbar_init(&sh->rempty[r], 1 + 5 * kATiles);       // TMA, MMA and softmax warps
+        }
         for (int t = 0; t < kATiles; ++t) {
-            tc::mbar_init(sfull + t, 1);
-            tc::mbar_init(pready + t, 4);
-            tc::mbar_init(ofull + t, 1);
+            tc::mbar_init(&sh->drain[t], 1);
+            for (int b = 0; b < 2; ++b) {
+                tc::mbar_init(&sh->sfull[t][b], 1);
+                tc::mbar_init(&sh->pready[t][b], 4);
+                tc::mbar_init(&sh->odone[t][b], 1);
+            }
         }
-        *abort = 0;
+        sh->abort = 0;
         tc::mbar_fence_init();
     }
     if (warp == 1) {
-        tc::tmem_alloc(tslot, 512);
+        tc::tmem_alloc(&sh->tmem, 512);
         tc::tmem_relinquish();
-    }
-    pdl_wait_then_release();
-    attn_check_table(p);
-    const int tile = (warp - kAFirst) >> 2, quad = warp & 3;
-    int lo = 0, hi = 0, wlo = 0, whi = 0;                         // this row's keys, and its warp's
-    const int row = row0 + tile * kAM + quad * 32 + lane;         // of a softmax thread
-    if (warp >= kAFirst) {
-        attn_range(p, row, lo, hi);
-        wlo = __reduce_min_sync(0xFFFFFFFFu, lo < hi ? lo : 0x7FFFFFFF);
-        whi = __reduce_max_sync(0xFFFFFFFFu, hi);
-        if (lane == 0) {
-            swlo[warp - kAFirst] = wlo;
-            swhi[warp - kAFirst] = whi;
-        }
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tbase = *tslot;
-    // the keys that each tile walks, in blocks of 128 from the first key of either
-    int kv0 = 0x7FFFFFFF, jb[kATiles], je[kATiles];
-#pragma unroll
-    for (int t = 0; t < kATiles; ++t) {
-        jb[t] = 0x7FFFFFFF;
-        je[t] = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            jb[t] = min(jb[t], swlo[4 * t + w]);
-            je[t] = max(je[t], swhi[4 * t + w]);
-        }
-        kv0 = min(kv0, jb[t]);
-    }
-#pragma unroll
-    for (int t = 0; t < kATiles; ++t) {
-        const bool any = je[t] > 0;
-        jb[t] = any ? (jb[t] - kv0) / kAM : 0;
-        je[t] = any ? (je[t] - kv0 + kAM - 1) / kAM : 0;
-    }
-    const int n = max(je[0], je[1]);                              // blocks per head
+    const uint32_t tbase = sh->tmem;
     bool failed = false;
+    pdl_wait_then_release();
 
     if (warp < kAFirst) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kARegsFew));
-    if (warp == 0) {
-        // ------------------------------------------------------------ TMA producer
-        if (lane == 0 && n > 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kARegsFew));
+        if (warp == 0 && lane == 0) {
+            // -------------------------------------------------------- TMA producer
+            // stage 0: K0; stage 1: K1; stage u + 2: the V of block u and the K of block u + 2, over all
+            // items' blocks
             const int per = p.heads / p.kv_heads;
-            int i = 0, hh = 0;
-            for (; hh < nh && !failed; ++hh) {
-                const int b = hh % NQ;
-                if (hh >= NQ && !tc::mbar_wait_or_abort(qempty + b, (hh / NQ - 1) & 1, abort, kAWaitLimit)) {
+            AttnWalk<DP, false> kw;
+            AttnWalk<DP, true> vw;
+            int pos = 0, nq = 0;
+            auto load = [&](const AttnBlocks& b, int j, const CUtensorMap* map, uint8_t* to, uint64_t* bar) {
+                for (int c = 0; c < DP / 64; ++c)
+                    tc::tma_load_3d(to + c * kAN * 128, map, 64 * c, b.head / per, b.kv0 + j * kAN, bar);
+            };
+            int k = 1;
+            for (; !failed; ++pos) {
+                if (k > 0) k = kw.next(sh);
+                const int v = pos < 2 ? 0 : vw.next(sh);
+                if (k < 0 || v < 0) failed = true;
+                if (failed || (pos >= 2 && v == 0)) break;
+                if (k == 0 && v == 0) {                           // fewer than two blocks in all: nothing to load
+                    if (pos == 0) break;
+                    continue;
+                }
+                const int s = pos % S;
+                if (pos >= S && !tc::mbar_wait_or_abort(&sh->empty[s], (pos / S - 1) & 1, abort, kAWaitLimit)) {
                     failed = true;
                     break;
                 }
-                tc::mbar_arrive_expect_tx(qfull + b, kATiles * Cfg::kTile);
-                for (int t = 0; t < kATiles; ++t)
-                    for (int c = 0; c < DP / 64; ++c)
-                        tc::tma_load_3d(sQ + (b * kATiles + t) * Cfg::kTile + c * kAM * 128, &maps.q, 64 * c, h0 + hh,
-                                        row0 + t * kAM, qfull + b);
-                const int g = (h0 + hh) / per;
-                for (int k = 0; k < 2 * n; ++k, ++i) {            // K0, V0, K1, V1, ...
-                    const int s = i % S;
-                    if (i >= S && !tc::mbar_wait_or_abort(empty + s, ((i / S) - 1) & 1, abort, kAWaitLimit)) {
+                uint8_t* at = sKV + s * Cfg::kStage;
+                tc::mbar_arrive_expect_tx(&sh->full[s], ((k > 0) + (v > 0)) * Cfg::kTileK);
+                if (v > 0) load(vw.b, vw.j, &maps.v, at + Cfg::kTileK, &sh->full[s]);
+                if (k > 0) load(kw.b, kw.j, &maps.k, at, &sh->full[s]);
+                if (k > 0 && kw.j == 0) {                         // a new item: its Q
+                    const int b = nq % NQ;
+                    if (nq >= NQ && !tc::mbar_wait_or_abort(&sh->qempty[b], (nq / NQ - 1) & 1, abort, kAWaitLimit)) {
                         failed = true;
                         break;
                     }
-                    tc::mbar_arrive_expect_tx(full + s, Cfg::kTile);
-                    for (int c = 0; c < DP / 64; ++c)
-                        tc::tma_load_3d(sKV + s * Cfg::kTile + c * kAM * 128, k & 1 ? &maps.v : &maps.k, 64 * c, g,
-                                        kv0 + (k >> 1) * kAM, full + s);
+                    tc::mbar_arrive_expect_tx(&sh->qfull[b], kATiles * Cfg::kTileQ);
+                    for (int t = 0; t < kATiles; ++t)
+                        for (int c = 0; c < DP / 64; ++c)
+                            tc::tma_load_3d(sQ + (b * kATiles + t) * Cfg::kTileQ + c * kAM * 128, &maps.q, 64 * c,
+                                            kw.b.head, kw.b.row0 + t * kAM, &sh->qfull[b]);
+                    ++nq;
                 }
             }
             if (failed) {                                         // copies in flight end before the CTA does
-                for (int k = max(0, hh - NQ); k < min(hh + 1, nh); ++k)
-                    (void)tc::mbar_wait_bounded(qfull + k % NQ, (k / NQ) & 1, 1u << 16);
-                for (int k = max(0, i - S); k < i; ++k)
-                    (void)tc::mbar_wait_bounded(full + k % S, (k / S) & 1, 1u << 16);
+                for (int i = max(0, nq - NQ); i < nq; ++i)
+                    (void)tc::mbar_wait_bounded(&sh->qfull[i % NQ], (i / NQ) & 1, 1u << 16);
+                for (int i = max(0, pos - S); i <= pos; ++i)
+                    (void)tc::mbar_wait_bounded(&sh->full[i % S], (i / S) & 1, 1u << 16);
             }
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer
-        if (lane == 0 && n > 0) {
-            constexpr uint32_t idS = tc::idesc_f16_f32(kAM, kAM) | idesc_type<T>();
+        } else if (warp == 1 || warp == 3) {
+            // -------------------------------------------------------- a tile's MMA issuer, one lane of a warp in step
+            constexpr uint32_t idS = tc::idesc_f16_f32(kAM, kAN) | idesc_type<T>();
             constexpr uint32_t idO = tc::idesc_f16_f32(kAM, DP) | idesc_type<T>() | kIdescBMn;
-            // step u: the product with V of block u, and the scores of block u + 1, over all heads' blocks
-            const int total = nh * n;
-            uint32_t pph[kATiles] = {0u, 0u};                     // pready phases used
-            int j = -1;                                           // u % n
-            for (int u = -1, hq = 0; u < total && !failed; ++u) {
-                const int vi = 2 * u + 1, ki = 2 * u + 2;
-                const int jn = j + 1 == n ? 0 : j + 1;            // block of u + 1, and
-                const bool next = u + 1 < total;                  // whether there is one
-                if (u >= 0) failed = !tc::mbar_wait_or_abort(full + vi % S, (vi / S) & 1, abort, kAWaitLimit);
-                if (!failed && next) failed = !tc::mbar_wait_or_abort(full + ki % S, (ki / S) & 1, abort, kAWaitLimit);
-                if (!failed && next && jn == 0) {                 // u + 1 begins head hq
-                    failed = !tc::mbar_wait_or_abort(qfull + hq % NQ, (hq / NQ) & 1, abort, kAWaitLimit);
-                    ++hq;
+            const int t = warp >> 1;
+            const uint32_t lead = tc::elect_one();
+            AttnWalk<DP, false> sw;                               // scores run two blocks ahead of
+            AttnWalk<DP, true> vw;                                // the products with V
+            vw.lead = lead != 0;
+            uint32_t ns = 0, nv = 0;                              // the tile's blocks begun
+            int nq = 0, more = 1;
+            for (int pos = 0;; ++pos) {
+                const int there = pos < 2 ? 0 : vw.next(sh);
+                if (more > 0) more = sw.next(sh);
+                if (!__all_sync(0xFFFFFFFFu, there >= 0 && more >= 0)) {
+                    failed = true;
+                    break;
                 }
-                if (failed) break;
-                tc::fence_after();
-                const uint32_t v = tc::smem_u32(sKV + (vi % S) * Cfg::kTile), k = tc::smem_u32(sKV + (ki % S) * Cfg::kTile);
-#pragma unroll
-                for (int t = 0; t < kATiles; ++t) {
-                    if (u >= 0 && j >= jb[t] && j < je[t]) {
-                        if (!tc::mbar_wait_or_abort(pready + t, pph[t] & 1, abort, kAWaitLimit)) {
-                            failed = true;
-                            break;
-                        }
-                        ++pph[t];
-                        tc::fence_after();
-#pragma unroll
-                        for (int c = 0; c < kAM / 16; ++c)
-                            tc::mma_ts(tbase + Cfg::kO + t * DP, tbase + t * kAM + 8 * c,
-                                       tc::sw128_mnmajor_desc(v + 2048 * c, kAM * 128), idO, j > jb[t] || c > 0);
-                        if (j == je[t] - 1) tc::mma_commit(ofull + t);
-                    }
-                    if (next && jn >= jb[t] && jn < je[t]) {
-                        // S takes the columns of the P that the product just issued reads: the tensor
-                        // pipe runs them one behind the other
-                        const uint32_t q = tc::smem_u32(sQ + (((hq - 1) % NQ) * kATiles + t) * Cfg::kTile);
-#pragma unroll
-                        for (int c = 0; c < DP / 16; ++c) {
-                            const uint32_t at = (c >> 2) * kAM * 128 + (c & 3) * 32;
-                            tc::mma_ss(tbase + t * kAM, tc::sw128_kmajor_desc(q + at), tc::sw128_kmajor_desc(k + at), idS,
-                                       c > 0);
-                        }
-                        tc::mma_commit(sfull + t);
-                    }
+                if (there == 0 && (pos >= 2 || more == 0)) {
+                    if (pos >= 2 || pos == 0) break;
+                    continue;
                 }
-                if (failed) break;
-                if (u >= 0) tc::mma_commit(empty + vi % S);
-                if (next) {
-                    tc::mma_commit(empty + ki % S);
-                    if (jn == n - 1) tc::mma_commit(qempty + (hq - 1) % NQ);
-                }
-                j = jn;
-            }
-            if (failed) {                                         // the last products read shared memory
-                tc::mma_commit(drain);
-                (void)tc::mbar_wait_bounded(drain, 0, 1u << 16);
-            }
-        }
-    }
-    } else {
-        // ------------------------------------------------------------ softmax, a thread per row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kARegsMany));
-        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const uint32_t ts = tbase + lanes + (uint32_t)(tile * kAM), to = tbase + lanes + Cfg::kO + (uint32_t)(tile * DP);
-        const float scale2 = p.scale * 1.4426950408889634f;       // weights are powers of two
-        const uint64_t scale22 = pack2(scale2, scale2);
-        const int b0 = tile == 0 ? jb[0] : jb[1], b1 = tile == 0 ? je[0] : je[1];
-        uint32_t sph = 0;
-        for (int hh = 0; hh < nh && b0 < b1 && !failed; ++hh) {
-            float m = -INFINITY, l = 0.f;
-            for (int j = b0; j < b1; ++j, ++sph) {
-                const bool ok = tc::mbar_wait_or_abort(sfull + tile, sph & 1, abort, kAWaitLimit);
+                const int stage = pos % S;
+                bool ok = tc::mbar_wait_or_abort(&sh->full[stage], (pos / S) & 1, abort, kAWaitLimit);
                 if (!__all_sync(0xFFFFFFFFu, ok)) {
                     failed = true;
                     break;
                 }
                 tc::fence_after();
-                const int first = kv0 + j * kAM;
-                // most blocks lie inside every row's range; in the others, 32-key steps that no row of
-                // the warp sees are left out
-                const bool whole = __all_sync(0xFFFFFFFFu, lo <= first && first + kAM <= hi);
-                float s[128];
-                if (whole) {
+                const uint32_t k = tc::smem_u32(sKV + stage * Cfg::kStage), v = k + Cfg::kTileK;
+                if (there > 0 && vw.j >= vw.b.lo(t) && vw.j < vw.b.hi(t)) {
+                    const uint32_t b = nv & 1u;
+                    ok = tc::mbar_wait_or_abort(&sh->pready[t][b], (nv >> 1) & 1, abort, kAWaitLimit);
+                    if (!__all_sync(0xFFFFFFFFu, ok)) {
+                        failed = true;
+                        break;
+                    }
+                    ++nv;
+                    tc::fence_after();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
-                    tc::wait_ld();
-                } else {
-                    const int c0 = lo - first, c1 = hi - first;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (first + 32 * c < whi && first + 32 * c + 32 > wlo) {
-                            tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
-                            tc::wait_ld();
-#pragma unroll
-                            for (int q = 32 * c; q < 32 * c + 32; ++q) s[q] = q >= c0 && q < c1 ? s[q] : -INFINITY;
-                        } else {
-#pragma unroll
-                            for (int q = 32 * c; q < 32 * c + 32; ++q) s[q] = -INFINITY;
+                    for (int c = 0; c < kAN / 16; ++c)
+                        tc::mma_ts_if(lead, tbase + Cfg::kO + t * DP, tbase + (2 * t + b) * kAN + 8 * c,
+                                      tc::sw128_mnmajor_desc(v + 2048 * c, kAN * 128), idO, vw.j > vw.b.lo(t) || c > 0);
+                    tc::mma_commit_if(lead, &sh->odone[t][b]);
+                }
+                if (more > 0) {
+                    if (sw.j == 0) {
+                        ok = tc::mbar_wait_or_abort(&sh->qfull[nq % NQ], (nq / NQ) & 1, abort, kAWaitLimit);
+                        if (!__all_sync(0xFFFFFFFFu, ok)) {
+                            failed = true;
+                            break;
                         }
+                        tc::fence_after();
+                    }
+                    if (sw.j >= sw.b.lo(t) && sw.j < sw.b.hi(t)) {
+                        // S takes the buffer whose weights the product just issued (or an earlier one)
+                        // reads: the tensor pipe runs them one behind the other
+                        const uint32_t q = tc::smem_u32(sQ + ((nq % NQ) * kATiles + t) * Cfg::kTileQ);
+                        const uint32_t b = ns & 1u;
+                        ++ns;
+#pragma unroll
+                        for (int c = 0; c < DP / 16; ++c)
+                            tc::mma_ss_if(lead, tbase + (2 * t + b) * kAN,
+                                          tc::sw128_kmajor_desc(q + (c >> 2) * kAM * 128 + (c & 3) * 32),
+                                          tc::sw128_kmajor_desc(k + (c >> 2) * kAN * 128 + (c & 3) * 32), idS, c > 0);
+                        tc::mma_commit_if(lead, &sh->sfull[t][b]);
+                    }
+                    if (sw.j == sw.b.n - 1) {
+                        tc::mma_commit_if(lead, &sh->qempty[nq % NQ]);
+                        ++nq;
                     }
                 }
-                float mx[4];
+                tc::mma_commit_if(lead, &sh->empty[stage]);
+            }
+            if (failed) {                                         // the last products read shared memory
+                tc::mma_commit_if(lead, &sh->drain[t]);
+                (void)tc::mbar_wait_bounded(&sh->drain[t], 0, 1u << 16);
+            }
+        } else if (warp == 2) {
+            // -------------------------------------------------------- the items' key ranges, 8 rows a lane
+            // This CTA's items: blockIdx.x, blockIdx.x + gridDim.x, ...; heads fastest, and the last rows
+            // first: the tiles of a causal sequence grow along it.  Items without a key are passed over.
+            constexpr int kRows = kATiles * kAM / 32;
+            const int pairs = (p.T + kATiles * kAM - 1) / (kATiles * kAM);
+            int lo[kRows], hi[kRows], tlo[kATiles], thi[kATiles], row0 = -1, rec = 0;
+            for (int64_t i = blockIdx.x; !failed; i += gridDim.x) {
+                const bool end = i >= p.items;
+                if (!end) {
+                    const int r0 = (pairs - 1 - (int)(i / p.heads)) * kATiles * kAM;
+                    if (r0 != row0) {
+                        row0 = r0;
+                        attn_ranges<kRows>(p, r0 + lane, lo, hi);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) mx[c] = fmaxf(s[c], s[c + 4]);
+                        for (int t = 0; t < kATiles; ++t) {
+                            tlo[t] = 0x7FFFFFFF;
+                            thi[t] = 0;
 #pragma unroll
-                for (int c = 8; c < 128; c += 8)
+                            for (int x = t * kRows / kATiles; x < (t + 1) * kRows / kATiles; ++x) {
+                                if (lo[x] < hi[x]) tlo[t] = min(tlo[t], lo[x]);
+                                thi[t] = max(thi[t], hi[x]);
+                            }
+                            tlo[t] = __reduce_min_sync(0xFFFFFFFFu, tlo[t]);
+                            thi[t] = __reduce_max_sync(0xFFFFFFFFu, thi[t]);
+                        }
+                    }
+                    if (max(thi[0], thi[1]) == 0) continue;
+                }
+                const int r = rec % kARanges;
+                const bool ok = rec < kARanges ||
+                                tc::mbar_wait_or_abort(&sh->rempty[r], (rec / kARanges - 1) & 1, abort, kAWaitLimit);
+                if (!__all_sync(0xFFFFFFFFu, ok)) {
+                    failed = true;
+                    break;
+                }
+                if (!end) {
+#pragma unroll
+                    for (int x = 0; x < kRows; ++x) {
+                        sh->lo[r][lane + 32 * x] = lo[x];
+                        sh->hi[r][lane + 32 * x] = hi[x];
+                    }
+                }
+                if (lane < kATiles) {
+                    sh->tlo[r][lane] = lane == 0 ? tlo[0] : tlo[1];
+                    sh->thi[r][lane] = end ? 0 : lane == 0 ? thi[0] : thi[1];
+                }
+                if (lane == 0) {
+                    sh->row0[r] = end ? -1 : row0;
+                    sh->head[r] = (int)(i % p.heads);
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sh->rfull[r]);
+                ++rec;
+                if (end) break;
+            }
+            attn_check_table(p, lane);
+        }
+    } else {
+        // ------------------------------------------------------------ softmax, a thread per row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kARegsMany));
+        const int tile = (warp - kAFirst) >> 2, quad = warp & 3;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const uint32_t ts = tbase + lanes + (uint32_t)(2 * tile * kAN), to = tbase + lanes + Cfg::kO + (uint32_t)(tile * DP);
+        const float scale2 = p.scale * 1.4426950408889634f;       // weights are powers of two
+        const uint64_t scale22 = pack2(scale2, scale2);
+        const int in_item = tile * kAM + quad * 32 + lane;
+        uint32_t blk = 0;                                         // blocks of this tile, over all items
+        for (int rec = 0; !failed; ++rec) {
+            const int r = rec % kARanges;
+            bool ok = tc::mbar_wait_or_abort(&sh->rfull[r], (rec / kARanges) & 1, abort, kAWaitLimit);
+            if (!__all_sync(0xFFFFFFFFu, ok)) {
+                failed = true;
+                break;
+            }
+            AttnBlocks b;
+            b.get(sh, r);
+            const int lo = sh->lo[r][in_item], hi = sh->hi[r][in_item];
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sh->rempty[r]);
+            if (b.row0 < 0) break;
+            const int b0 = b.lo(tile), b1 = b.hi(tile);
+            if (b0 >= b1) continue;
+            const int wlo = __reduce_min_sync(0xFFFFFFFFu, lo < hi ? lo : 0x7FFFFFFF);
+            const int whi = __reduce_max_sync(0xFFFFFFFFu, hi);
+            float m = -INFINITY, l = 0.f;
+            for (int j = b0; j < b1; ++j, ++blk) {
+                ok = tc::mbar_wait_or_abort(&sh->sfull[tile][blk & 1], (blk >> 1) & 1, abort, kAWaitLimit);
+                if (!__all_sync(0xFFFFFFFFu, ok)) {
+                    failed = true;
+                    break;
+                }
+                tc::fence_after();
+                const uint32_t tb = ts + (blk & 1) * kAN;
+                const int first = b.kv0 + j * kAN;
+                // most blocks lie inside every row's range; in the others, 32-key steps that no row of
+                // the warp sees are left out
+                const bool whole = __all_sync(0xFFFFFFFFu, lo <= first && first + kAN <= hi);
+                bool seen[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) seen[c] = whole || (first + 32 * c < whi && first + 32 * c + 32 > wlo);
+                float s[kAN];
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (seen[c]) tc::ld32x32(tb + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+                tc::wait_ld();
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (!whole) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t see = low_bits(hi - first - 32 * c) & ~low_bits(lo - first - 32 * c);
+#pragma unroll
+                        for (int q = 0; q < 32; ++q) s[32 * c + q] = (see >> q) & 1u ? s[32 * c + q] : -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < kAN; c += 8)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + e + 4]);
                 const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
                 if (__any_sync(0xFFFFFFFFu, bm > m + kARescale)) {
-                    // the scores of this block came behind the product with the last weights, so the
-                    // accumulator is at rest
                     const float mn = fmaxf(m, bm);
                     const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
                     l *= alpha;
                     m = mn;
-                    if (j > b0) {
+                    if (j > b0) {                                 // behind the product with the last weights
+                        ok = tc::mbar_wait_or_abort(&sh->odone[tile][(blk - 1) & 1], ((blk - 1) >> 1) & 1, abort, kAWaitLimit);
+                        if (!__all_sync(0xFFFFFFFFu, ok)) {
+                            failed = true;
+                            break;
+                        }
+                        tc::fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DP / 32; ++c) {
-                            uint32_t r[32];
-                            tc::ld32x32(to + 32 * c, r);
+                            uint32_t r32[32];
+                            tc::ld32x32(to + 32 * c, r32);
                             tc::wait_ld();
 #pragma unroll
-                            for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(__uint_as_float(r[q]) * alpha);
-                            tc::st32x32(to + 32 * c, r);
+                            for (int q = 0; q < 32; ++q) r32[q] = __float_as_uint(__uint_as_float(r32[q]) * alpha);
+                            tc::st32x32(to + 32 * c, r32);
                         }
                     }
                 }
@@ -434,47 +580,49 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
                 const uint64_t ref2 = pack2(-ref, -ref);
                 uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 2; ++c) {
                     uint32_t w[16];
-                    if (whole || (first + 32 * c < whi && first + 32 * c + 32 > wlo)) {
+                    if (seen[c]) {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) {
-                            float a, b;
-                            unpack2(fma2(pack2(s[32 * c + 2 * q], s[32 * c + 2 * q + 1]), scale22, ref2), a, b);
-                            a = ex2(a);
-                            b = ex2(b);
-                            sum[q & 1] = add2(sum[q & 1], pack2(a, b));
-                            const typename Pair16<T>::type ab = Pair16<T>::down(a, b);
-                            w[q] = *reinterpret_cast<const uint32_t*>(&ab);
+                            float x, y;
+                            unpack2(fma2(pack2(s[32 * c + 2 * q], s[32 * c + 2 * q + 1]), scale22, ref2), x, y);
+                            x = ex2(x);
+                            y = ex2(y);
+                            sum[q & 1] = add2(sum[q & 1], pack2(x, y));
+                            const typename Pair16<T>::type xy = Pair16<T>::down(x, y);
+                            w[q] = *reinterpret_cast<const uint32_t*>(&xy);
                         }
                     } else {
 #pragma unroll
                         for (int q = 0; q < 16; ++q) w[q] = 0u;
                     }
-                    tc::st32x16(ts + 16 * c, w);
+                    tc::st32x16(tb + 16 * c, w);
                 }
-                float sa, sb;
-                unpack2(add2(sum[0], sum[1]), sa, sb);
-                l += sa + sb;
+                float sx, sy;
+                unpack2(add2(sum[0], sum[1]), sx, sy);
+                l += sx + sy;
                 tc::wait_st();
                 tc::fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(pready + tile);
-            }
-            if (!failed) {
-                const bool ok = tc::mbar_wait_or_abort(ofull + tile, hh & 1, abort, kAWaitLimit);
-                failed = !__all_sync(0xFFFFFFFFu, ok);
+                if (lane == 0) tc::mbar_arrive(&sh->pready[tile][blk & 1]);
             }
             if (failed) break;
+            // the last product; the one two blocks before it came before this block's scores, so that the
+            // parity names it
+            ok = tc::mbar_wait_or_abort(&sh->odone[tile][(blk - 1) & 1], ((blk - 1) >> 1) & 1, abort, kAWaitLimit);
+            if (!__all_sync(0xFFFFFFFFu, ok)) {
+                failed = true;
+                break;
+            }
             tc::fence_after();
-            // The next head's weights are announced behind these loads, so that its first product finds
+            // The next item's weights are announced behind these loads, so that its first product finds
             // the accumulator read.
             const float inv = 1.0f / l;
-            const int h = h0 + hh;
             const bool mine = lo < hi;
-            T* dst = static_cast<T*>(p.out) + row * p.out_stride + (int64_t)h * p.dim;
-            float odd = 0.f;
-            float o[DP];
+            const int row = b.row0 + in_item;
+            T* dst = static_cast<T*>(p.out) + row * p.out_stride + (int64_t)b.head * p.dim;
+            float odd = 0.f, o[DP];
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) tc::ld32x32(to + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o + 32 * c));
             tc::wait_ld();
@@ -491,12 +639,12 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
             }
             for (unsigned left = __ballot_sync(0xFFFFFFFFu, bad); left; left &= left - 1) {
                 const int src = __ffs(left) - 1;
-                attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), h, __shfl_sync(0xFFFFFFFFu, lo, src),
+                attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), b.head, __shfl_sync(0xFFFFFFFFu, lo, src),
                             __shfl_sync(0xFFFFFFFFu, hi, src));
             }
         }
     }
-    if (failed && lane == 0) atomicExch(p.err, 1);
+    if (failed) atomicExch(p.err, 1);
     tc::fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -506,22 +654,17 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
 }
 
 template <typename T, int DP>
-int attn_launch(int dtype, AttnParams p, cudaStream_t stream) {
+int attn_launch(int dtype, const AttnParams& p, cudaStream_t stream) {
     static std::atomic<uint64_t> done{0};
     int rc = enc_allow_smem(packed_attn_mma<T, DP>, AttnCfg<DP>::kSmem, done);
     if (rc) return rc;
     AttnMaps m;
     if ((rc = enc_map_heads(&m.q, dtype, p.q, p.T, p.heads, p.dim, p.q_stride, kAM)) ||
-        (rc = enc_map_heads(&m.k, dtype, p.k, p.T, p.kv_heads, p.dim, p.k_stride, kAM)) ||
-        (rc = enc_map_heads(&m.v, dtype, p.v, p.T, p.kv_heads, p.dim, p.v_stride, kAM)))
+        (rc = enc_map_heads(&m.k, dtype, p.k, p.T, p.kv_heads, p.dim, p.k_stride, kAN)) ||
+        (rc = enc_map_heads(&m.v, dtype, p.v, p.T, p.kv_heads, p.dim, p.v_stride, kAN)))
         return rc;
-    // Several heads per CTA save its set-up (barriers, tensor memory, the bisection of the table), as
-    // long as eight CTAs remain for each SM to even out their lengths.
-    const int64_t pairs = ceil_div(p.T, kATiles * kAM);
-    p.per_cta = (int)std::max<int64_t>(1, std::min<int64_t>(p.heads, pairs * p.heads / (8 * (int64_t)num_sms())));
-    const int64_t blocks = pairs * ceil_div(p.heads, p.per_cta);
-    if (blocks > 0x7FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many rows x heads");
-    return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)blocks), dim3(kAThreads), AttnCfg<DP>::kSmem, stream, m, p);
+    return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)std::min(p.items, num_sms())), dim3(kAThreads),
+                      AttnCfg<DP>::kSmem, stream, m, p);
 }
 
 }  // namespace
@@ -537,6 +680,7 @@ extern "C" int ragrt_enc_packed_attention(const void* d_q, const void* d_k, cons
     RAGRT_REQUIRE(dtype == RAGRT_F16 || dtype == RAGRT_BF16, "dtype must be RAGRT_F16 or RAGRT_BF16; got %d",
                   (int)dtype);
     RAGRT_REQUIRE(T >= 0 && B >= 0, "T and B must be >= 0");
+    RAGRT_REQUIRE(T <= 0x7FFFFFFF - 1024, "too many rows");          // row numbers past the last tile stay in 32 bits
     RAGRT_REQUIRE(heads >= 1 && heads <= 65535 && kv_heads >= 1 && heads % kv_heads == 0,
                   "heads must be in [1, 65535] and a multiple of kv_heads (heads=%d kv_heads=%d)", (int)heads,
                   (int)kv_heads);
@@ -554,8 +698,10 @@ extern "C" int ragrt_enc_packed_attention(const void* d_q, const void* d_k, cons
                   "packed_attention operands must be 16-byte aligned");
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
+    const int64_t items = ceil_div(T, kATiles * kAM) * heads;
+    if (items > 0x7FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many rows x heads");
     AttnParams p{d_q, d_k, d_v, d_out, d_cu_seqlens, q_stride, k_stride, v_stride, out_stride, T, B, heads, kv_heads,
-                 head_dim, causal != 0, 1, scale, err};
+                 head_dim, causal != 0, (int)items, scale, err};
     cudaStream_t stream = (cudaStream_t)stream_;
     if (dtype == RAGRT_BF16)
         return head_dim <= 64 ? attn_launch<__nv_bfloat16, 64>(dtype, p, stream)
