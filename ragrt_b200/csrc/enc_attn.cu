@@ -5,15 +5,10 @@
 // over the keys j of t's own sequence (with causal set: those up to t).  The sequences lie one behind
 // the other in the rows of q, k, v; cu_seqlens names where each begins.
 //
-//   packed_attn_mma    persistent; an item is 256 packed rows (two tiles of 128) of one head.  The tiles run
-//                      over the rows as they lie, whatever sequences they belong to: a tile walks the
-//                      keys of the sequences that it touches, and each row masks what is not its own.
-//                      Short sequences thus share a tile, and no tile is padded but the last.  Warp 0
-//                      streams Q and the 64-key blocks of K and V by TMA, warps 1 and 3 issue a tile's
-//                      products each (S = Q K^T and O += P V, P from tensor memory), warp 2 finds the
-//                      coming items' key ranges, and per tile four warps run the softmax, a thread per row.
-//                      Each tile has two score buffers, so that the scores of the block after next are
-//                      computed while a block's weights are: no role waits for a whole turn of another.
+//   packed_attn_mma    persistent; an item is one or two tiles of 128 rows of a head, each tile of one sequence.
+//                      Warp 0 streams Q and the blocks of K and V by TMA, warp 1 issues the products
+//                      (S = Q K^T and O += P V, P from tensor memory), warp 2 finds the coming items'
+//                      sequences, and per tile four warps run the softmax, a thread per row.
 //   attn_row           one row of one head by a warp, in fp32.  A weight of zero does not keep a NaN or
 //                      an infinity in a masked row of V out of a matrix product: rows that come out
 //                      of it not finite are computed once more by this, over their own keys alone.
@@ -38,34 +33,41 @@ struct AttnParams {
     int* err;
 };
 
-// The keys [lo, hi) that rows t, t + 32, ... see; empty for rows outside every sequence.  The last begin
-// <= t is found by bisection, for N rows side by side; what a table that is not ascending names outside
-// [0, T] gives an empty range.
-template <int N>
-__device__ __forceinline__ void attn_ranges(const AttnParams& p, int t, int (&lo)[N], int (&hi)[N]) {
-    int a[N], b[N];                                  // cu[a] <= t (or a == 0), cu[b] > t (or b == B)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        a[i] = 0;
-        b[i] = p.B;
+constexpr int kAM = 128;                       // rows per tile
+
+// Where the tiles lie: sequence b has the slots floor(cu[b] / 128) + b on, one for each 128 of its rows.
+// A sequence's slots end where the next one's begin or one before, so that no sums over the sequences'
+// lengths are needed: a slot's sequence is the last one that begins at or before it.
+__device__ __forceinline__ int64_t attn_slot(int begin, int b) { return (int64_t)(begin >> 7) + b; }
+
+// The rows [row0, row0 + rows) of a slot and the keys [lo, hi) they see (the last row's, if causal); rows
+// = 0 for a slot without any.  By a whole warp: 32 entries of the table are looked at a time.  What a
+// table that is not ascending names outside [0, T] counts as none.
+struct AttnTile {
+    int row0, rows, lo, hi;
+};
+__device__ __forceinline__ AttnTile attn_tile(const AttnParams& p, int64_t slot, int lane) {
+    int b = 0, n = p.B;                              // the sequence is among b .. b + n - 1
+    bool any = true;
+    while (n > 1 && any) {
+        const int step = (n + 31) >> 5;
+        const int i = b + min(lane * step, n - 1);
+        const bool before = lane * step < n && attn_slot(__ldg(p.cu + i), i) <= slot;
+        const int k = __popc(__ballot_sync(0xFFFFFFFFu, before));
+        any = k > 0;
+        b += max(k - 1, 0) * step;
+        n = min(step, n - max(k - 1, 0) * step);
     }
-    for (int size = p.B; size > 1; size = (size + 1) >> 1) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int m = (a[i] + b[i]) >> 1;
-            if (b[i] - a[i] > 1) {
-                if (__ldg(p.cu + m) <= t + 32 * i) a[i] = m; else b[i] = m;
-            }
-        }
+    const int begin = __ldg(p.cu + b), end = __ldg(p.cu + b + 1);
+    const int64_t first = begin + (slot - attn_slot(begin, b)) * kAM;
+    AttnTile t{0, 0, 0, 0};
+    if (any && begin >= 0 && end <= p.T && first >= begin && first < end) {
+        t.row0 = (int)first;
+        t.rows = min(kAM, end - t.row0);
+        t.lo = begin;
+        t.hi = p.causal ? t.row0 + t.rows : end;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int row = t + 32 * i, begin = __ldg(p.cu + a[i]), end = __ldg(p.cu + a[i] + 1);
-        // behind T, a bad table, before the first or behind the last sequence
-        const bool none = row >= p.T || begin < 0 || end > p.T || row < begin || row >= end;
-        lo[i] = none ? 0 : begin;
-        hi[i] = none ? 0 : p.causal ? row + 1 : end;
-    }
+    return t;
 }
 
 // Every entry of the table is looked at by one thread of the grid: bisection alone does not see them all.
@@ -131,30 +133,33 @@ __device__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi) {
         if (lane + 32 * c < p.dim) dst[lane + 32 * c] = (T)(o[c] / l);
 }
 
-constexpr int kAM = 128;                       // rows per tile
-constexpr int kAN = 64;                        // keys per block
-constexpr int kATiles = 2;
-constexpr int kAFirst = 4;                     // first softmax warp: TMA, two MMA and the range warp before them
-constexpr int kAThreads = 32 * (kAFirst + 4 * kATiles);
-constexpr int kARanges = 4;                    // items whose key ranges are in shared memory
+constexpr int kAFirst = 4;                     // first softmax warp: TMA, MMA and search warp before them, one idle
+constexpr int kAItems = 4;                     // items whose tiles are in shared memory
 constexpr uint32_t kAWaitLimit = 1u << 26;
-// The launch's 384 x 168 registers, dealt out anew: a softmax thread holds its row of scores.
-constexpr int kARegsFew = 88, kARegsMany = 208;
-static_assert(128 * kARegsFew + 256 * kARegsMany <= kAThreads * 168, "more registers than the launch holds");
 // The reference maximum of a row moves only when it is exceeded by 2^8: until then the weights are
 // at most 256, well inside either type, and the accumulator is not rescaled.
 constexpr float kARescale = 8.0f;
 
+// Heads of up to 64: CTAs of one tile, four to an SM, so that the many short steps of short sequences
+// (loads, products, weights, stores) of one run while another's wait.  Wider heads: two tiles that share
+// K and V and take turns, one's products running while the other's weights are computed.
 template <int DP>
 struct AttnCfg {
+    static constexpr int kTiles = DP == 128 ? 2 : 1;
+    static constexpr int kCtas = DP == 128 ? 1 : 4;               // per SM
+    static constexpr int kThreads = 32 * (kAFirst + 4 * kTiles);
+    static constexpr int kN = DP == 128 ? 128 : 64;               // keys per block
+    static constexpr int kHalves = kN / 64;                       // a block's weights are announced 64 at a time
+    static constexpr bool kTwice = DP != 128;                     // scores are loaded again for the weights, not kept
     static constexpr int kTileQ = kAM * DP * 2;                   // bytes of a Q tile
-    static constexpr int kTileK = kAN * DP * 2;                   // bytes of a K or a V block
-    static constexpr int kQ = DP == 128 ? 1 : 2;                  // items whose Q is in shared memory
-    static constexpr int kStage = 2 * kTileK;                     // the V of a block, the K of the one after next
-    static constexpr int kStages = DP == 128 ? 4 : 6;
-    static constexpr int kShared = kARanges * 8 * kATiles * kAM + 1024;      // at least sizeof(AttnShared)
-    static constexpr int kSmem = 1024 + kQ * kATiles * kTileQ + kStages * kStage + kShared;
-    static constexpr uint32_t kO = 2 * kATiles * kAN;             // first accumulator column: S and P lie before
+    static constexpr int kTileK = kN * DP * 2;                    // bytes of a K or a V block
+    static constexpr int kStages = 2;                             // K blocks, and V blocks, in flight
+    static constexpr int kSmem = 1024 + kTiles * kTileQ + 2 * kStages * kTileK + 1024;
+    static constexpr uint32_t kO = kTiles * kN;                   // first accumulator column: S and P lie before
+    static constexpr uint32_t kCols = kO + kTiles * DP;           // tensor-memory columns
+    // The launch's registers, dealt out anew: a softmax thread holds its row of scores.
+    static constexpr int kRegs = DP == 128 ? 168 : 64, kRegsFew = DP == 128 ? 88 : 40, kRegsMany = DP == 128 ? 208 : 88;
+    static_assert(128 * kRegsFew + (kThreads - 128) * kRegsMany <= kThreads * kRegs, "more registers than the launch holds");
 };
 
 struct AttnMaps {
@@ -164,49 +169,46 @@ struct AttnMaps {
 // What the roles hand one another, behind the tiles in shared memory.
 template <int DP>
 struct AttnShared {
-    int lo[kARanges][kATiles * kAM], hi[kARanges][kATiles * kAM];     // keys [lo, hi) of each row
-    int tlo[kARanges][kATiles], thi[kARanges][kATiles];               // of each tile; [1, 0) where it has none
-    int row0[kARanges], head[kARanges];                               // row0 < 0: no more items
-    uint64_t full[AttnCfg<DP>::kStages], empty[AttnCfg<DP>::kStages];
-    uint64_t qfull[AttnCfg<DP>::kQ], qempty[AttnCfg<DP>::kQ];
-    uint64_t rfull[kARanges], rempty[kARanges];
-    uint64_t sfull[kATiles][2];              // scores ready (MMA -> softmax)
-    uint64_t pready[kATiles][2];             // weights written (softmax -> MMA)
-    uint64_t odone[kATiles][2];              // product with V done, even and odd blocks
-    uint64_t drain[kATiles];
+    static constexpr int kTiles = AttnCfg<DP>::kTiles, kStages = AttnCfg<DP>::kStages;
+    AttnTile tile[kAItems][kTiles];
+    int head[kAItems];                       // < 0: no more items
+    uint64_t kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
+    uint64_t qfull, qempty;
+    uint64_t ifull[kAItems], iempty[kAItems];
+    uint64_t sfull[kTiles];                  // scores ready (MMA -> softmax)
+    uint64_t pready[kTiles][AttnCfg<DP>::kHalves];       // weights written (softmax -> MMA)
+    uint64_t odone[kTiles];                  // product with V done
+    uint64_t drain;
     uint32_t tmem;
     int abort;
 };
 
-// The blocks of an item: 64-key blocks 0 .. n - 1 from key kv0 on, tile t takes [jb[t], je[t]) of them.
+// The blocks of an item: blocks 0 .. n - 1 from key kv0 on, tile t takes [jb[t], je[t]) of them.
+template <int DP>
 struct AttnBlocks {
-    int row0 = -1, head, kv0, n = 0, jb[kATiles], je[kATiles];
-    __device__ __forceinline__ int lo(int t) const { return t == 0 ? jb[0] : jb[1]; }
-    __device__ __forceinline__ int hi(int t) const { return t == 0 ? je[0] : je[1]; }
-    template <int DP>
+    int head = -1, kv0, n = 0, jb[AttnCfg<DP>::kTiles], je[AttnCfg<DP>::kTiles];
     __device__ __forceinline__ void get(const AttnShared<DP>* sh, int r) {
-        row0 = sh->row0[r];
         head = sh->head[r];
         kv0 = 0x7FFFFFFF;
         n = 0;
 #pragma unroll
-        for (int t = 0; t < kATiles; ++t)
-            if (sh->thi[r][t] > 0) kv0 = min(kv0, sh->tlo[r][t]);
+        for (int t = 0; t < AttnCfg<DP>::kTiles; ++t)
+            if (sh->tile[r][t].rows > 0) kv0 = min(kv0, sh->tile[r][t].lo);
 #pragma unroll
-        for (int t = 0; t < kATiles; ++t) {
-            const bool any = sh->thi[r][t] > 0;
-            jb[t] = any ? (sh->tlo[r][t] - kv0) / kAN : 0;
-            je[t] = any ? (sh->thi[r][t] - kv0 + kAN - 1) / kAN : 0;
+        for (int t = 0; t < AttnCfg<DP>::kTiles; ++t) {
+            const bool any = sh->tile[r][t].rows > 0;
+            jb[t] = any ? (unsigned)(sh->tile[r][t].lo - kv0) / AttnCfg<DP>::kN : 0;
+            je[t] = any ? (unsigned)(sh->tile[r][t].hi - kv0 + AttnCfg<DP>::kN - 1) / AttnCfg<DP>::kN : 0;
             n = max(n, je[t]);
         }
     }
 };
 
 // A walk of a thread or a whole warp over the blocks of its CTA's items.  The last of a role's walks
-// gives the items' ranges back behind itself (by the lane with `lead` set).
+// gives the items' records back behind itself (by the lane with `lead` set).
 template <int DP, bool kRelease>
 struct AttnWalk {
-    AttnBlocks b;
+    AttnBlocks<DP> b;
     int rec = -1, j = 0;
     bool lead = true;
     // On to the next block; 1: there is one, 0: no more, -1: gave up waiting.
@@ -215,12 +217,12 @@ struct AttnWalk {
             ++j;
             return 1;
         }
-        if (kRelease && rec >= 0 && lead) tc::mbar_arrive(&sh->rempty[rec % kARanges]);
+        if (kRelease && rec >= 0 && lead) tc::mbar_arrive(&sh->iempty[rec % kAItems]);
         ++rec;
-        if (!tc::mbar_wait_or_abort(&sh->rfull[rec % kARanges], (rec / kARanges) & 1, &sh->abort, kAWaitLimit)) return -1;
-        b.get(sh, rec % kARanges);
+        if (!tc::mbar_wait_or_abort(&sh->ifull[rec % kAItems], (rec / kAItems) & 1, &sh->abort, kAWaitLimit)) return -1;
+        b.get(sh, rec % kAItems);
         j = 0;
-        return b.row0 >= 0;
+        return b.head >= 0;
     }
 };
 
@@ -254,45 +256,64 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return v;
 }
 
+// w = 2^(s scale + ref) of 32 scores, packed in pairs; returns their sum.
+template <typename T>
+__device__ __forceinline__ float attn_weights(const float* s, uint64_t scale, uint64_t ref, uint32_t* w) {
+    uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        float x, y;
+        unpack2(fma2(pack2(s[2 * q], s[2 * q + 1]), scale, ref), x, y);
+        x = ex2(x);
+        y = ex2(y);
+        sum[q & 1] = add2(sum[q & 1], pack2(x, y));
+        const typename Pair16<T>::type xy = Pair16<T>::down(x, y);
+        w[q] = *reinterpret_cast<const uint32_t*>(&xy);
+    }
+    float x, y;
+    unpack2(add2(sum[0], sum[1]), x, y);
+    return x + y;
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
+__global__ void __launch_bounds__(AttnCfg<DP>::kThreads, AttnCfg<DP>::kCtas)
+packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
     using Cfg = AttnCfg<DP>;
-    constexpr int S = Cfg::kStages, NQ = Cfg::kQ;
+    constexpr int S = Cfg::kStages, N = Cfg::kN, kTiles = Cfg::kTiles;
     extern __shared__ uint8_t attn_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)attn_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sQ = sm;
-    uint8_t* sKV = sm + NQ * kATiles * Cfg::kTileQ;
-    AttnShared<DP>* sh = reinterpret_cast<AttnShared<DP>*>(sKV + S * Cfg::kStage);
-    static_assert(sizeof(AttnShared<DP>) <= Cfg::kShared, "shared memory of the roles");
+    uint8_t* sK = sm + kTiles * Cfg::kTileQ;
+    uint8_t* sV = sK + S * Cfg::kTileK;
+    AttnShared<DP>* sh = reinterpret_cast<AttnShared<DP>*>(sV + S * Cfg::kTileK);
+    static_assert(sizeof(AttnShared<DP>) <= 1024, "shared memory of the roles");
     volatile int* abort = &sh->abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
-            tc::mbar_init(&sh->full[s], 1);
-            tc::mbar_init(&sh->empty[s], kATiles);
+            tc::mbar_init(&sh->kfull[s], 1);
+            tc::mbar_init(&sh->vfull[s], 1);
+            tc::mbar_init(&sh->kempty[s], 1);
+            tc::mbar_init(&sh->vempty[s], 1);
         }
-        for (int s = 0; s < NQ; ++s) {
-            tc::mbar_init(&sh->qfull[s], 1);
-            tc::mbar_init(&sh->qempty[s], kATiles);
+        tc::mbar_init(&sh->qfull, 1);
+        tc::mbar_init(&sh->qempty, 1);
+        for (int r = 0; r < kAItems; ++r) {
+            tc::mbar_init(&sh->ifull[r], 1);
+            tc::mbar_init(&sh->iempty[r], 2 + 4 * kTiles);        // TMA, MMA and softmax warps
         }
-        for (int r = 0; r < kARanges; ++r) {
-            tc::mbar_init(&sh->rfull[r], 1);
-            tc::mbar_init(&sh->rempty[r], 1 + 5 * kATiles);       // TMA, MMA and softmax warps
+        for (int t = 0; t < kTiles; ++t) {
+            tc::mbar_init(&sh->sfull[t], 1);
+            for (int x = 0; x < Cfg::kHalves; ++x) tc::mbar_init(&sh->pready[t][x], 4);
+            tc::mbar_init(&sh->odone[t], 1);
         }
-        for (int t = 0; t < kATiles; ++t) {
-            tc::mbar_init(&sh->drain[t], 1);
-            for (int b = 0; b < 2; ++b) {
-                tc::mbar_init(&sh->sfull[t][b], 1);
-                tc::mbar_init(&sh->pready[t][b], 4);
-                tc::mbar_init(&sh->odone[t][b], 1);
-            }
-        }
+        tc::mbar_init(&sh->drain, 1);
         sh->abort = 0;
         tc::mbar_fence_init();
     }
     if (warp == 1) {
-        tc::tmem_alloc(&sh->tmem, 512);
+        tc::tmem_alloc(&sh->tmem, Cfg::kCols);
         tc::tmem_relinquish();
     }
     tc::fence_before();
@@ -303,189 +324,189 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
     pdl_wait_then_release();
 
     if (warp < kAFirst) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kARegsFew));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsFew));
         if (warp == 0 && lane == 0) {
             // -------------------------------------------------------- TMA producer
-            // stage 0: K0; stage 1: K1; stage u + 2: the V of block u and the K of block u + 2, over all
-            // items' blocks
+            // K blocks run one ahead of V blocks, over all items' blocks, as the products want them
             const int per = p.heads / p.kv_heads;
             AttnWalk<DP, false> kw;
             AttnWalk<DP, true> vw;
-            int pos = 0, nq = 0;
-            auto load = [&](const AttnBlocks& b, int j, const CUtensorMap* map, uint8_t* to, uint64_t* bar) {
+            int nk = 0, nv = 0, nq = 0, k = 1;
+            auto load = [&](const AttnBlocks<DP>& b, int j, int i, const CUtensorMap* map, uint8_t* ring, uint64_t* full,
+                            uint64_t* empty) {
+                const int s = i % S;
+                if (i >= S && !tc::mbar_wait_or_abort(empty + s, (i / S - 1) & 1, abort, kAWaitLimit)) return false;
+                tc::mbar_arrive_expect_tx(full + s, Cfg::kTileK);
                 for (int c = 0; c < DP / 64; ++c)
-                    tc::tma_load_3d(to + c * kAN * 128, map, 64 * c, b.head / per, b.kv0 + j * kAN, bar);
+                    tc::tma_load_3d(ring + s * Cfg::kTileK + c * N * 128, map, 64 * c, b.head / per, b.kv0 + j * N,
+                                    full + s);
+                return true;
             };
-            int k = 1;
-            for (; !failed; ++pos) {
-                if (k > 0) k = kw.next(sh);
-                const int v = pos < 2 ? 0 : vw.next(sh);
-                if (k < 0 || v < 0) failed = true;
-                if (failed || (pos >= 2 && v == 0)) break;
-                if (k == 0 && v == 0) {                           // fewer than two blocks in all: nothing to load
-                    if (pos == 0) break;
-                    continue;
+            for (int pos = 0; !failed; ++pos) {
+                if (pos > 0) {
+                    const int v = vw.next(sh);
+                    if (v == 0) break;
+                    failed = v < 0 || !load(vw.b, vw.j, nv, &maps.v, sV, sh->vfull, sh->vempty);
+                    if (failed) break;
+                    ++nv;
                 }
-                const int s = pos % S;
-                if (pos >= S && !tc::mbar_wait_or_abort(&sh->empty[s], (pos / S - 1) & 1, abort, kAWaitLimit)) {
+                if (k > 0) k = kw.next(sh);
+                if (k < 0) failed = true;
+                if (k <= 0) continue;
+                if (!load(kw.b, kw.j, nk, &maps.k, sK, sh->kfull, sh->kempty)) {
                     failed = true;
                     break;
                 }
-                uint8_t* at = sKV + s * Cfg::kStage;
-                tc::mbar_arrive_expect_tx(&sh->full[s], ((k > 0) + (v > 0)) * Cfg::kTileK);
-                if (v > 0) load(vw.b, vw.j, &maps.v, at + Cfg::kTileK, &sh->full[s]);
-                if (k > 0) load(kw.b, kw.j, &maps.k, at, &sh->full[s]);
-                if (k > 0 && kw.j == 0) {                         // a new item: its Q
-                    const int b = nq % NQ;
-                    if (nq >= NQ && !tc::mbar_wait_or_abort(&sh->qempty[b], (nq / NQ - 1) & 1, abort, kAWaitLimit)) {
+                ++nk;
+                if (kw.j == 0) {                                  // a new item: its Q
+                    if (nq > 0 && !tc::mbar_wait_or_abort(&sh->qempty, (nq - 1) & 1, abort, kAWaitLimit)) {
                         failed = true;
                         break;
                     }
-                    tc::mbar_arrive_expect_tx(&sh->qfull[b], kATiles * Cfg::kTileQ);
-                    for (int t = 0; t < kATiles; ++t)
+                    // rows of a tile behind its sequence are another's: read along and not used
+                    const int r = kw.rec % kAItems;
+                    tc::mbar_arrive_expect_tx(&sh->qfull, kTiles * Cfg::kTileQ);
+                    for (int t = 0; t < kTiles; ++t)
                         for (int c = 0; c < DP / 64; ++c)
-                            tc::tma_load_3d(sQ + (b * kATiles + t) * Cfg::kTileQ + c * kAM * 128, &maps.q, 64 * c,
-                                            kw.b.head, kw.b.row0 + t * kAM, &sh->qfull[b]);
+                            tc::tma_load_3d(sQ + t * Cfg::kTileQ + c * kAM * 128, &maps.q, 64 * c, kw.b.head,
+                                            sh->tile[r][t].row0, &sh->qfull);
                     ++nq;
                 }
             }
             if (failed) {                                         // copies in flight end before the CTA does
-                for (int i = max(0, nq - NQ); i < nq; ++i)
-                    (void)tc::mbar_wait_bounded(&sh->qfull[i % NQ], (i / NQ) & 1, 1u << 16);
-                for (int i = max(0, pos - S); i <= pos; ++i)
-                    (void)tc::mbar_wait_bounded(&sh->full[i % S], (i / S) & 1, 1u << 16);
+                if (nq > 0) (void)tc::mbar_wait_bounded(&sh->qfull, (nq - 1) & 1, 1u << 16);
+                for (int i = max(0, nk - S); i < nk; ++i)
+                    (void)tc::mbar_wait_bounded(&sh->kfull[i % S], (i / S) & 1, 1u << 16);
+                for (int i = max(0, nv - S); i < nv; ++i)
+                    (void)tc::mbar_wait_bounded(&sh->vfull[i % S], (i / S) & 1, 1u << 16);
             }
-        } else if (warp == 1 || warp == 3) {
-            // -------------------------------------------------------- a tile's MMA issuer, one lane of a warp in step
-            constexpr uint32_t idS = tc::idesc_f16_f32(kAM, kAN) | idesc_type<T>();
+        } else if (warp == 1) {
+            // -------------------------------------------------------- MMA issuer, one lane of a warp in step
+            constexpr uint32_t idS = tc::idesc_f16_f32(kAM, N) | idesc_type<T>();
             constexpr uint32_t idO = tc::idesc_f16_f32(kAM, DP) | idesc_type<T>() | kIdescBMn;
-            const int t = warp >> 1;
             const uint32_t lead = tc::elect_one();
-            AttnWalk<DP, false> sw;                               // scores run two blocks ahead of
+            AttnWalk<DP, false> sw;                               // scores run one block ahead of
             AttnWalk<DP, true> vw;                                // the products with V
             vw.lead = lead != 0;
-            uint32_t ns = 0, nv = 0;                              // the tile's blocks begun
-            int nq = 0, more = 1;
-            for (int pos = 0;; ++pos) {
-                const int there = pos < 2 ? 0 : vw.next(sh);
-                if (more > 0) more = sw.next(sh);
-                if (!__all_sync(0xFFFFFFFFu, there >= 0 && more >= 0)) {
-                    failed = true;
-                    break;
-                }
-                if (there == 0 && (pos >= 2 || more == 0)) {
-                    if (pos >= 2 || pos == 0) break;
-                    continue;
-                }
-                const int stage = pos % S;
-                bool ok = tc::mbar_wait_or_abort(&sh->full[stage], (pos / S) & 1, abort, kAWaitLimit);
-                if (!__all_sync(0xFFFFFFFFu, ok)) {
-                    failed = true;
-                    break;
-                }
-                tc::fence_after();
-                const uint32_t k = tc::smem_u32(sKV + stage * Cfg::kStage), v = k + Cfg::kTileK;
-                if (there > 0 && vw.j >= vw.b.lo(t) && vw.j < vw.b.hi(t)) {
-                    const uint32_t b = nv & 1u;
-                    ok = tc::mbar_wait_or_abort(&sh->pready[t][b], (nv >> 1) & 1, abort, kAWaitLimit);
-                    if (!__all_sync(0xFFFFFFFFu, ok)) {
-                        failed = true;
-                        break;
-                    }
-                    ++nv;
+            uint32_t np[kTiles] = {};                             // products of each tile
+            int nk = 0, nv = 0, nq = 0, more = 1;
+            auto scores = [&](int t) {
+                if (sw.j < sw.b.jb[t] || sw.j >= sw.b.je[t]) return;
+                // S takes the columns of the weights that the product just issued reads: the tensor pipe
+                // runs them one behind the other
+                const uint32_t q = tc::smem_u32(sQ + t * Cfg::kTileQ), k = tc::smem_u32(sK + (nk % S) * Cfg::kTileK);
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c)
+                    tc::mma_ss_if(lead, tbase + t * N, tc::sw128_kmajor_desc(q + (c >> 2) * kAM * 128 + (c & 3) * 32),
+                                  tc::sw128_kmajor_desc(k + (c >> 2) * N * 128 + (c & 3) * 32), idS, c > 0);
+                tc::mma_commit_if(lead, &sh->sfull[t]);
+            };
+            auto product = [&](int t) {
+                if (vw.j < vw.b.jb[t] || vw.j >= vw.b.je[t]) return true;
+                const uint32_t v = tc::smem_u32(sV + (nv % S) * Cfg::kTileK);
+                const bool begun = vw.j > vw.b.jb[t];
+#pragma unroll
+                for (int x = 0; x < Cfg::kHalves; ++x) {
+                    const bool ok = tc::mbar_wait_or_abort(&sh->pready[t][x], np[t] & 1, abort, kAWaitLimit);
+                    if (!__all_sync(0xFFFFFFFFu, ok)) return false;
                     tc::fence_after();
 #pragma unroll
-                    for (int c = 0; c < kAN / 16; ++c)
-                        tc::mma_ts_if(lead, tbase + Cfg::kO + t * DP, tbase + (2 * t + b) * kAN + 8 * c,
-                                      tc::sw128_mnmajor_desc(v + 2048 * c, kAN * 128), idO, vw.j > vw.b.lo(t) || c > 0);
-                    tc::mma_commit_if(lead, &sh->odone[t][b]);
+                    for (int c = 4 * x; c < 4 * x + 4; ++c)
+                        tc::mma_ts_if(lead, tbase + Cfg::kO + t * DP, tbase + t * N + 8 * c,
+                                      tc::sw128_mnmajor_desc(v + 2048 * c, N * 128), idO, begun || c > 0);
+                }
+                ++np[t];
+                if (vw.j == vw.b.je[t] - 1) tc::mma_commit_if(lead, &sh->odone[t]);
+                return true;
+            };
+            auto k_arrived = [&] {
+                const bool ok = tc::mbar_wait_or_abort(&sh->kfull[nk % S], (nk / S) & 1, abort, kAWaitLimit) &&
+                                (sw.j != 0 || tc::mbar_wait_or_abort(&sh->qfull, nq & 1, abort, kAWaitLimit));
+                if (!__all_sync(0xFFFFFFFFu, ok)) return false;
+                tc::fence_after();
+                return true;
+            };
+            for (int pos = 0;; ++pos) {
+                const int there = pos == 0 ? 0 : vw.next(sh);
+                if (more > 0) more = sw.next(sh);
+                failed = !__all_sync(0xFFFFFFFFu, there >= 0 && more >= 0);
+                if (failed || there + more == 0) break;
+                // Where the scores want a new Q, which may still be on its way, they come behind all
+                // products; else each tile's follow its product, which also keeps two tiles in turns:
+                // one's products run while the other's weights are computed.
+                const bool apart = more > 0 && sw.j == 0;
+                if (there > 0) {
+                    const bool ok = tc::mbar_wait_or_abort(&sh->vfull[nv % S], (nv / S) & 1, abort, kAWaitLimit);
+                    failed = !__all_sync(0xFFFFFFFFu, ok) || (more > 0 && !apart && !k_arrived());
+                    if (failed) break;
+                    tc::fence_after();
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        failed = failed || !product(t);
+                        if (!failed && more > 0 && !apart) scores(t);
+                    }
+                    if (failed) break;
+                    tc::mma_commit_if(lead, &sh->vempty[nv % S]);
+                    ++nv;
                 }
                 if (more > 0) {
-                    if (sw.j == 0) {
-                        ok = tc::mbar_wait_or_abort(&sh->qfull[nq % NQ], (nq / NQ) & 1, abort, kAWaitLimit);
-                        if (!__all_sync(0xFFFFFFFFu, ok)) {
-                            failed = true;
-                            break;
-                        }
-                        tc::fence_after();
-                    }
-                    if (sw.j >= sw.b.lo(t) && sw.j < sw.b.hi(t)) {
-                        // S takes the buffer whose weights the product just issued (or an earlier one)
-                        // reads: the tensor pipe runs them one behind the other
-                        const uint32_t q = tc::smem_u32(sQ + ((nq % NQ) * kATiles + t) * Cfg::kTileQ);
-                        const uint32_t b = ns & 1u;
-                        ++ns;
+                    if (apart) {
+                        failed = !k_arrived();
+                        if (failed) break;
 #pragma unroll
-                        for (int c = 0; c < DP / 16; ++c)
-                            tc::mma_ss_if(lead, tbase + (2 * t + b) * kAN,
-                                          tc::sw128_kmajor_desc(q + (c >> 2) * kAM * 128 + (c & 3) * 32),
-                                          tc::sw128_kmajor_desc(k + (c >> 2) * kAN * 128 + (c & 3) * 32), idS, c > 0);
-                        tc::mma_commit_if(lead, &sh->sfull[t][b]);
+                        for (int t = 0; t < kTiles; ++t) scores(t);
                     }
+                    tc::mma_commit_if(lead, &sh->kempty[nk % S]);
+                    ++nk;
                     if (sw.j == sw.b.n - 1) {
-                        tc::mma_commit_if(lead, &sh->qempty[nq % NQ]);
+                        tc::mma_commit_if(lead, &sh->qempty);
                         ++nq;
                     }
                 }
-                tc::mma_commit_if(lead, &sh->empty[stage]);
             }
             if (failed) {                                         // the last products read shared memory
-                tc::mma_commit_if(lead, &sh->drain[t]);
-                (void)tc::mbar_wait_bounded(&sh->drain[t], 0, 1u << 16);
+                tc::mma_commit_if(lead, &sh->drain);
+                (void)tc::mbar_wait_bounded(&sh->drain, 0, 1u << 16);
             }
         } else if (warp == 2) {
-            // -------------------------------------------------------- the items' key ranges, 8 rows a lane
-            // This CTA's items: blockIdx.x, blockIdx.x + gridDim.x, ...; heads fastest, and the last rows
-            // first: the tiles of a causal sequence grow along it.  Items without a key are passed over.
-            constexpr int kRows = kATiles * kAM / 32;
-            const int pairs = (p.T + kATiles * kAM - 1) / (kATiles * kAM);
-            int lo[kRows], hi[kRows], tlo[kATiles], thi[kATiles], row0 = -1, rec = 0;
-            for (int64_t i = blockIdx.x; !failed; i += gridDim.x) {
-                const bool end = i >= p.items;
+            // -------------------------------------------------------- the coming items
+            // Heads fastest, and the last rows first: the tiles of a causal sequence grow along it.  The
+            // CTAs take a round of items in one order and the next in the other, so that none always
+            // gets a round's longest.  Items without a row are passed over.
+            const int groups = p.items / p.heads;
+            int rec = 0, group = -1;
+            AttnTile tile[kTiles];
+            bool any = false;
+            for (int round = 0; !failed; ++round) {
+                const int64_t i = (int64_t)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                const bool end = (int64_t)round * gridDim.x >= p.items;
                 if (!end) {
-                    const int r0 = (pairs - 1 - (int)(i / p.heads)) * kATiles * kAM;
-                    if (r0 != row0) {
-                        row0 = r0;
-                        attn_ranges<kRows>(p, r0 + lane, lo, hi);
+                    if (i >= p.items) continue;
+                    const int g = groups - 1 - (int)(i / p.heads);
+                    if (g != group) {
+                        group = g;
+                        any = false;
 #pragma unroll
-                        for (int t = 0; t < kATiles; ++t) {
-                            tlo[t] = 0x7FFFFFFF;
-                            thi[t] = 0;
-#pragma unroll
-                            for (int x = t * kRows / kATiles; x < (t + 1) * kRows / kATiles; ++x) {
-                                if (lo[x] < hi[x]) tlo[t] = min(tlo[t], lo[x]);
-                                thi[t] = max(thi[t], hi[x]);
-                            }
-                            tlo[t] = __reduce_min_sync(0xFFFFFFFFu, tlo[t]);
-                            thi[t] = __reduce_max_sync(0xFFFFFFFFu, thi[t]);
+                        for (int t = 0; t < kTiles; ++t) {
+                            tile[t] = attn_tile(p, (int64_t)g * kTiles + t, lane);
+                            any = any || tile[t].rows > 0;
                         }
                     }
-                    if (max(thi[0], thi[1]) == 0) continue;
+                    if (!any) continue;
                 }
-                const int r = rec % kARanges;
-                const bool ok = rec < kARanges ||
-                                tc::mbar_wait_or_abort(&sh->rempty[r], (rec / kARanges - 1) & 1, abort, kAWaitLimit);
+                const int r = rec % kAItems;
+                const bool ok = rec < kAItems ||
+                                tc::mbar_wait_or_abort(&sh->iempty[r], (rec / kAItems - 1) & 1, abort, kAWaitLimit);
                 if (!__all_sync(0xFFFFFFFFu, ok)) {
                     failed = true;
                     break;
                 }
-                if (!end) {
-#pragma unroll
-                    for (int x = 0; x < kRows; ++x) {
-                        sh->lo[r][lane + 32 * x] = lo[x];
-                        sh->hi[r][lane + 32 * x] = hi[x];
-                    }
-                }
-                if (lane < kATiles) {
-                    sh->tlo[r][lane] = lane == 0 ? tlo[0] : tlo[1];
-                    sh->thi[r][lane] = end ? 0 : lane == 0 ? thi[0] : thi[1];
-                }
                 if (lane == 0) {
-                    sh->row0[r] = end ? -1 : row0;
-                    sh->head[r] = (int)(i % p.heads);
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) sh->tile[r][t] = end ? AttnTile{0, 0, 0, 0} : tile[t];
+                    sh->head[r] = end ? -1 : (int)(i % p.heads);
+                    tc::mbar_arrive(&sh->ifull[r]);
                 }
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&sh->rfull[r]);
                 ++rec;
                 if (end) break;
             }
@@ -493,78 +514,100 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
         }
     } else {
         // ------------------------------------------------------------ softmax, a thread per row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kARegsMany));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsMany));
         const int tile = (warp - kAFirst) >> 2, quad = warp & 3;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const uint32_t ts = tbase + lanes + (uint32_t)(2 * tile * kAN), to = tbase + lanes + Cfg::kO + (uint32_t)(tile * DP);
+        const uint32_t ts = tbase + lanes + (uint32_t)(tile * N), to = tbase + lanes + Cfg::kO + (uint32_t)(tile * DP);
         const float scale2 = p.scale * 1.4426950408889634f;       // weights are powers of two
         const uint64_t scale22 = pack2(scale2, scale2);
-        const int in_item = tile * kAM + quad * 32 + lane;
-        uint32_t blk = 0;                                         // blocks of this tile, over all items
+        uint32_t blk = 0, outs = 0;                               // blocks and items of this tile
         for (int rec = 0; !failed; ++rec) {
-            const int r = rec % kARanges;
-            bool ok = tc::mbar_wait_or_abort(&sh->rfull[r], (rec / kARanges) & 1, abort, kAWaitLimit);
+            const int r = rec % kAItems;
+            bool ok = tc::mbar_wait_or_abort(&sh->ifull[r], (rec / kAItems) & 1, abort, kAWaitLimit);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 failed = true;
                 break;
             }
-            AttnBlocks b;
+            AttnBlocks<DP> b;
             b.get(sh, r);
-            const int lo = sh->lo[r][in_item], hi = sh->hi[r][in_item];
+            const AttnTile own = sh->tile[r][tile];
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&sh->rempty[r]);
-            if (b.row0 < 0) break;
-            const int b0 = b.lo(tile), b1 = b.hi(tile);
-            if (b0 >= b1) continue;
-            const int wlo = __reduce_min_sync(0xFFFFFFFFu, lo < hi ? lo : 0x7FFFFFFF);
-            const int whi = __reduce_max_sync(0xFFFFFFFFu, hi);
+            if (lane == 0) tc::mbar_arrive(&sh->iempty[r]);
+            if (b.head < 0) break;
+            if (own.rows == 0) continue;
+            const int in_tile = quad * 32 + lane, row = own.row0 + in_tile;
+            const bool mine = in_tile < own.rows, idle = quad * 32 >= own.rows;      // idle: no row of the warp
+            const int hi = p.causal ? min(row + 1, own.hi) : own.hi;
+            const int wlast = p.causal ? min(own.row0 + quad * 32 + 32, own.hi) : own.hi;      // keys some row sees
+            const int wall = p.causal ? min(own.row0 + quad * 32 + 1, own.hi) : own.hi;        // keys all rows see
             float m = -INFINITY, l = 0.f;
+            const int b0 = tile == 0 ? b.jb[0] : b.jb[kTiles - 1], b1 = tile == 0 ? b.je[0] : b.je[kTiles - 1];
             for (int j = b0; j < b1; ++j, ++blk) {
-                ok = tc::mbar_wait_or_abort(&sh->sfull[tile][blk & 1], (blk >> 1) & 1, abort, kAWaitLimit);
+                ok = tc::mbar_wait_or_abort(&sh->sfull[tile], blk & 1, abort, kAWaitLimit);
                 if (!__all_sync(0xFFFFFFFFu, ok)) {
                     failed = true;
                     break;
                 }
                 tc::fence_after();
-                const uint32_t tb = ts + (blk & 1) * kAN;
-                const int first = b.kv0 + j * kAN;
-                // most blocks lie inside every row's range; in the others, 32-key steps that no row of
-                // the warp sees are left out
-                const bool whole = __all_sync(0xFFFFFFFFu, lo <= first && first + kAN <= hi);
-                bool seen[2];
+                const int first = b.kv0 + j * N;
+                // 32-key steps: all rows see all of it, some see some of it, or none sees any (left out)
+                bool full[N / 32], seen[N / 32];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) seen[c] = whole || (first + 32 * c < whi && first + 32 * c + 32 > wlo);
-                float s[kAN];
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    if (seen[c]) tc::ld32x32(tb + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
-                tc::wait_ld();
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (!whole) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const uint32_t see = low_bits(hi - first - 32 * c) & ~low_bits(lo - first - 32 * c);
-#pragma unroll
-                        for (int q = 0; q < 32; ++q) s[32 * c + q] = (see >> q) & 1u ? s[32 * c + q] : -INFINITY;
-                    }
+                for (int c = 0; c < N / 32; ++c) {
+                    full[c] = first + 32 * c >= own.lo && first + 32 * c + 32 <= wall;
+                    seen[c] = !idle && first + 32 * c + 32 > own.lo && first + 32 * c < wlast;
                 }
+                auto load = [&](int c, float* v) {
+                    tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v));
+                    tc::wait_ld();
+                    if (!full[c]) {
+                        const uint32_t see = low_bits(hi - first - 32 * c) & ~low_bits(own.lo - first - 32 * c);
 #pragma unroll
-                for (int c = 0; c < kAN; c += 8)
+                        for (int q = 0; q < 32; ++q) v[q] = (see >> q) & 1u ? v[q] : -INFINITY;
+                    }
+                };
+                float s[Cfg::kTwice ? 32 : N];
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (Cfg::kTwice) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + e + 4]);
+                    for (int c = 0; c < N / 32; ++c) {
+                        if (seen[c]) {
+                            load(c, s);
+#pragma unroll
+                            for (int q = 0; q < 32; q += 8)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[q + e], s[q + e + 4]);
+                        }
+                    }
+                } else {
+                    if (!idle && first >= own.lo && first + N <= wall) {
+#pragma unroll
+                        for (int c = 0; c < N / 32; ++c)
+                            tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+                        tc::wait_ld();
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < N / 32; ++c) {
+                            if (seen[c]) {
+                                load(c, s + 32 * c);
+                            } else {
+#pragma unroll
+                                for (int q = 0; q < 32; ++q) s[32 * c + q] = -INFINITY;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < N; c += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + e + 4]);
+                }
                 const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
                 if (__any_sync(0xFFFFFFFFu, bm > m + kARescale)) {
                     const float mn = fmaxf(m, bm);
                     const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
                     l *= alpha;
                     m = mn;
-                    if (j > b0) {                                 // behind the product with the last weights
-                        ok = tc::mbar_wait_or_abort(&sh->odone[tile][(blk - 1) & 1], ((blk - 1) >> 1) & 1, abort, kAWaitLimit);
-                        if (!__all_sync(0xFFFFFFFFu, ok)) {
-                            failed = true;
-                            break;
-                        }
-                        tc::fence_after();
+                    if (j > b0) {       // these scores came behind the last product: the accumulator is at rest
 #pragma unroll 1
                         for (int c = 0; c < DP / 32; ++c) {
                             uint32_t r32[32];
@@ -578,49 +621,37 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
                 const uint64_t ref2 = pack2(-ref, -ref);
-                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[16];
-                    if (seen[c]) {
+                for (int x = 0; x < Cfg::kHalves; ++x) {
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            float x, y;
-                            unpack2(fma2(pack2(s[32 * c + 2 * q], s[32 * c + 2 * q + 1]), scale22, ref2), x, y);
-                            x = ex2(x);
-                            y = ex2(y);
-                            sum[q & 1] = add2(sum[q & 1], pack2(x, y));
-                            const typename Pair16<T>::type xy = Pair16<T>::down(x, y);
-                            w[q] = *reinterpret_cast<const uint32_t*>(&xy);
+                    for (int c = 2 * x; c < 2 * x + 2; ++c) {
+                        uint32_t w[16];
+                        if (seen[c]) {
+                            if (Cfg::kTwice) load(c, s);
+                            l += attn_weights<T>(s + (Cfg::kTwice ? 0 : 32 * c), scale22, ref2, w);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) w[q] = 0u;
                         }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) w[q] = 0u;
+                        tc::st32x16(ts + 16 * c, w);
                     }
-                    tc::st32x16(tb + 16 * c, w);
+                    tc::wait_st();
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&sh->pready[tile][x]);
                 }
-                float sx, sy;
-                unpack2(add2(sum[0], sum[1]), sx, sy);
-                l += sx + sy;
-                tc::wait_st();
-                tc::fence_before();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&sh->pready[tile][blk & 1]);
             }
             if (failed) break;
-            // the last product; the one two blocks before it came before this block's scores, so that the
-            // parity names it
-            ok = tc::mbar_wait_or_abort(&sh->odone[tile][(blk - 1) & 1], ((blk - 1) >> 1) & 1, abort, kAWaitLimit);
+            ok = tc::mbar_wait_or_abort(&sh->odone[tile], outs++ & 1, abort, kAWaitLimit);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 failed = true;
                 break;
             }
+            if (idle) continue;
             tc::fence_after();
             // The next item's weights are announced behind these loads, so that its first product finds
             // the accumulator read.
             const float inv = 1.0f / l;
-            const bool mine = lo < hi;
-            const int row = b.row0 + in_item;
             T* dst = static_cast<T*>(p.out) + row * p.out_stride + (int64_t)b.head * p.dim;
             float odd = 0.f, o[DP];
 #pragma unroll
@@ -639,8 +670,7 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
             }
             for (unsigned left = __ballot_sync(0xFFFFFFFFu, bad); left; left &= left - 1) {
                 const int src = __ffs(left) - 1;
-                attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), b.head, __shfl_sync(0xFFFFFFFFu, lo, src),
-                            __shfl_sync(0xFFFFFFFFu, hi, src));
+                attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), b.head, own.lo, __shfl_sync(0xFFFFFFFFu, hi, src));
             }
         }
     }
@@ -649,22 +679,25 @@ __global__ void __launch_bounds__(kAThreads, 1) packed_attn_mma(const __grid_con
     __syncthreads();
     if (warp == 1) {
         tc::fence_after();
-        tc::tmem_dealloc(tbase, 512);
+        tc::tmem_dealloc(tbase, Cfg::kCols);
     }
 }
 
 template <typename T, int DP>
-int attn_launch(int dtype, const AttnParams& p, cudaStream_t stream) {
+int attn_launch(int dtype, AttnParams p, cudaStream_t stream) {
     static std::atomic<uint64_t> done{0};
     int rc = enc_allow_smem(packed_attn_mma<T, DP>, AttnCfg<DP>::kSmem, done);
     if (rc) return rc;
     AttnMaps m;
     if ((rc = enc_map_heads(&m.q, dtype, p.q, p.T, p.heads, p.dim, p.q_stride, kAM)) ||
-        (rc = enc_map_heads(&m.k, dtype, p.k, p.T, p.kv_heads, p.dim, p.k_stride, kAN)) ||
-        (rc = enc_map_heads(&m.v, dtype, p.v, p.T, p.kv_heads, p.dim, p.v_stride, kAN)))
+        (rc = enc_map_heads(&m.k, dtype, p.k, p.T, p.kv_heads, p.dim, p.k_stride, AttnCfg<DP>::kN)) ||
+        (rc = enc_map_heads(&m.v, dtype, p.v, p.T, p.kv_heads, p.dim, p.v_stride, AttnCfg<DP>::kN)))
         return rc;
-    return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)std::min(p.items, num_sms())), dim3(kAThreads),
-                      AttnCfg<DP>::kSmem, stream, m, p);
+    const int64_t groups = ceil_div(p.T / kAM + (int64_t)p.B, AttnCfg<DP>::kTiles);
+    if (groups * p.heads > 0x7FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many rows x heads");
+    p.items = (int)(groups * p.heads);
+    return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)std::min(p.items, num_sms() * AttnCfg<DP>::kCtas)),
+                      dim3(AttnCfg<DP>::kThreads), AttnCfg<DP>::kSmem, stream, m, p);
 }
 
 }  // namespace
@@ -698,10 +731,8 @@ extern "C" int ragrt_enc_packed_attention(const void* d_q, const void* d_k, cons
                   "packed_attention operands must be 16-byte aligned");
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
-    const int64_t items = ceil_div(T, kATiles * kAM) * heads;
-    if (items > 0x7FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many rows x heads");
     AttnParams p{d_q, d_k, d_v, d_out, d_cu_seqlens, q_stride, k_stride, v_stride, out_stride, T, B, heads, kv_heads,
-                 head_dim, causal != 0, (int)items, scale, err};
+                 head_dim, causal != 0, 0, scale, err};
     cudaStream_t stream = (cudaStream_t)stream_;
     if (dtype == RAGRT_BF16)
         return head_dim <= 64 ? attn_launch<__nv_bfloat16, 64>(dtype, p, stream)
