@@ -83,7 +83,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 
 
 // One row of one head by one warp.
 template <typename T>
-__device__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi) {
+__device__ __noinline__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi) {
     const int lane = threadIdx.x & 31;
     const int g = h / (p.heads / p.kv_heads);
     const T* q = static_cast<const T*>(p.q) + t * p.q_stride + (int64_t)h * p.dim;
@@ -136,7 +136,7 @@ __device__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi) {
 constexpr int kAFirst = 4;                     // first softmax warp: TMA, MMA and search warp before them, one idle
 constexpr int kAItems = 4;                     // items whose tiles are in shared memory
 constexpr uint32_t kAWaitLimit = 1u << 26;
-// The reference maximum of a row moves only when it is exceeded by 2^8: until then the weights are
+// The reference maximum of a row moves only when it is exceeded by a factor of 2^8: until then the weights are
 // at most 256, well inside either type, and the accumulator is not rescaled.
 constexpr float kARescale = 8.0f;
 
@@ -150,7 +150,7 @@ struct AttnCfg {
     static constexpr int kThreads = 32 * (kAFirst + 4 * kTiles);
     static constexpr int kN = DP == 128 ? 128 : 64;               // keys per block
     static constexpr int kHalves = kN / 64;                       // a block's weights are announced 64 at a time
-    static constexpr bool kTwice = DP != 128;                     // scores are loaded again for the weights, not kept
+    static constexpr bool kSteps = DP != 128;                     // a row's scores are held 32 at a time, not a block's
     static constexpr int kTileQ = kAM * DP * 2;                   // bytes of a Q tile
     static constexpr int kTileK = kN * DP * 2;                    // bytes of a K or a V block
     static constexpr int kStages = 2;                             // K blocks, and V blocks, in flight
@@ -277,7 +277,7 @@ __device__ __forceinline__ float attn_weights(const float* s, uint64_t scale, ui
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(AttnCfg<DP>::kThreads, AttnCfg<DP>::kCtas)
-packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
+packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
     using Cfg = AttnCfg<DP>;
     constexpr int S = Cfg::kStages, N = Cfg::kN, kTiles = Cfg::kTiles;
     extern __shared__ uint8_t attn_raw[];
@@ -434,16 +434,16 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
                 // Where the scores want a new Q, which may still be on its way, they come behind all
                 // products; else each tile's follow its product, which also keeps two tiles in turns:
                 // one's products run while the other's weights are computed.
-                const bool apart = more > 0 && sw.j == 0;
+                const bool apart = more > 0 && (kTiles == 1 || sw.j == 0);
                 if (there > 0) {
                     const bool ok = tc::mbar_wait_or_abort(&sh->vfull[nv % S], (nv / S) & 1, abort, kAWaitLimit);
-                    failed = !__all_sync(0xFFFFFFFFu, ok) || (more > 0 && !apart && !k_arrived());
+                    failed = !__all_sync(0xFFFFFFFFu, ok) || (kTiles > 1 && more > 0 && !apart && !k_arrived());
                     if (failed) break;
                     tc::fence_after();
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
                         failed = failed || !product(t);
-                        if (!failed && more > 0 && !apart) scores(t);
+                        if (kTiles > 1 && !failed && more > 0 && !apart) scores(t);
                     }
                     if (failed) break;
                     tc::mma_commit_if(lead, &sh->vempty[nv % S]);
@@ -551,35 +551,81 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
                 tc::fence_after();
                 const int first = b.kv0 + j * N;
                 // 32-key steps: all rows see all of it, some see some of it, or none sees any (left out)
-                bool full[N / 32], seen[N / 32];
-#pragma unroll
-                for (int c = 0; c < N / 32; ++c) {
-                    full[c] = first + 32 * c >= own.lo && first + 32 * c + 32 <= wall;
-                    seen[c] = !idle && first + 32 * c + 32 > own.lo && first + 32 * c < wlast;
-                }
+                auto seen = [&](int c) { return !idle && first + 32 * c + 32 > own.lo && first + 32 * c < wlast; };
                 auto load = [&](int c, float* v) {
                     tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v));
                     tc::wait_ld();
-                    if (!full[c]) {
+                    if (first + 32 * c < own.lo || first + 32 * c + 32 > wall) {
                         const uint32_t see = low_bits(hi - first - 32 * c) & ~low_bits(own.lo - first - 32 * c);
 #pragma unroll
                         for (int q = 0; q < 32; ++q) v[q] = (see >> q) & 1u ? v[q] : -INFINITY;
                     }
                 };
-                float s[Cfg::kTwice ? 32 : N];
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (Cfg::kTwice) {
+                auto maxima = [&](const float* v, float (&mx)[4]) {
 #pragma unroll
-                    for (int c = 0; c < N / 32; ++c) {
-                        if (seen[c]) {
-                            load(c, s);
+                    for (int q = 0; q < 32; q += 8)
 #pragma unroll
-                            for (int q = 0; q < 32; q += 8)
+                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], v[q + e], v[q + e + 4]);
+                };
+                // Moves the row's reference maximum where scores pass it by too much; returns what earlier
+                // weights are to be multiplied with.  The reference is a whole number: the factor is a
+                // power of two and rounds nothing.
+                auto refer = [&](const float (&mx)[4]) {
+                    const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
+                    float alpha = 1.0f;
+                    if (__any_sync(0xFFFFFFFFu, bm > m + kARescale)) {
+                        const float mn = fmaxf(m, ceilf(bm));
+                        alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+                        l *= alpha;
+                        m = mn;
+                        if (j > b0) {   // these scores came behind the last product: the accumulator is at rest
+#pragma unroll 1
+                            for (int c = 0; c < DP / 16; ++c) {
+                                uint32_t r16[16];
+                                tc::ld32x16(to + 16 * c, r16);
+                                tc::wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[q + e], s[q + e + 4]);
+                                for (int q = 0; q < 16; ++q) r16[q] = __float_as_uint(__uint_as_float(r16[q]) * alpha);
+                                tc::st32x16(to + 16 * c, r16);
+                            }
                         }
                     }
+                    return alpha;
+                };
+                auto announce = [&](int x) {
+                    tc::wait_st();
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&sh->pready[tile][x]);
+                };
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if constexpr (Cfg::kSteps) {
+                    // 32 keys at a time, each step with a maximum of its own
+                    uint32_t w[N / 2] = {};
+#pragma unroll
+                    for (int c = 0; c < N / 32; ++c) {
+                        if (seen(c)) {
+                            float s[32];
+                            load(c, s);
+                            mx[0] = mx[1] = mx[2] = mx[3] = -INFINITY;
+                            maxima(s, mx);
+                            const float alpha = refer(mx);
+                            if (c > 0 && __any_sync(0xFFFFFFFFu, alpha != 1.0f)) {
+#pragma unroll
+                                for (int q = 0; q < 16 * c; ++q) {
+                                    const float2 f = Pair16<T>::up(*reinterpret_cast<typename Pair16<T>::type*>(w + q));
+                                    const typename Pair16<T>::type h = Pair16<T>::down(f.x * alpha, f.y * alpha);
+                                    w[q] = *reinterpret_cast<const uint32_t*>(&h);
+                                }
+                            }
+                            const float ref = m == -INFINITY ? 0.f : m;
+                            l += attn_weights<T>(s, scale22, pack2(-ref, -ref), w + 16 * c);
+                        }
+                    }
+                    tc::st32x32(ts, w);
+                    announce(0);
                 } else {
+                    float s[N];
                     if (!idle && first >= own.lo && first + N <= wall) {
 #pragma unroll
                         for (int c = 0; c < N / 32; ++c)
@@ -588,7 +634,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
                     } else {
 #pragma unroll
                         for (int c = 0; c < N / 32; ++c) {
-                            if (seen[c]) {
+                            if (seen(c)) {
                                 load(c, s + 32 * c);
                             } else {
 #pragma unroll
@@ -597,48 +643,17 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
                         }
                     }
 #pragma unroll
-                    for (int c = 0; c < N; c += 8)
+                    for (int c = 0; c < N / 32; ++c) maxima(s + 32 * c, mx);
+                    (void)refer(mx);
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    const uint64_t ref2 = pack2(-ref, -ref);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + e + 4]);
-                }
-                const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
-                if (__any_sync(0xFFFFFFFFu, bm > m + kARescale)) {
-                    const float mn = fmaxf(m, bm);
-                    const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
-                    l *= alpha;
-                    m = mn;
-                    if (j > b0) {       // these scores came behind the last product: the accumulator is at rest
-#pragma unroll 1
-                        for (int c = 0; c < DP / 32; ++c) {
-                            uint32_t r32[32];
-                            tc::ld32x32(to + 32 * c, r32);
-                            tc::wait_ld();
-#pragma unroll
-                            for (int q = 0; q < 32; ++q) r32[q] = __float_as_uint(__uint_as_float(r32[q]) * alpha);
-                            tc::st32x32(to + 32 * c, r32);
-                        }
-                    }
-                }
-                const float ref = m == -INFINITY ? 0.f : m;
-                const uint64_t ref2 = pack2(-ref, -ref);
-#pragma unroll
-                for (int x = 0; x < Cfg::kHalves; ++x) {
-#pragma unroll
-                    for (int c = 2 * x; c < 2 * x + 2; ++c) {
-                        uint32_t w[16];
-                        if (seen[c]) {
-                            if (Cfg::kTwice) load(c, s);
-                            l += attn_weights<T>(s + (Cfg::kTwice ? 0 : 32 * c), scale22, ref2, w);
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < 16; ++q) w[q] = 0u;
-                        }
+                    for (int c = 0; c < N / 32; ++c) {
+                        uint32_t w[16] = {};
+                        if (seen(c)) l += attn_weights<T>(s + 32 * c, scale22, ref2, w);
                         tc::st32x16(ts + 16 * c, w);
+                        if (c & 1) announce(c / 2);
                     }
-                    tc::wait_st();
-                    tc::fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&sh->pready[tile][x]);
                 }
             }
             if (failed) break;
@@ -653,21 +668,25 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const AttnParams p) {
             // the accumulator read.
             const float inv = 1.0f / l;
             T* dst = static_cast<T*>(p.out) + row * p.out_stride + (int64_t)b.head * p.dim;
-            float odd = 0.f, o[DP];
+            bool bad = false;
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+                float o[32], odd = 0.f;
+                tc::ld32x32(to + c, *reinterpret_cast<uint32_t(*)[32]>(o));
+                tc::wait_ld();
 #pragma unroll
-            for (int c = 0; c < DP / 32; ++c) tc::ld32x32(to + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(o + 32 * c));
-            tc::wait_ld();
+                for (int q = 0; q < 32; ++q) {
+                    o[q] *= inv;
+                    odd = fmaf(o[q], 0.f, odd);                   // NaN as soon as one is not finite
+                }
+                bad = bad || (mine && !(odd == 0.f));
+                if (mine) {
 #pragma unroll
-            for (int c = 0; c < DP; ++c) {
-                o[c] *= inv;
-                odd = fmaf(o[c], 0.f, odd);                       // NaN as soon as one is not finite
+                    for (int q = 0; q < 32; q += 8)
+                        if (c + q < p.dim) *reinterpret_cast<uint4*>(dst + c + q) = down8<T>(*reinterpret_cast<float(*)[8]>(o + q));
+                }
             }
-            const bool bad = mine && !(odd == 0.f);
-            if (mine && !bad) {
-#pragma unroll
-                for (int c = 0; c < DP; c += 8)
-                    if (c < p.dim) *reinterpret_cast<uint4*>(dst + c) = down8<T>(*reinterpret_cast<float(*)[8]>(o + c));
-            }
+            __syncwarp();                                         // a bad row's values above come before attn_row's
             for (unsigned left = __ballot_sync(0xFFFFFFFFu, bad); left; left &= left - 1) {
                 const int src = __ffs(left) - 1;
                 attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), b.head, own.lo, __shfl_sync(0xFFFFFFFFu, hi, src));
