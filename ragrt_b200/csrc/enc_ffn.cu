@@ -4,7 +4,10 @@
 //   backward   dg = dh * u * act'(g), du = dh * act(g)
 //              dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
 //
-//   ffn_mma<T, kGated>  both projections of a 128-row tile in one accumulator (columns 0-127 gate,
+// ffn_mma is persistent: pairs of CTAs (cta_group::2) walk 256 x 256 accumulator tiles, each CTA loading
+// and draining its half.
+//
+//   ffn_mma<T, kGated>  both projections of a 256-row tile in one accumulator (columns 0-127 gate,
 //                       128-255 up), so that one pass over x feeds both and the activation and the
 //                       product are done on the accumulator.  Keeps g and u for the backward pass
 //                       when asked to.
@@ -27,13 +30,14 @@ namespace ragrt {
 
 namespace {
 
-constexpr int kFM = 128;                       // rows per tile
+constexpr int kFM = 256;                       // rows per tile, half of them in each CTA of a pair
 constexpr int kFN = 256;                       // accumulator columns
 constexpr int kFK = 64;                        // contraction values per stage (one swizzle atom)
-constexpr int kFTileA = kFM * kFK * 2;
-constexpr int kFTileB = kFN * kFK * 2;
-constexpr int kFStages = 4;
-constexpr int kFSmem = 1024 + kFStages * (kFTileA + kFTileB) + 256;
+constexpr int kFTileA = kFM / 2 * kFK * 2;     // bytes of a CTA's half of an operand
+constexpr int kFTileB = kFN / 2 * kFK * 2;
+constexpr int kFStages = 6;
+constexpr int kFOut = 32 * 64 * 2;             // an epilogue warp's 32 rows x 64 columns on their way out
+constexpr int kFSmem = 1024 + kFStages * (kFTileA + kFTileB) + 8 * kFOut + 256;
 constexpr int kFThreads = 320;                 // TMA warp, MMA warp, 8 epilogue warps
 constexpr uint32_t kFWaitLimit = 1u << 26;
 
@@ -42,15 +46,14 @@ enum FfnAct : int { kSilu = 0, kGelu = 1, kGeluTanh = 2 };
 
 struct FfnMaps {
     CUtensorMap a[2], b[2];
+    CUtensorMap out[3];        // kGated: h, g, u; kDx: dx; kDw: dWg, dWu
 };
 
 struct FfnParams {
     int rows, cols;            // of one output matrix
     int depth;                 // length of one contraction
     int act;
-    void* out[2];              // kGated: h; kDx: dx; kDw: dWg, dWu
-    void* gate;                // kGated: g and u are kept where not null
-    void* up;
+    int keep;                  // kGated: g and u are written too
     int* err;
 };
 
@@ -79,22 +82,35 @@ __device__ __forceinline__ void ffn_act_grad(float x, int act, float& a, float& 
     }
 }
 
+// Tile t of an output of tiles_m x tiles_n tiles, eight tile rows at a time, so that the tiles in flight
+// together read few distinct rows and columns.
+__device__ __forceinline__ void ffn_place(int t, int tiles_m, int tiles_n, int& m, int& n) {
+    const int band = t / (8 * tiles_n), in = t % (8 * tiles_n);
+    const int high = min(8, tiles_m - 8 * band);
+    m = 8 * band + in % high;
+    n = in / high;
+}
+
 template <typename T, int kMode>
-__global__ void __launch_bounds__(kFThreads, 1) ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
+ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
     constexpr bool kAMn = kMode == kDw, kBMn = kMode != kGated;
     constexpr int kOutCols = kMode == kGated ? kFN / 2 : kFN;
     extern __shared__ uint8_t ffn_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)ffn_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sA = sm;
     uint8_t* sB = sm + kFStages * kFTileA;
-    uint64_t* full = reinterpret_cast<uint64_t*>(sB + kFStages * kFTileB);
+    uint8_t* sO = sB + kFStages * kFTileB;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sO + 8 * kFOut);     // [rank 0] both CTAs' halves are there
     uint64_t* empty = full + kFStages;
-    uint64_t* accf = empty + kFStages;
-    uint64_t* acce = accf + 2;
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(acce + 2);
+    uint64_t* accf = empty + kFStages;       // [2] accumulator ready (MMA -> epilogue)
+    uint64_t* acce = accf + 2;               // [2] [rank 0] accumulator drained (both epilogues -> MMA)
+    uint64_t* drain = acce + 2;
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)tc::cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int chunks = (p.depth + kFK - 1) / kFK;
     const int nk = kMode == kDx ? 2 * chunks : chunks;
     const int tiles_n = (p.cols + kOutCols - 1) / kOutCols;
@@ -109,17 +125,19 @@ __global__ void __launch_bounds__(kFThreads, 1) ffn_mma(const __grid_constant__ 
         }
         for (int b = 0; b < 2; ++b) {
             tc::mbar_init(accf + b, 1);
-            tc::mbar_init(acce + b, 8);
+            tc::mbar_init(acce + b, 16);
         }
+        tc::mbar_init(drain, 1);
         *abort = 0;
         tc::mbar_fence_init();
     }
     if (warp == 1) {
-        tc::tmem_alloc(tslot, 512);
-        tc::tmem_relinquish();
+        tc::tmem_alloc2(tslot, 512);
+        tc::tmem_relinquish2();
     }
     tc::fence_before();
     __syncthreads();
+    tc::cluster_sync();                      // the other CTA's barriers are there before anything arrives on them
     tc::fence_after();
     const uint32_t tbase = *tslot;
     bool failed = false;
@@ -129,9 +147,12 @@ __global__ void __launch_bounds__(kFThreads, 1) ffn_mma(const __grid_constant__ 
         // ------------------------------------------------------------ TMA producer
         if (lane == 0) {
             int g = 0;
-            for (int t = blockIdx.x; t < tiles && !failed; t += gridDim.x) {
-                const int o = kMode == kDw ? t / per_out : 0, tt = kMode == kDw ? t % per_out : t;
-                const int m0 = (tt / tiles_n) * kFM, n0 = (tt % tiles_n) * kOutCols;
+            for (int t = pair; t < tiles && !failed; t += pairs) {
+                const int o = kMode == kDw ? t / per_out : 0;
+                int m, n;
+                ffn_place(kMode == kDw ? t % per_out : t, tiles_m, tiles_n, m, n);
+                const int m0 = m * kFM + rank * (kFM / 2);
+                const int n0 = n * kOutCols + (kMode == kGated ? 0 : rank * (kFN / 2));
                 for (int i = 0; i < nk; ++i, ++g) {
                     const int s = g % kFStages;
                     if (g >= kFStages && !tc::mbar_wait_or_abort(empty + s, ((g / kFStages) - 1) & 1, abort, kFWaitLimit)) {
@@ -142,71 +163,94 @@ __global__ void __launch_bounds__(kFThreads, 1) ffn_mma(const __grid_constant__ 
                     const int k = (kMode == kDx && i >= chunks ? i - chunks : i) * kFK;
                     uint8_t* da = sA + s * kFTileA;
                     uint8_t* db = sB + s * kFTileB;
-                    tc::mbar_arrive_expect_tx(full + s, kFTileA + kFTileB);
+                    const uint32_t bar = tc::cluster_addr(full + s, 0);
+                    if (rank == 0) tc::mbar_arrive_expect_tx(full + s, 2 * (kFTileA + kFTileB));
                     if (kAMn) {
 #pragma unroll
-                        for (int j = 0; j < kFM / 64; ++j)
-                            tc::tma_load_2d(da + j * 8192, &maps.a[set], m0 + 64 * j, k, full + s);
+                        for (int j = 0; j < kFM / 128; ++j)
+                            tc::tma_load_2d_pair(da + j * 8192, &maps.a[set], m0 + 64 * j, k, bar);
                     } else {
-                        tc::tma_load_2d(da, &maps.a[set], k, m0, full + s);
+                        tc::tma_load_2d_pair(da, &maps.a[set], k, m0, bar);
                     }
-                    if (kMode == kGated) {
-                        tc::tma_load_2d(db, &maps.b[0], k, n0, full + s);
-                        tc::tma_load_2d(db + kFTileB / 2, &maps.b[1], k, n0, full + s);
+                    if (kMode == kGated) {           // rank 0: the gate's half of the columns, rank 1: the other
+                        tc::tma_load_2d_pair(db, &maps.b[rank], k, n0, bar);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < kFN / 64; ++j)
-                            tc::tma_load_2d(db + j * 8192, &maps.b[kMode == kDx ? set : 0], n0 + 64 * j, k, full + s);
+                        for (int j = 0; j < kFN / 128; ++j)
+                            tc::tma_load_2d_pair(db + j * 8192, &maps.b[kMode == kDx ? set : 0], n0 + 64 * j, k, bar);
                     }
                 }
             }
+            if (failed && rank == 0)         // copies in flight end before the CTA does
+                for (int i = max(0, g - kFStages); i < g; ++i)
+                    (void)tc::mbar_wait_bounded(full + i % kFStages, (i / kFStages) & 1, 1u << 16);
         }
     } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
-            constexpr uint32_t idesc = tc::idesc_f16_f32(kFM, kFN) | fmt | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
-            int g = 0, j = 0, issued_g = -1;
-            for (int t = blockIdx.x; t < tiles && !failed; t += gridDim.x, ++j) {
+        // ------------------------------------------------------------ MMA issuer, one lane of rank 0's warp
+        if (rank == 0) {
+            constexpr uint32_t idesc = tc::idesc_f16_f32(kFM, kFN) | idesc_type<T>() | (kAMn ? kIdescAMn : 0u) |
+                                       (kBMn ? kIdescBMn : 0u);
+            const uint32_t lead = tc::elect_one();
+            int g = 0, j = 0;
+            for (int t = pair; t < tiles && !failed; t += pairs, ++j) {
                 const int b = j & 1;
-                if (j >= 2 && !tc::mbar_wait_or_abort(acce + b, ((j >> 1) - 1) & 1, abort, kFWaitLimit)) {
-                    failed = true;
-                    break;
-                }
+                bool ok = j < 2 || tc::mbar_wait_or_abort(acce + b, ((j >> 1) - 1) & 1, abort, kFWaitLimit);
+                failed = !__all_sync(0xFFFFFFFFu, ok);
+                if (failed) break;
                 tc::fence_after();
                 const uint32_t d = tbase + (uint32_t)(b * kFN);
                 for (int i = 0; i < nk; ++i, ++g) {
                     const int s = g % kFStages;
-                    if (!tc::mbar_wait_or_abort(full + s, (g / kFStages) & 1, abort, kFWaitLimit)) {
-                        failed = true;
-                        break;
-                    }
+                    ok = tc::mbar_wait_or_abort(full + s, (g / kFStages) & 1, abort, kFWaitLimit);
+                    failed = !__all_sync(0xFFFFFFFFu, ok);
+                    if (failed) break;
                     tc::fence_after();
                     const uint32_t a = tc::smem_u32(sA + s * kFTileA), bb = tc::smem_u32(sB + s * kFTileB);
 #pragma unroll
                     for (int k = 0; k < kFK / 16; ++k)
-                        tc::mma_ss(d, kAMn ? tc::sw128_mnmajor_desc(a + 2048 * k, 8192) : tc::sw128_kmajor_desc(a + 32 * k),
-                                   kBMn ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192) : tc::sw128_kmajor_desc(bb + 32 * k),
-                                   idesc, (i | k) != 0 ? 1u : 0u);
-                    tc::mma_commit(empty + s);
-                    issued_g = g;
+                        tc::mma_ss2_if(lead, d,
+                                       kAMn ? tc::sw128_mnmajor_desc(a + 2048 * k, 8192) : tc::sw128_kmajor_desc(a + 32 * k),
+                                       kBMn ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192) : tc::sw128_kmajor_desc(bb + 32 * k),
+                                       idesc, (i | k) != 0 ? 1u : 0u);
+                    tc::mma_commit2_if(lead, empty + s);
                 }
-                if (!failed) tc::mma_commit(accf + b);
+                if (!failed) tc::mma_commit2_if(lead, accf + b);
             }
-            if (failed && issued_g >= 0)   // the last MMAs read shared memory: let them finish
-                (void)tc::mbar_wait_bounded(empty + issued_g % kFStages, (issued_g / kFStages) & 1, kFWaitLimit);
+            if (failed) {                    // the last products read shared memory: let them finish
+                tc::mma_commit2_if(lead, drain);
+                (void)tc::mbar_wait_bounded(drain, 0, 1u << 16);
+            }
         }
     } else {
         // ------------------------------------------------------------ epilogue
         const int quad = warp & 3;                  // tensor-memory lane quadrant of this warp
         const int half = (warp - 2) >> 2;           // which half of the tile's columns
-        constexpr int kPer = kOutCols / 64;         // 32-column steps of a half
+        constexpr int kBoxes = kOutCols / 128;      // 64-column boxes of a half
+        uint8_t* out = sO + (warp - 2) * kFOut;
+        const uint32_t drained[2] = {tc::cluster_addr(acce, 0), tc::cluster_addr(acce + 1, 0)};
+        // 32 rows x 32 columns of the box: into shared memory, swizzled like the map
+        auto put = [&](int c, const float (&f)[32]) {
+#pragma unroll
+            for (int q = 0; q < 32; q += 8)
+                *reinterpret_cast<uint4*>(out + lane * 128 + ((((c & 1) * 4 + q / 8) ^ (lane & 7)) << 4)) =
+                    down8<T>(*reinterpret_cast<const float(*)[8]>(f + q));
+        };
+        auto send = [&](const CUtensorMap* map, int x, int y) {
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                tc::tma_store_2d(map, x, y, out);
+                tc::bulk_commit();
+                tc::bulk_wait_read();
+            }
+            __syncwarp();
+        };
         int j = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++j) {
-            const int o = kMode == kDw ? t / per_out : 0, tt = kMode == kDw ? t % per_out : t;
-            const int b = j & 1;
-            const int m0 = (tt / tiles_n) * kFM, n0 = (tt % tiles_n) * kOutCols;
-            const int row = m0 + quad * 32 + lane;
+        for (int t = pair; t < tiles; t += pairs, ++j) {
+            const int o = kMode == kDw ? t / per_out : 0, b = j & 1;
+            int m, n;
+            ffn_place(kMode == kDw ? t % per_out : t, tiles_m, tiles_n, m, n);
+            const int y = m * kFM + rank * (kFM / 2) + quad * 32;
             const bool ok = tc::mbar_wait_or_abort(accf + b, (j >> 1) & 1, abort, kFWaitLimit);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 failed = true;
@@ -214,48 +258,69 @@ __global__ void __launch_bounds__(kFThreads, 1) ffn_mma(const __grid_constant__ 
             }
             tc::fence_after();
             const uint32_t taddr = tbase + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kFN);
+            const bool rows = y < p.rows;           // of this warp
 #pragma unroll 1
-            for (int c = half * kPer; c < (half + 1) * kPer; ++c) {
-                uint32_t r[32], u[32];
-                __syncwarp();
-                tc::ld32x32(taddr + 32 * c, r);
-                if (kMode == kGated) tc::ld32x32(taddr + kFN / 2 + 32 * c, u);
-                tc::wait_ld();
-                if (row < p.rows) {
-                    const int64_t at = (int64_t)row * p.cols + n0 + 32 * c;
+            for (int x = 0; x < kBoxes; ++x) {
+                const int c0 = (half * kBoxes + x) * 64, at = n * kOutCols + c0;
+                if (!rows || at >= p.cols) break;
+                if (kMode == kGated && p.keep) {
+#pragma unroll 1
+                    for (int w = 0; w < 2; ++w) {
 #pragma unroll
-                    for (int q = 0; q < 32; q += 8) {
-                        if (n0 + 32 * c + q < p.cols) {          // cols is a multiple of 8
-                            float f[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(r[q + e]);
-                            if (kMode == kGated) {
-                                float v[8];
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(u[q + e]);
-                                if (p.gate) {
-                                    *reinterpret_cast<uint4*>(static_cast<T*>(p.gate) + at + q) = down8<T>(f);
-                                    *reinterpret_cast<uint4*>(static_cast<T*>(p.up) + at + q) = down8<T>(v);
-                                }
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) f[e] = ffn_act(f[e], p.act) * v[e];
-                            }
-                            *reinterpret_cast<uint4*>(static_cast<T*>(p.out[o]) + at + q) = down8<T>(f);
+                        for (int c = 0; c < 2; ++c) {
+                            float f[32];
+                            tc::ld32x32(taddr + w * (kFN / 2) + c0 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(f));
+                            tc::wait_ld();
+                            put(c, f);
                         }
+                        send(&maps.out[1 + w], at, y);
                     }
                 }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float f[32];
+                    tc::ld32x32(taddr + c0 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(f));
+                    if (kMode == kGated) {
+                        float v[32];
+                        tc::ld32x32(taddr + kFN / 2 + c0 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v));
+                        tc::wait_ld();
+                        if (p.act == kSilu) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kSilu) * v[e];
+                        } else if (p.act == kGelu) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kGelu) * v[e];
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kGeluTanh) * v[e];
+                        }
+                    } else {
+                        tc::wait_ld();
+                    }
+                    put(c, f);
+                }
+                if (x == kBoxes - 1) {              // all of the accumulator is in registers
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive_cluster(drained[b]);
+                }
+                send(&maps.out[kMode == kDw ? o : 0], at, y);
             }
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(acce + b);
+            if (!rows || n * kOutCols + (half * kBoxes + kBoxes - 1) * 64 >= p.cols) {
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive_cluster(drained[b]);
+            }
         }
+        if (lane == 0) tc::bulk_wait();
     }
     if (failed && lane == 0) atomicExch(p.err, 1);
     tc::fence_before();
     __syncthreads();
+    tc::cluster_sync();                      // neither CTA's memory goes while the other may still reach it
     if (warp == 1) {
         tc::fence_after();
-        tc::tmem_dealloc(tbase, 512);
+        tc::tmem_dealloc2(tbase, 512);
     }
 }
 
@@ -284,19 +349,14 @@ __global__ void __launch_bounds__(256) ffn_act_backward(const T* __restrict__ dh
 
 template <typename T, int kMode>
 int ffn_launch(const FfnMaps& maps, const FfnParams& p, cudaStream_t stream) {
-    // the shared-memory attribute is per device: set it once for each device used
-    static std::atomic<uint64_t> attr_set{0};
-    int dev = 0;
-    RAGRT_CUDA_TRY(cudaGetDevice(&dev));
-    const uint64_t bit = 1ull << (dev & 63);
-    if (!(attr_set.load() & bit)) {
-        RAGRT_CUDA_TRY(cudaFuncSetAttribute(ffn_mma<T, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFSmem));
-        attr_set.fetch_or(bit);
-    }
+    static std::atomic<uint64_t> done{0};
+    int rc = enc_allow_smem(ffn_mma<T, kMode>, kFSmem, done);
+    if (rc) return rc;
     const int out_cols = kMode == kGated ? kFN / 2 : kFN;
     const int64_t tiles = ceil_div(p.rows, kFM) * ceil_div(p.cols, out_cols) * (kMode == kDw ? 2 : 1);
-    return enc_launch(ffn_mma<T, kMode>, dim3((unsigned)std::min<int64_t>(tiles, num_sms())), dim3(kFThreads), kFSmem,
-                      stream, maps, p);
+    if (tiles > 0x3FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many tiles");
+    return enc_launch(ffn_mma<T, kMode>, dim3((unsigned)(2 * std::min<int64_t>(tiles, num_sms() / 2))), dim3(kFThreads),
+                      kFSmem, stream, maps, p);
 }
 
 template <int kMode>
@@ -333,12 +393,15 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
     FfnMaps m;
-    if ((rc = enc_map_2d(&m.a[0], dtype, d_x, M, K, K, kFM)) ||
+    if ((rc = enc_map_2d(&m.a[0], dtype, d_x, M, K, K, kFM / 2)) ||
         (rc = enc_map_2d(&m.b[0], dtype, d_w_gate, F, K, K, kFN / 2)) ||
-        (rc = enc_map_2d(&m.b[1], dtype, d_w_up, F, K, K, kFN / 2)))
+        (rc = enc_map_2d(&m.b[1], dtype, d_w_up, F, K, K, kFN / 2)) ||
+        (rc = enc_map_2d(&m.out[0], dtype, d_h, M, F, F, 32)) ||
+        (rc = enc_map_2d(&m.out[1], dtype, d_gate ? d_gate : d_h, M, F, F, 32)) ||
+        (rc = enc_map_2d(&m.out[2], dtype, d_up ? d_up : d_h, M, F, F, 32)))
         return rc;
     m.a[1] = m.a[0];
-    FfnParams p{M, F, K, act, {d_h, nullptr}, d_gate, d_up, err};
+    FfnParams p{M, F, K, act, d_gate != nullptr, err};
     return ffn_launch_typed<kGated>(dtype, m, p, (cudaStream_t)stream_);
 }
 
@@ -377,21 +440,26 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
     if (rc) return rc;
     FfnMaps m;
     if (d_dx) {
-        if ((rc = enc_map_2d(&m.a[0], dtype, d_dgate, M, F, F, kFM)) ||
-            (rc = enc_map_2d(&m.a[1], dtype, d_dup, M, F, F, kFM)) ||
+        if ((rc = enc_map_2d(&m.a[0], dtype, d_dgate, M, F, F, kFM / 2)) ||
+            (rc = enc_map_2d(&m.a[1], dtype, d_dup, M, F, F, kFM / 2)) ||
             (rc = enc_map_2d(&m.b[0], dtype, d_w_gate, F, K, K, kFK)) ||
-            (rc = enc_map_2d(&m.b[1], dtype, d_w_up, F, K, K, kFK)))
+            (rc = enc_map_2d(&m.b[1], dtype, d_w_up, F, K, K, kFK)) ||
+            (rc = enc_map_2d(&m.out[0], dtype, d_dx, M, K, K, 32)))
             return rc;
-        FfnParams p{M, K, F, act, {d_dx, nullptr}, nullptr, nullptr, err};
+        m.out[1] = m.out[2] = m.out[0];
+        FfnParams p{M, K, F, act, 0, err};
         if ((rc = ffn_launch_typed<kDx>(dtype, m, p, stream))) return rc;
     }
     if (d_dw_gate) {
         if ((rc = enc_map_2d(&m.a[0], dtype, d_dgate, M, F, F, kFK)) ||
             (rc = enc_map_2d(&m.a[1], dtype, d_dup, M, F, F, kFK)) ||
-            (rc = enc_map_2d(&m.b[0], dtype, d_x, M, K, K, kFK)))
+            (rc = enc_map_2d(&m.b[0], dtype, d_x, M, K, K, kFK)) ||
+            (rc = enc_map_2d(&m.out[0], dtype, d_dw_gate, F, K, K, 32)) ||
+            (rc = enc_map_2d(&m.out[1], dtype, d_dw_up, F, K, K, 32)))
             return rc;
         m.b[1] = m.b[0];
-        FfnParams p{F, K, M, act, {d_dw_gate, d_dw_up}, nullptr, nullptr, err};
+        m.out[2] = m.out[1];
+        FfnParams p{F, K, M, act, 0, err};
         if ((rc = ffn_launch_typed<kDw>(dtype, m, p, stream))) return rc;
     }
     return RAGRT_OK;
