@@ -4,17 +4,18 @@
 //   backward   dg = dh * u * act'(g), du = dh * act(g)
 //              dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x
 //
-// ffn_mma is persistent: pairs of CTAs (cta_group::2) walk 256 x 256 accumulator tiles, each CTA loading
-// and draining its half.
-//
-//   ffn_mma<T, kGated>  both projections of a 256-row tile in one accumulator (columns 0-127 gate,
-//                       128-255 up), so that one pass over x feeds both and the activation and the
-//                       product are done on the accumulator.  Keeps g and u for the backward pass
-//                       when asked to.
-//   ffn_mma<T, kDx>     one product over the 2 F columns of [dg | du] and the rows of [Wg ; Wu]:
-//                       the two halves add up in the accumulator.
-//   ffn_mma<T, kDw>     both weight gradients in one launch, contracted over the rows of x.
-//   ffn_act_backward    dg and du, elementwise.
+//   ffn_pair<T, kForward>   both projections in one accumulator (half of its columns gate, half up), so that
+//                           one pass over x feeds both and the activation and the product are done on
+//                           the accumulator.  Keeps g and u for the backward pass when asked to.
+//   ffn_pair<T, kBackward>  dx, one product over the 2 F columns of [dg | du] and the rows of [Wg ; Wu] (the
+//                           halves add up in the accumulator), and both weight gradients, contracted
+//                           over the rows of x: one list of tiles.  Persistent pairs of CTAs
+//                           (cta_group::2) on 256 x 256 accumulators, each CTA loading and draining its half.
+//   ffn_small<T, ...>       the same on 128 x 64 accumulators, two single CTAs per SM: more and shorter
+//                           tiles where the large ones would leave SMs without work.
+//   ffn_rows                forward of up to four rows: a warp per pair of weight rows, fp32 on the CUDA
+//                           cores, bound by the weights' bytes.
+//   ffn_act_backward        dg and du, elementwise.
 //
 // The weight matrices and x are read as they lie: an operand whose contraction index is the row of
 // its matrix is fed to the tensor cores MN-major.  Accumulators are fp32; g and u are rounded once
@@ -41,20 +42,61 @@ constexpr int kFSmem = 1024 + kFStages * (kFTileA + kFTileB) + 8 * kFOut + 256;
 constexpr int kFThreads = 320;                 // TMA warp, MMA warp, 8 epilogue warps
 constexpr uint32_t kFWaitLimit = 1u << 26;
 
-enum FfnMode : int { kGated = 0, kDx = 1, kDw = 2 };
+enum FfnMode : int { kForward = 0, kBackward = 1 };
 enum FfnAct : int { kSilu = 0, kGelu = 1, kGeluTanh = 2 };
 
 struct FfnMaps {
-    CUtensorMap a[2], b[2];
-    CUtensorMap out[3];        // kGated: h, g, u; kDx: dx; kDw: dWg, dWu
+    // kForward: a[0] = x, b[0], b[1] = Wg, Wu, out = h, g, u
+    // kBackward: dx: a[0], a[1] = dg, du, b[0], b[1] = Wg, Wu, out[0] = dx
+    //            dWg, dWu: a[2], a[3] = dg, du, b[2] = x, out[1], out[2]
+    CUtensorMap a[4], b[3], out[3];
 };
 
 struct FfnParams {
-    int rows, cols;            // of one output matrix
-    int depth;                 // length of one contraction
+    int M, F, K;
     int act;
-    int keep;                  // kGated: g and u are written too
+    int keep;                  // kForward: g and u are written too
+    int dx, dw;                // kBackward: which gradients
+    void* out[3];              // as in FfnMaps
     int* err;
+};
+
+// A tile of one of the products: output `out` (0, or 1 and 2 for the weight gradients), its rows x cols,
+// the tile's first row and column, and the length of the contraction in chunks of kFK (dx: of each half).
+struct FfnTile {
+    int out, rows, cols, m0, n0, chunks;
+};
+
+// Tile t of the list: dx first, the longest contraction, then dWg, dWu.  Within an output eight tile
+// rows at a time, so that the tiles in flight together read few distinct rows and columns.
+template <int kMode, int kTileM, int kTileN>
+struct FfnList {
+    int tn, first, per, total;               // tiles of dx (or h) per tile row, of dx, of dWg, in all
+    __device__ __forceinline__ FfnList(const FfnParams& p) {
+        const int cols = kMode == kForward ? p.F : p.K;
+        tn = (cols + kTileN - 1) / kTileN;
+        first = kMode == kForward || p.dx ? tn * ((p.M + kTileM - 1) / kTileM) : 0;
+        per = kMode == kBackward && p.dw ? tn * ((p.F + kTileM - 1) / kTileM) : 0;
+        total = first + 2 * per;
+    }
+    __device__ __forceinline__ FfnTile get(const FfnParams& p, int t) const {
+        FfnTile r;
+        const bool dw = t >= first;
+        r.out = 0;
+        if (dw) {
+            t -= first;
+            r.out = 1 + (t >= per);
+            if (t >= per) t -= per;
+        }
+        r.rows = dw ? p.F : p.M;
+        r.cols = kMode == kForward ? p.F : p.K;
+        r.chunks = ((kMode == kForward ? p.K : dw ? p.M : p.F) + kFK - 1) / kFK;
+        const int tm = (r.rows + kTileM - 1) / kTileM;
+        const int band = t / (8 * tn), in = t % (8 * tn), high = min(8, tm - 8 * band);
+        r.m0 = (8 * band + in % high) * kTileM;
+        r.n0 = in / high * kTileN;
+        return r;
+    }
 };
 
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
@@ -64,6 +106,19 @@ __device__ __forceinline__ float ffn_act(float x, int act) {
     if (act == kSilu) return x * sigmoid(x);
     if (act == kGelu) return gelu_erf(x);
     return x * sigmoid(1.5957691216057308f * (x + 0.044715f * x * x * x));
+}
+// f = act(f) * v
+__device__ __forceinline__ void ffn_gate(float (&f)[32], const float (&v)[32], int act) {
+    if (act == kSilu) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kSilu) * v[e];
+    } else if (act == kGelu) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kGelu) * v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kGeluTanh) * v[e];
+    }
 }
 // act(x) and act'(x)
 __device__ __forceinline__ void ffn_act_grad(float x, int act, float& a, float& d) {
@@ -82,20 +137,10 @@ __device__ __forceinline__ void ffn_act_grad(float x, int act, float& a, float& 
     }
 }
 
-// Tile t of an output of tiles_m x tiles_n tiles, eight tile rows at a time, so that the tiles in flight
-// together read few distinct rows and columns.
-__device__ __forceinline__ void ffn_place(int t, int tiles_m, int tiles_n, int& m, int& n) {
-    const int band = t / (8 * tiles_n), in = t % (8 * tiles_n);
-    const int high = min(8, tiles_m - 8 * band);
-    m = 8 * band + in % high;
-    n = in / high;
-}
-
 template <typename T, int kMode>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFThreads, 1)
-ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
-    constexpr bool kAMn = kMode == kDw, kBMn = kMode != kGated;
-    constexpr int kOutCols = kMode == kGated ? kFN / 2 : kFN;
+ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams p) {
+    constexpr int kOutCols = kMode == kForward ? kFN / 2 : kFN;
     extern __shared__ uint8_t ffn_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)ffn_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sA = sm;
@@ -111,12 +156,7 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)tc::cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int chunks = (p.depth + kFK - 1) / kFK;
-    const int nk = kMode == kDx ? 2 * chunks : chunks;
-    const int tiles_n = (p.cols + kOutCols - 1) / kOutCols;
-    const int tiles_m = (p.rows + kFM - 1) / kFM;
-    const int per_out = tiles_n * tiles_m;
-    const int tiles = kMode == kDw ? 2 * per_out : per_out;
+    const FfnList<kMode, kFM, kOutCols> list(p);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFStages; ++s) {
@@ -147,37 +187,37 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
         // ------------------------------------------------------------ TMA producer
         if (lane == 0) {
             int g = 0;
-            for (int t = pair; t < tiles && !failed; t += pairs) {
-                const int o = kMode == kDw ? t / per_out : 0;
-                int m, n;
-                ffn_place(kMode == kDw ? t % per_out : t, tiles_m, tiles_n, m, n);
-                const int m0 = m * kFM + rank * (kFM / 2);
-                const int n0 = n * kOutCols + (kMode == kGated ? 0 : rank * (kFN / 2));
+            for (int t = pair; t < list.total && !failed; t += pairs) {
+                const FfnTile tile = list.get(p, t);
+                const bool dw = kMode == kBackward && tile.out > 0;
+                const int nk = kMode == kBackward && !dw ? 2 * tile.chunks : tile.chunks;
+                const int m0 = tile.m0 + rank * (kFM / 2);
+                const int n0 = tile.n0 + (kMode == kForward ? 0 : rank * (kFN / 2));
                 for (int i = 0; i < nk; ++i, ++g) {
                     const int s = g % kFStages;
                     if (g >= kFStages && !tc::mbar_wait_or_abort(empty + s, ((g / kFStages) - 1) & 1, abort, kFWaitLimit)) {
                         failed = true;
                         break;
                     }
-                    const int set = kMode == kDx ? (i >= chunks) : o;
-                    const int k = (kMode == kDx && i >= chunks ? i - chunks : i) * kFK;
+                    const bool second = i >= tile.chunks;        // dx: the half of du and Wu
+                    const int k = (second ? i - tile.chunks : i) * kFK;
                     uint8_t* da = sA + s * kFTileA;
                     uint8_t* db = sB + s * kFTileB;
                     const uint32_t bar = tc::cluster_addr(full + s, 0);
                     if (rank == 0) tc::mbar_arrive_expect_tx(full + s, 2 * (kFTileA + kFTileB));
-                    if (kAMn) {
+                    if (dw) {
 #pragma unroll
                         for (int j = 0; j < kFM / 128; ++j)
-                            tc::tma_load_2d_pair(da + j * 8192, &maps.a[set], m0 + 64 * j, k, bar);
+                            tc::tma_load_2d_pair(da + j * 8192, &maps.a[1 + tile.out], m0 + 64 * j, k, bar);
                     } else {
-                        tc::tma_load_2d_pair(da, &maps.a[set], k, m0, bar);
+                        tc::tma_load_2d_pair(da, &maps.a[second], k, m0, bar);
                     }
-                    if (kMode == kGated) {           // rank 0: the gate's half of the columns, rank 1: the other
+                    if (kMode == kForward) {         // rank 0: the gate's half of the columns, rank 1: the other
                         tc::tma_load_2d_pair(db, &maps.b[rank], k, n0, bar);
                     } else {
 #pragma unroll
                         for (int j = 0; j < kFN / 128; ++j)
-                            tc::tma_load_2d_pair(db + j * 8192, &maps.b[kMode == kDx ? set : 0], n0 + 64 * j, k, bar);
+                            tc::tma_load_2d_pair(db + j * 8192, &maps.b[dw ? 2 : (int)second], n0 + 64 * j, k, bar);
                     }
                 }
             }
@@ -188,11 +228,15 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer, one lane of rank 0's warp
         if (rank == 0) {
-            constexpr uint32_t idesc = tc::idesc_f16_f32(kFM, kFN) | idesc_type<T>() | (kAMn ? kIdescAMn : 0u) |
-                                       (kBMn ? kIdescBMn : 0u);
             const uint32_t lead = tc::elect_one();
             int g = 0, j = 0;
-            for (int t = pair; t < tiles && !failed; t += pairs, ++j) {
+            for (int t = pair; t < list.total && !failed; t += pairs, ++j) {
+                const FfnTile tile = list.get(p, t);
+                const bool dw = kMode == kBackward && tile.out > 0;
+                const int nk = kMode == kBackward && !dw ? 2 * tile.chunks : tile.chunks;
+                const uint32_t idesc = tc::idesc_f16_f32(kFM, kFN) | idesc_type<T>() | (dw ? kIdescAMn : 0u) |
+                                       (kMode == kBackward ? kIdescBMn : 0u);
+                const uint32_t step = dw ? 2048 : 32;
                 const int b = j & 1;
                 bool ok = j < 2 || tc::mbar_wait_or_abort(acce + b, ((j >> 1) - 1) & 1, abort, kFWaitLimit);
                 failed = !__all_sync(0xFFFFFFFFu, ok);
@@ -205,12 +249,13 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
                     failed = !__all_sync(0xFFFFFFFFu, ok);
                     if (failed) break;
                     tc::fence_after();
+                    // the leading byte offset, which only an MN-major operand has, is there for both
                     const uint32_t a = tc::smem_u32(sA + s * kFTileA), bb = tc::smem_u32(sB + s * kFTileB);
 #pragma unroll
                     for (int k = 0; k < kFK / 16; ++k)
-                        tc::mma_ss2_if(lead, d,
-                                       kAMn ? tc::sw128_mnmajor_desc(a + 2048 * k, 8192) : tc::sw128_kmajor_desc(a + 32 * k),
-                                       kBMn ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192) : tc::sw128_kmajor_desc(bb + 32 * k),
+                        tc::mma_ss2_if(lead, d, tc::sw128_mnmajor_desc(a + step * k, 8192),
+                                       kMode == kBackward ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192)
+                                                          : tc::sw128_kmajor_desc(bb + 32 * k),
                                        idesc, (i | k) != 0 ? 1u : 0u);
                     tc::mma_commit2_if(lead, empty + s);
                 }
@@ -246,11 +291,10 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
             __syncwarp();
         };
         int j = 0;
-        for (int t = pair; t < tiles; t += pairs, ++j) {
-            const int o = kMode == kDw ? t / per_out : 0, b = j & 1;
-            int m, n;
-            ffn_place(kMode == kDw ? t % per_out : t, tiles_m, tiles_n, m, n);
-            const int y = m * kFM + rank * (kFM / 2) + quad * 32;
+        for (int t = pair; t < list.total; t += pairs, ++j) {
+            const FfnTile tile = list.get(p, t);
+            const int b = j & 1;
+            const int y = tile.m0 + rank * (kFM / 2) + quad * 32;
             const bool ok = tc::mbar_wait_or_abort(accf + b, (j >> 1) & 1, abort, kFWaitLimit);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 failed = true;
@@ -258,12 +302,12 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
             }
             tc::fence_after();
             const uint32_t taddr = tbase + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kFN);
-            const bool rows = y < p.rows;           // of this warp
+            const bool rows = y < tile.rows;        // of this warp
 #pragma unroll 1
             for (int x = 0; x < kBoxes; ++x) {
-                const int c0 = (half * kBoxes + x) * 64, at = n * kOutCols + c0;
-                if (!rows || at >= p.cols) break;
-                if (kMode == kGated && p.keep) {
+                const int c0 = (half * kBoxes + x) * 64, at = tile.n0 + c0;
+                if (!rows || at >= tile.cols) break;
+                if (kMode == kForward && p.keep) {
 #pragma unroll 1
                     for (int w = 0; w < 2; ++w) {
 #pragma unroll
@@ -280,20 +324,11 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
                 for (int c = 0; c < 2; ++c) {
                     float f[32];
                     tc::ld32x32(taddr + c0 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(f));
-                    if (kMode == kGated) {
+                    if (kMode == kForward) {
                         float v[32];
                         tc::ld32x32(taddr + kFN / 2 + c0 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v));
                         tc::wait_ld();
-                        if (p.act == kSilu) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kSilu) * v[e];
-                        } else if (p.act == kGelu) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kGelu) * v[e];
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) f[e] = ffn_act(f[e], kGeluTanh) * v[e];
-                        }
+                        ffn_gate(f, v, p.act);
                     } else {
                         tc::wait_ld();
                     }
@@ -304,9 +339,9 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive_cluster(drained[b]);
                 }
-                send(&maps.out[kMode == kDw ? o : 0], at, y);
+                send(&maps.out[kMode == kForward ? 0 : tile.out], at, y);
             }
-            if (!rows || n * kOutCols + (half * kBoxes + kBoxes - 1) * 64 >= p.cols) {
+            if (!rows || tile.n0 + (half * kBoxes + kBoxes - 1) * 64 >= tile.cols) {
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive_cluster(drained[b]);
@@ -321,6 +356,247 @@ ffn_mma(const __grid_constant__ FfnMaps maps, const FfnParams p) {
     if (warp == 1) {
         tc::fence_after();
         tc::tmem_dealloc2(tbase, 512);
+    }
+}
+
+// ------------------------------------------------------------------ 128 x 64 tiles
+constexpr int kSN = 64;                        // accumulator columns
+constexpr int kSTileA = kFM / 2 * kFK * 2;
+constexpr int kSTileB = kSN * kFK * 2;
+constexpr int kSStages = 4;
+constexpr int kSSmem = 1024 + kSStages * (kSTileA + kSTileB) + 256;
+constexpr int kFewRows = 4;                    // up to here ffn_rows
+constexpr int kSThreads = 192;                 // TMA warp, MMA warp, 4 epilogue warps
+
+template <typename T, int kMode>
+__global__ void __launch_bounds__(kSThreads, 2)
+ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams p) {
+    constexpr int kOutCols = kMode == kForward ? kSN / 2 : kSN;
+    extern __shared__ uint8_t ffn_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)ffn_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* sA = sm;
+    uint8_t* sB = sm + kSStages * kSTileA;
+    uint64_t* full = reinterpret_cast<uint64_t*>(sB + kSStages * kSTileB);
+    uint64_t* empty = full + kSStages;
+    uint64_t* accf = empty + kSStages;
+    uint64_t* acce = accf + 2;
+    uint64_t* drain = acce + 2;
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort = reinterpret_cast<volatile int*>(tslot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const FfnList<kMode, kFM / 2, kOutCols> list(p);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kSStages; ++s) {
+            tc::mbar_init(full + s, 1);
+            tc::mbar_init(empty + s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(accf + b, 1);
+            tc::mbar_init(acce + b, 4);
+        }
+        tc::mbar_init(drain, 1);
+        *abort = 0;
+        tc::mbar_fence_init();
+    }
+    if (warp == 1) {
+        tc::tmem_alloc(tslot, 2 * kSN);
+        tc::tmem_relinquish();
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tbase = *tslot;
+    bool failed = false;
+    pdl_wait_then_release();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int g = 0;
+            for (int t = blockIdx.x; t < list.total && !failed; t += gridDim.x) {
+                const FfnTile tile = list.get(p, t);
+                const bool dw = kMode == kBackward && tile.out > 0;
+                const int nk = kMode == kBackward && !dw ? 2 * tile.chunks : tile.chunks;
+                for (int i = 0; i < nk; ++i, ++g) {
+                    const int s = g % kSStages;
+                    if (g >= kSStages && !tc::mbar_wait_or_abort(empty + s, ((g / kSStages) - 1) & 1, abort, kFWaitLimit)) {
+                        failed = true;
+                        break;
+                    }
+                    const bool second = i >= tile.chunks;
+                    const int k = (second ? i - tile.chunks : i) * kFK;
+                    uint8_t* da = sA + s * kSTileA;
+                    uint8_t* db = sB + s * kSTileB;
+                    tc::mbar_arrive_expect_tx(full + s, kSTileA + kSTileB);
+                    if (dw) {
+                        tc::tma_load_2d(da, &maps.a[1 + tile.out], tile.m0, k, full + s);
+                        tc::tma_load_2d(da + 8192, &maps.a[1 + tile.out], tile.m0 + 64, k, full + s);
+                    } else {
+                        tc::tma_load_2d(da, &maps.a[second], k, tile.m0, full + s);
+                    }
+                    if (kMode == kForward) {
+                        tc::tma_load_2d(db, &maps.b[0], k, tile.n0, full + s);
+                        tc::tma_load_2d(db + kSTileB / 2, &maps.b[1], k, tile.n0, full + s);
+                    } else {
+                        tc::tma_load_2d(db, &maps.b[dw ? 2 : (int)second], tile.n0, k, full + s);
+                    }
+                }
+            }
+            if (failed)                      // copies in flight end before the CTA does
+                for (int i = max(0, g - kSStages); i < g; ++i)
+                    (void)tc::mbar_wait_bounded(full + i % kSStages, (i / kSStages) & 1, 1u << 16);
+        }
+    } else if (warp == 1) {
+        const uint32_t lead = tc::elect_one();
+        int g = 0, j = 0;
+        for (int t = blockIdx.x; t < list.total && !failed; t += gridDim.x, ++j) {
+            const FfnTile tile = list.get(p, t);
+            const bool dw = kMode == kBackward && tile.out > 0;
+            const int nk = kMode == kBackward && !dw ? 2 * tile.chunks : tile.chunks;
+            const uint32_t idesc = tc::idesc_f16_f32(kFM / 2, kSN) | idesc_type<T>() | (dw ? kIdescAMn : 0u) |
+                                   (kMode == kBackward ? kIdescBMn : 0u);
+            const uint32_t step = dw ? 2048 : 32;
+            const int b = j & 1;
+            bool ok = j < 2 || tc::mbar_wait_or_abort(acce + b, ((j >> 1) - 1) & 1, abort, kFWaitLimit);
+            failed = !__all_sync(0xFFFFFFFFu, ok);
+            if (failed) break;
+            tc::fence_after();
+            for (int i = 0; i < nk; ++i, ++g) {
+                const int s = g % kSStages;
+                ok = tc::mbar_wait_or_abort(full + s, (g / kSStages) & 1, abort, kFWaitLimit);
+                failed = !__all_sync(0xFFFFFFFFu, ok);
+                if (failed) break;
+                tc::fence_after();
+                const uint32_t a = tc::smem_u32(sA + s * kSTileA), bb = tc::smem_u32(sB + s * kSTileB);
+#pragma unroll
+                for (int k = 0; k < kFK / 16; ++k)
+                    tc::mma_ss_if(lead, tbase + (uint32_t)(b * kSN), tc::sw128_mnmajor_desc(a + step * k, 8192),
+                                  kMode == kBackward ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192)
+                                                     : tc::sw128_kmajor_desc(bb + 32 * k),
+                                  idesc, (i | k) != 0 ? 1u : 0u);
+                tc::mma_commit_if(lead, empty + s);
+            }
+            if (!failed) tc::mma_commit_if(lead, accf + b);
+        }
+        if (failed) {                        // the last products read shared memory: let them finish
+            tc::mma_commit_if(lead, drain);
+            (void)tc::mbar_wait_bounded(drain, 0, 1u << 16);
+        }
+    } else {
+        const int quad = warp & 3;
+        int j = 0;
+        for (int t = blockIdx.x; t < list.total; t += gridDim.x, ++j) {
+            const FfnTile tile = list.get(p, t);
+            const int b = j & 1, row = tile.m0 + quad * 32 + lane;
+            const bool ok = tc::mbar_wait_or_abort(accf + b, (j >> 1) & 1, abort, kFWaitLimit);
+            if (!__all_sync(0xFFFFFFFFu, ok)) {
+                failed = true;
+                break;
+            }
+            tc::fence_after();
+            const uint32_t taddr = tbase + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kSN);
+            float f[32], v[32];
+            tc::ld32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(f));
+            tc::ld32x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(v));
+            tc::wait_ld();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(acce + b);
+            if (row < tile.rows) {
+                const int64_t at = (int64_t)row * tile.cols + tile.n0;
+                auto put = [&](void* base, int off, const float (&x)[32]) {
+#pragma unroll
+                    for (int q = 0; q < 32; q += 8)
+                        if (tile.n0 + off + q < tile.cols)       // cols is a multiple of 8
+                            *reinterpret_cast<uint4*>(static_cast<T*>(base) + at + off + q) =
+                                down8<T>(*reinterpret_cast<const float(*)[8]>(x + q));
+                };
+                if (kMode == kForward) {
+                    if (p.keep) {
+                        put(p.out[1], 0, f);
+                        put(p.out[2], 0, v);
+                    }
+                    ffn_gate(f, v, p.act);
+                    put(p.out[0], 0, f);
+                } else {
+                    put(p.out[tile.out], 0, f);
+                    put(p.out[tile.out], 32, v);
+                }
+            }
+        }
+    }
+    if (failed && lane == 0) atomicExch(p.err, 1);
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc::fence_after();
+        tc::tmem_dealloc(tbase, 2 * kSN);
+    }
+}
+
+// ------------------------------------------------------------------ few rows
+// A warp per output column: it reads one row of Wg and one of Wu, 8 values a lane and step, against the
+// same values of up to kRows rows of x.
+template <typename T, int kRows>
+__global__ void __launch_bounds__(256) ffn_rows(const T* __restrict__ x, const T* __restrict__ wg,
+                                                const T* __restrict__ wu, const __grid_constant__ FfnParams p) {
+    const int f = (int)((blockIdx.x * 256 + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+    pdl_wait_then_release();
+    if (f >= p.F) return;
+    const T* g = wg + (int64_t)f * p.K;
+    const T* u = wu + (int64_t)f * p.K;
+    uint64_t sg[kRows] = {}, su[kRows] = {};
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    constexpr int kAhead = 4;                        // steps whose weights are in flight together
+    for (int k0 = lane * 8; k0 < p.K + lane * 8; k0 += 256 * kAhead) {
+        uint4 a[kAhead], b[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const bool in = k0 + 256 * i < p.K;
+            a[i] = in ? __ldg(reinterpret_cast<const uint4*>(g + k0 + 256 * i)) : zero;
+            b[i] = in ? __ldg(reinterpret_cast<const uint4*>(u + k0 + 256 * i)) : zero;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (k0 + 256 * i >= p.K) break;
+            float fa[8], fb[8];
+            up8<T>(a[i], fa);
+            up8<T>(b[i], fb);
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                if (r >= p.M) break;
+                float fx[8];
+                up8<T>(__ldg(reinterpret_cast<const uint4*>(x + (int64_t)r * p.K + k0 + 256 * i)), fx);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const uint64_t x2 = pack2(fx[e], fx[e + 1]);
+                    sg[r] = fma2(pack2(fa[e], fa[e + 1]), x2, sg[r]);
+                    su[r] = fma2(pack2(fb[e], fb[e + 1]), x2, su[r]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        if (r >= p.M) break;
+        float a, b, c, d;
+        unpack2(sg[r], a, b);
+        unpack2(su[r], c, d);
+        a += b;
+        c += d;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+            c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
+        }
+        if (lane == 0) {
+            const int64_t at = (int64_t)r * p.F + f;
+            if (p.keep) {
+                static_cast<T*>(p.out[1])[at] = (T)a;
+                static_cast<T*>(p.out[2])[at] = (T)c;
+            }
+            static_cast<T*>(p.out[0])[at] = (T)(ffn_act(a, p.act) * c);
+        }
     }
 }
 
@@ -347,22 +623,63 @@ __global__ void __launch_bounds__(256) ffn_act_backward(const T* __restrict__ dh
     }
 }
 
-template <typename T, int kMode>
-int ffn_launch(const FfnMaps& maps, const FfnParams& p, cudaStream_t stream) {
-    static std::atomic<uint64_t> done{0};
-    int rc = enc_allow_smem(ffn_mma<T, kMode>, kFSmem, done);
-    if (rc) return rc;
-    const int out_cols = kMode == kGated ? kFN / 2 : kFN;
-    const int64_t tiles = ceil_div(p.rows, kFM) * ceil_div(p.cols, out_cols) * (kMode == kDw ? 2 : 1);
-    if (tiles > 0x3FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many tiles");
-    return enc_launch(ffn_mma<T, kMode>, dim3((unsigned)(2 * std::min<int64_t>(tiles, num_sms() / 2))), dim3(kFThreads),
-                      kFSmem, stream, maps, p);
+// The operands' maps differ in their boxes between the two kernels.
+int ffn_maps(FfnMaps& m, int mode, bool pair, int dtype, const FfnParams& p, const void* x, const void* wg, const void* wu,
+             const void* dg, const void* du) {
+    int rc;
+    if (mode == kForward) {
+        const int wrows = pair ? kFN / 2 : kSN / 2;
+        if ((rc = enc_map_2d(&m.a[0], dtype, x, p.M, p.K, p.K, kFM / 2)) ||
+            (rc = enc_map_2d(&m.b[0], dtype, wg, p.F, p.K, p.K, wrows)) ||
+            (rc = enc_map_2d(&m.b[1], dtype, wu, p.F, p.K, p.K, wrows)))
+            return rc;
+        if (pair)
+            for (int i = 0; i < (p.keep ? 3 : 1); ++i)
+                if ((rc = enc_map_2d(&m.out[i], dtype, p.out[i], p.M, p.F, p.F, 32))) return rc;
+        return RAGRT_OK;
+    }
+    if (p.dx && ((rc = enc_map_2d(&m.a[0], dtype, dg, p.M, p.F, p.F, kFM / 2)) ||
+                 (rc = enc_map_2d(&m.a[1], dtype, du, p.M, p.F, p.F, kFM / 2)) ||
+                 (rc = enc_map_2d(&m.b[0], dtype, wg, p.F, p.K, p.K, kFK)) ||
+                 (rc = enc_map_2d(&m.b[1], dtype, wu, p.F, p.K, p.K, kFK)) ||
+                 (pair && (rc = enc_map_2d(&m.out[0], dtype, p.out[0], p.M, p.K, p.K, 32)))))
+        return rc;
+    if (p.dw && ((rc = enc_map_2d(&m.a[2], dtype, dg, p.M, p.F, p.F, kFK)) ||
+                 (rc = enc_map_2d(&m.a[3], dtype, du, p.M, p.F, p.F, kFK)) ||
+                 (rc = enc_map_2d(&m.b[2], dtype, x, p.M, p.K, p.K, kFK)) ||
+                 (pair && ((rc = enc_map_2d(&m.out[1], dtype, p.out[1], p.F, p.K, p.K, 32)) ||
+                           (rc = enc_map_2d(&m.out[2], dtype, p.out[2], p.F, p.K, p.K, 32))))))
+        return rc;
+    return RAGRT_OK;
 }
 
-template <int kMode>
-int ffn_launch_typed(int dtype, const FfnMaps& maps, const FfnParams& p, cudaStream_t stream) {
-    return dtype == RAGRT_BF16 ? ffn_launch<__nv_bfloat16, kMode>(maps, p, stream)
-                               : ffn_launch<__half, kMode>(maps, p, stream);
+int64_t ffn_tiles(int mode, const FfnParams& p, int tile_m, int tile_n) {
+    if (mode == kForward) return ceil_div(p.M, tile_m) * ceil_div(p.F, tile_n);
+    return ((p.dx ? ceil_div(p.M, tile_m) : 0) + (p.dw ? 2 * ceil_div(p.F, tile_m) : 0)) * ceil_div(p.K, tile_n);
+}
+
+template <typename T, int kMode>
+int ffn_launch(int dtype, const FfnParams& p, const void* x, const void* wg, const void* wu, const void* dg,
+               const void* du, cudaStream_t stream) {
+    FfnMaps m = {};
+    int rc;
+    const int64_t large = ffn_tiles(kMode, p, kFM, kMode == kForward ? kFN / 2 : kFN), pairs = num_sms() / 2;
+    if (2 * large >= pairs) {
+        static std::atomic<uint64_t> done{0};
+        if (large > 0x3FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many tiles");
+        if ((rc = enc_allow_smem(ffn_pair<T, kMode>, kFSmem, done)) ||
+            (rc = ffn_maps(m, kMode, true, dtype, p, x, wg, wu, dg, du)))
+            return rc;
+        return enc_launch(ffn_pair<T, kMode>, dim3((unsigned)(2 * std::min(large, pairs))), dim3(kFThreads), kFSmem,
+                          stream, m, p);
+    }
+    static std::atomic<uint64_t> done{0};
+    const int64_t small = ffn_tiles(kMode, p, kFM / 2, kMode == kForward ? kSN / 2 : kSN);
+    if ((rc = enc_allow_smem(ffn_small<T, kMode>, kSSmem, done)) ||
+        (rc = ffn_maps(m, kMode, false, dtype, p, x, wg, wu, dg, du)))
+        return rc;
+    return enc_launch(ffn_small<T, kMode>, dim3((unsigned)std::min<int64_t>(small, 2 * num_sms())), dim3(kSThreads), kSSmem,
+                      stream, m, p);
 }
 
 int ffn_check(int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype) {
@@ -392,17 +709,19 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
                   "gated_ffn operands must be 16-byte aligned");
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
-    FfnMaps m;
-    if ((rc = enc_map_2d(&m.a[0], dtype, d_x, M, K, K, kFM / 2)) ||
-        (rc = enc_map_2d(&m.b[0], dtype, d_w_gate, F, K, K, kFN / 2)) ||
-        (rc = enc_map_2d(&m.b[1], dtype, d_w_up, F, K, K, kFN / 2)) ||
-        (rc = enc_map_2d(&m.out[0], dtype, d_h, M, F, F, 32)) ||
-        (rc = enc_map_2d(&m.out[1], dtype, d_gate ? d_gate : d_h, M, F, F, 32)) ||
-        (rc = enc_map_2d(&m.out[2], dtype, d_up ? d_up : d_h, M, F, F, 32)))
-        return rc;
-    m.a[1] = m.a[0];
-    FfnParams p{M, F, K, act, d_gate != nullptr, err};
-    return ffn_launch_typed<kGated>(dtype, m, p, (cudaStream_t)stream_);
+    cudaStream_t stream = (cudaStream_t)stream_;
+    FfnParams p{M, F, K, act, d_gate != nullptr, 0, 0, {d_h, d_gate, d_up}, err};
+    if (M <= kFewRows) {
+        const unsigned blocks = (unsigned)ceil_div(F, 8);
+        return dtype == RAGRT_BF16
+                   ? enc_launch(ffn_rows<__nv_bfloat16, kFewRows>, dim3(blocks), dim3(256), 0, stream,
+                                (const __nv_bfloat16*)d_x, (const __nv_bfloat16*)d_w_gate, (const __nv_bfloat16*)d_w_up, p)
+                   : enc_launch(ffn_rows<__half, kFewRows>, dim3(blocks), dim3(256), 0, stream, (const __half*)d_x,
+                                (const __half*)d_w_gate, (const __half*)d_w_up, p);
+    }
+    return dtype == RAGRT_BF16
+               ? ffn_launch<__nv_bfloat16, kForward>(dtype, p, d_x, d_w_gate, d_w_up, nullptr, nullptr, stream)
+               : ffn_launch<__half, kForward>(dtype, p, d_x, d_w_gate, d_w_up, nullptr, nullptr, stream);
 }
 
 extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* d_w_gate,
@@ -438,29 +757,9 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
              : enc_launch(ffn_act_backward<__half>, dim3(blocks), dim3(256), 0, stream, (const __half*)d_dh,
                           (const __half*)d_gate, (const __half*)d_up, (__half*)d_dgate, (__half*)d_dup, n8, (int)act);
     if (rc) return rc;
-    FfnMaps m;
-    if (d_dx) {
-        if ((rc = enc_map_2d(&m.a[0], dtype, d_dgate, M, F, F, kFM / 2)) ||
-            (rc = enc_map_2d(&m.a[1], dtype, d_dup, M, F, F, kFM / 2)) ||
-            (rc = enc_map_2d(&m.b[0], dtype, d_w_gate, F, K, K, kFK)) ||
-            (rc = enc_map_2d(&m.b[1], dtype, d_w_up, F, K, K, kFK)) ||
-            (rc = enc_map_2d(&m.out[0], dtype, d_dx, M, K, K, 32)))
-            return rc;
-        m.out[1] = m.out[2] = m.out[0];
-        FfnParams p{M, K, F, act, 0, err};
-        if ((rc = ffn_launch_typed<kDx>(dtype, m, p, stream))) return rc;
-    }
-    if (d_dw_gate) {
-        if ((rc = enc_map_2d(&m.a[0], dtype, d_dgate, M, F, F, kFK)) ||
-            (rc = enc_map_2d(&m.a[1], dtype, d_dup, M, F, F, kFK)) ||
-            (rc = enc_map_2d(&m.b[0], dtype, d_x, M, K, K, kFK)) ||
-            (rc = enc_map_2d(&m.out[0], dtype, d_dw_gate, F, K, K, 32)) ||
-            (rc = enc_map_2d(&m.out[1], dtype, d_dw_up, F, K, K, 32)))
-            return rc;
-        m.b[1] = m.b[0];
-        m.out[2] = m.out[1];
-        FfnParams p{F, K, M, act, 0, err};
-        if ((rc = ffn_launch_typed<kDw>(dtype, m, p, stream))) return rc;
-    }
-    return RAGRT_OK;
+    if (!d_dx && !d_dw_gate) return RAGRT_OK;
+    FfnParams p{M, F, K, act, 0, d_dx != nullptr, d_dw_gate != nullptr, {d_dx, d_dw_gate, d_dw_up}, err};
+    return dtype == RAGRT_BF16
+               ? ffn_launch<__nv_bfloat16, kBackward>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, stream)
+               : ffn_launch<__half, kBackward>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, stream);
 }
