@@ -57,6 +57,7 @@ struct FfnParams {
     int act;
     int keep;                  // kForward: g and u are written too
     int dx, dw;                // kBackward: which gradients
+    int a_rows;                // ffn_small: rows of x, dg, du that a load brings
     void* out[3];              // as in FfnMaps
     int* err;
 };
@@ -427,7 +428,7 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
                     const int k = (second ? i - tile.chunks : i) * kFK;
                     uint8_t* da = sA + s * kSTileA;
                     uint8_t* db = sB + s * kSTileB;
-                    tc::mbar_arrive_expect_tx(full + s, kSTileA + kSTileB);
+                    tc::mbar_arrive_expect_tx(full + s, (dw ? kSTileA : p.a_rows * kFK * 2) + kSTileB);
                     if (dw) {
                         tc::tma_load_2d(da, &maps.a[1 + tile.out], tile.m0, k, full + s);
                         tc::tma_load_2d(da + 8192, &maps.a[1 + tile.out], tile.m0 + 64, k, full + s);
@@ -535,69 +536,85 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
 }
 
 // ------------------------------------------------------------------ few rows
-// A warp per output column: it reads one row of Wg and one of Wu, 8 values a lane and step, against the
+// A warp per kCols output columns: it reads their rows of Wg and Wu, 8 values a lane and step, against the
 // same values of up to kRows rows of x.
-template <typename T, int kRows>
+template <typename T, int kRows, int kCols>
 __global__ void __launch_bounds__(256) ffn_rows(const T* __restrict__ x, const T* __restrict__ wg,
                                                 const T* __restrict__ wu, const __grid_constant__ FfnParams p) {
-    const int f = (int)((blockIdx.x * 256 + threadIdx.x) >> 5), lane = threadIdx.x & 31;
+    const int f0 = (int)((blockIdx.x * 256 + threadIdx.x) >> 5) * kCols, lane = threadIdx.x & 31;
     pdl_wait_then_release();
-    if (f >= p.F) return;
-    const T* g = wg + (int64_t)f * p.K;
-    const T* u = wu + (int64_t)f * p.K;
-    uint64_t sg[kRows] = {}, su[kRows] = {};
+    if (f0 >= p.F) return;                           // F is a multiple of 8
+    const T* w[2] = {wg + (int64_t)f0 * p.K, wu + (int64_t)f0 * p.K};
+    uint64_t sum[kRows][2][kCols] = {};
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    constexpr int kAhead = 4;                        // steps whose weights are in flight together
+    constexpr int kAhead = 4 / kCols;                // steps whose weights are in flight together
     for (int k0 = lane * 8; k0 < p.K + lane * 8; k0 += 256 * kAhead) {
-        uint4 a[kAhead], b[kAhead];
+        uint4 a[kAhead][2][kCols], xr[kAhead][kRows];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const bool in = k0 + 256 * i < p.K;
-            a[i] = in ? __ldg(reinterpret_cast<const uint4*>(g + k0 + 256 * i)) : zero;
-            b[i] = in ? __ldg(reinterpret_cast<const uint4*>(u + k0 + 256 * i)) : zero;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int c = 0; c < kCols; ++c)
+                    a[i][m][c] = in ? __ldg(reinterpret_cast<const uint4*>(w[m] + (int64_t)c * p.K + k0 + 256 * i)) : zero;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+                xr[i][r] = in && r < p.M ? __ldg(reinterpret_cast<const uint4*>(x + (int64_t)r * p.K + k0 + 256 * i)) : zero;
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            if (k0 + 256 * i >= p.K) break;
-            float fa[8], fb[8];
-            up8<T>(a[i], fa);
-            up8<T>(b[i], fb);
+            if (k0 + 256 * i >= p.K) break;          // a row of x behind M adds nothing, weights of no value could
+            float fx[kRows][8];
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                if (r >= p.M) break;
-                float fx[8];
-                up8<T>(__ldg(reinterpret_cast<const uint4*>(x + (int64_t)r * p.K + k0 + 256 * i)), fx);
+            for (int r = 0; r < kRows; ++r) up8<T>(xr[i][r], fx[r]);
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const uint64_t x2 = pack2(fx[e], fx[e + 1]);
-                    sg[r] = fma2(pack2(fa[e], fa[e + 1]), x2, sg[r]);
-                    su[r] = fma2(pack2(fb[e], fb[e + 1]), x2, su[r]);
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int c = 0; c < kCols; ++c) {
+                    float fw[8];
+                    up8<T>(a[i][m][c], fw);
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2)
+                            sum[r][m][c] = fma2(pack2(fw[e], fw[e + 1]), pack2(fx[r][e], fx[r][e + 1]), sum[r][m][c]);
                 }
-            }
         }
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         if (r >= p.M) break;
-        float a, b, c, d;
-        unpack2(sg[r], a, b);
-        unpack2(su[r], c, d);
-        a += b;
-        c += d;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-            c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
-        }
-        if (lane == 0) {
-            const int64_t at = (int64_t)r * p.F + f;
-            if (p.keep) {
-                static_cast<T*>(p.out[1])[at] = (T)a;
-                static_cast<T*>(p.out[2])[at] = (T)c;
+        for (int c = 0; c < kCols; ++c) {
+            float v[2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                float a, b;
+                unpack2(sum[r][m][c], a, b);
+                v[m] = a + b;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) v[m] += __shfl_xor_sync(0xFFFFFFFFu, v[m], o);
             }
-            static_cast<T*>(p.out[0])[at] = (T)(ffn_act(a, p.act) * c);
+            if (lane == 0) {
+                const int64_t at = (int64_t)r * p.F + f0 + c;
+                if (p.keep) {
+                    static_cast<T*>(p.out[1])[at] = (T)v[0];
+                    static_cast<T*>(p.out[2])[at] = (T)v[1];
+                }
+                static_cast<T*>(p.out[0])[at] = (T)(ffn_act(v[0], p.act) * v[1]);
+            }
         }
     }
+}
+
+template <typename T>
+int ffn_rows_launch(const void* x, const void* wg, const void* wu, const FfnParams& p, cudaStream_t stream) {
+    if (p.M == 1)
+        return enc_launch(ffn_rows<T, 1, 1>, dim3((unsigned)ceil_div(p.F, 8)), dim3(256), 0, stream, (const T*)x,
+                          (const T*)wg, (const T*)wu, p);
+    return enc_launch(ffn_rows<T, kFewRows, 2>, dim3((unsigned)ceil_div(p.F, 16)), dim3(256), 0, stream, (const T*)x,
+                      (const T*)wg, (const T*)wu, p);
 }
 
 // dg = dh * u * act'(g), du = dh * act(g); a thread per 8 values
@@ -629,7 +646,7 @@ int ffn_maps(FfnMaps& m, int mode, bool pair, int dtype, const FfnParams& p, con
     int rc;
     if (mode == kForward) {
         const int wrows = pair ? kFN / 2 : kSN / 2;
-        if ((rc = enc_map_2d(&m.a[0], dtype, x, p.M, p.K, p.K, kFM / 2)) ||
+        if ((rc = enc_map_2d(&m.a[0], dtype, x, p.M, p.K, p.K, pair ? kFM / 2 : p.a_rows)) ||
             (rc = enc_map_2d(&m.b[0], dtype, wg, p.F, p.K, p.K, wrows)) ||
             (rc = enc_map_2d(&m.b[1], dtype, wu, p.F, p.K, p.K, wrows)))
             return rc;
@@ -638,8 +655,8 @@ int ffn_maps(FfnMaps& m, int mode, bool pair, int dtype, const FfnParams& p, con
                 if ((rc = enc_map_2d(&m.out[i], dtype, p.out[i], p.M, p.F, p.F, 32))) return rc;
         return RAGRT_OK;
     }
-    if (p.dx && ((rc = enc_map_2d(&m.a[0], dtype, dg, p.M, p.F, p.F, kFM / 2)) ||
-                 (rc = enc_map_2d(&m.a[1], dtype, du, p.M, p.F, p.F, kFM / 2)) ||
+    if (p.dx && ((rc = enc_map_2d(&m.a[0], dtype, dg, p.M, p.F, p.F, pair ? kFM / 2 : p.a_rows)) ||
+                 (rc = enc_map_2d(&m.a[1], dtype, du, p.M, p.F, p.F, pair ? kFM / 2 : p.a_rows)) ||
                  (rc = enc_map_2d(&m.b[0], dtype, wg, p.F, p.K, p.K, kFK)) ||
                  (rc = enc_map_2d(&m.b[1], dtype, wu, p.F, p.K, p.K, kFK)) ||
                  (pair && (rc = enc_map_2d(&m.out[0], dtype, p.out[0], p.M, p.K, p.K, 32)))))
@@ -659,27 +676,43 @@ int64_t ffn_tiles(int mode, const FfnParams& p, int tile_m, int tile_n) {
 }
 
 template <typename T, int kMode>
-int ffn_launch(int dtype, const FfnParams& p, const void* x, const void* wg, const void* wu, const void* dg,
-               const void* du, cudaStream_t stream) {
+int ffn_launch(int dtype, FfnParams p, const void* x, const void* wg, const void* wu, const void* dg, const void* du,
+               cudaStream_t stream) {
     FfnMaps m = {};
     int rc;
-    const int64_t large = ffn_tiles(kMode, p, kFM, kMode == kForward ? kFN / 2 : kFN), pairs = num_sms() / 2;
-    if (2 * large >= pairs) {
+    const int64_t sms = num_sms(), pairs = sms / 2;
+    const int64_t large = ffn_tiles(kMode, p, kFM, kMode == kForward ? kFN / 2 : kFN);
+    const int64_t small = ffn_tiles(kMode, p, kFM / 2, kMode == kForward ? kSN / 2 : kSN);
+    bool pair;
+    if (kMode == kForward) {
+        // small tiles while they are one round of two CTAs per SM: 128 rows 2048 -> 5504 (172 tiles) 12.9 us
+        // against 16.2, 512 rows 768 -> 2048 (256) 7.2 against 9.3; 256 rows 2048 -> 5504 (344) 19.9
+        // against 16.5, 1000 rows 768 -> 2048 (512) 11.5 against 10.3
+        pair = small > 2 * sms;
+    } else {
+        // small tiles where the large ones' longest contraction is far above their average per pair of SMs
+        // (five times): all gradients of 512 rows 768 -> 2048 (6.4 times) 25.8 us against 27.5, 128 rows
+        // 2048 -> 5504 (6.1) 67.7 against 70.8; 1000 rows (3.1) 29.2 against 28.9, 256 rows (4.6) 82.3
+        // against 73.1
+        const int64_t of_dx = 2 * ceil_div(p.F, kFK), of_dw = ceil_div(p.M, kFK);
+        const int64_t n_dx = p.dx ? ceil_div(p.M, kFM) * ceil_div(p.K, kFN) : 0;
+        const int64_t sum = n_dx * of_dx + (large - n_dx) * of_dw;
+        pair = 5 * sum >= pairs * std::max(p.dx ? of_dx : 0, p.dw ? of_dw : 0);
+    }
+    if (std::max(large, small) > 0x3FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many tiles");
+    // few rows: a load brings no more of them than there are (one row of 2048 -> 5504 10.6 us; with
+    // 128-row boxes, most of them outside the tensor, 30)
+    p.a_rows = std::min(kFM / 2, (int)ceil_div(p.M, 8) * 8);
+    if ((rc = ffn_maps(m, kMode, pair, dtype, p, x, wg, wu, dg, du))) return rc;
+    if (pair) {
         static std::atomic<uint64_t> done{0};
-        if (large > 0x3FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many tiles");
-        if ((rc = enc_allow_smem(ffn_pair<T, kMode>, kFSmem, done)) ||
-            (rc = ffn_maps(m, kMode, true, dtype, p, x, wg, wu, dg, du)))
-            return rc;
+        if ((rc = enc_allow_smem(ffn_pair<T, kMode>, kFSmem, done))) return rc;
         return enc_launch(ffn_pair<T, kMode>, dim3((unsigned)(2 * std::min(large, pairs))), dim3(kFThreads), kFSmem,
                           stream, m, p);
     }
     static std::atomic<uint64_t> done{0};
-    const int64_t small = ffn_tiles(kMode, p, kFM / 2, kMode == kForward ? kSN / 2 : kSN);
-    if ((rc = enc_allow_smem(ffn_small<T, kMode>, kSSmem, done)) ||
-        (rc = ffn_maps(m, kMode, false, dtype, p, x, wg, wu, dg, du)))
-        return rc;
-    return enc_launch(ffn_small<T, kMode>, dim3((unsigned)std::min<int64_t>(small, 2 * num_sms())), dim3(kSThreads), kSSmem,
-                      stream, m, p);
+    if ((rc = enc_allow_smem(ffn_small<T, kMode>, kSSmem, done))) return rc;
+    return enc_launch(ffn_small<T, kMode>, dim3((unsigned)std::min(small, 2 * sms)), dim3(kSThreads), kSSmem, stream, m, p);
 }
 
 int ffn_check(int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype) {
@@ -710,14 +743,10 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
     cudaStream_t stream = (cudaStream_t)stream_;
-    FfnParams p{M, F, K, act, d_gate != nullptr, 0, 0, {d_h, d_gate, d_up}, err};
+    FfnParams p{M, F, K, act, d_gate != nullptr, 0, 0, 0, {d_h, d_gate, d_up}, err};
     if (M <= kFewRows) {
-        const unsigned blocks = (unsigned)ceil_div(F, 8);
-        return dtype == RAGRT_BF16
-                   ? enc_launch(ffn_rows<__nv_bfloat16, kFewRows>, dim3(blocks), dim3(256), 0, stream,
-                                (const __nv_bfloat16*)d_x, (const __nv_bfloat16*)d_w_gate, (const __nv_bfloat16*)d_w_up, p)
-                   : enc_launch(ffn_rows<__half, kFewRows>, dim3(blocks), dim3(256), 0, stream, (const __half*)d_x,
-                                (const __half*)d_w_gate, (const __half*)d_w_up, p);
+        return dtype == RAGRT_BF16 ? ffn_rows_launch<__nv_bfloat16>(d_x, d_w_gate, d_w_up, p, stream)
+                                   : ffn_rows_launch<__half>(d_x, d_w_gate, d_w_up, p, stream);
     }
     return dtype == RAGRT_BF16
                ? ffn_launch<__nv_bfloat16, kForward>(dtype, p, d_x, d_w_gate, d_w_up, nullptr, nullptr, stream)
@@ -758,7 +787,7 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
                           (const __half*)d_gate, (const __half*)d_up, (__half*)d_dgate, (__half*)d_dup, n8, (int)act);
     if (rc) return rc;
     if (!d_dx && !d_dw_gate) return RAGRT_OK;
-    FfnParams p{M, F, K, act, 0, d_dx != nullptr, d_dw_gate != nullptr, {d_dx, d_dw_gate, d_dw_up}, err};
+    FfnParams p{M, F, K, act, 0, d_dx != nullptr, d_dw_gate != nullptr, 0, {d_dx, d_dw_gate, d_dw_up}, err};
     return dtype == RAGRT_BF16
                ? ffn_launch<__nv_bfloat16, kBackward>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, stream)
                : ffn_launch<__half, kBackward>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, stream);
