@@ -157,6 +157,11 @@ def _dtype16(*ts):
     return _DTYPES[want]
 
 
+def _raw_stream(t):
+    """torch's current stream of t's device (which _need_cuda has found to be the current one), as a number."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
 def _row_stride(t):
     """Row stride in elements of [T, H, D] rows that can be used in place (heads side by side, rows
     apart by a multiple of 16 bytes that holds them all, 16-byte aligned); 0 if they cannot."""
@@ -226,23 +231,26 @@ def packed_attention(q, k, v, cu_seqlens, causal=False, scale=None, out=None):
     device error flag (6) and leaves rows unwritten.  Not differentiable."""
     _need_cuda(q, k, v, cu_seqlens, out)
     dt = _dtype16(q, k, v)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise RuntimeError(f"q [T, H, D], k and v [T, KV, D] wanted; got {tuple(q.shape)}, {tuple(k.shape)}, "
+    shape, kshape = q.shape, k.shape
+    if len(shape) != 3 or len(kshape) != 3 or kshape != v.shape or shape[0] != kshape[0] or shape[2] != kshape[2]:
+        raise RuntimeError(f"q [T, H, D], k and v [T, KV, D] wanted; got {tuple(shape)}, {tuple(kshape)}, "
                            f"{tuple(v.shape)}")
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise RuntimeError("cu_seqlens must be int32 [B + 1]")
     if cu_seqlens.dtype is not torch.int32 or not cu_seqlens.is_contiguous():
         cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
     (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
-    T, H, D = q.shape
+    T, H, D = shape
     if out is None:
-        out, os = q.new_empty((T, H, D)), H * D
+        out, os = torch.empty_like(q, memory_format=torch.contiguous_format), H * D
     else:
-        _check_output(out, q.shape, q.dtype, (q, k, v))
+        _check_output(out, shape, q.dtype, (q, k, v))
         os = _row_stride(out)
-    _lib.check(_lib.lib().ragrt_enc_packed_attention(
+    rc = _lib.lib().ragrt_enc_packed_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), out.data_ptr(), T, cu_seqlens.shape[0] - 1, H,
-        k.shape[1], D, qs, ks, vs, os, D ** -0.5 if scale is None else scale, bool(causal), dt, _stream()))
+        kshape[1], D, qs, ks, vs, os, D ** -0.5 if scale is None else scale, bool(causal), dt, _raw_stream(q))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -255,10 +263,11 @@ def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     of 16.  A position outside the table reads its row 0 and raises the device error flag (5)."""
     _need_cuda(q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out)
     dt = _dtype16(q, k, q_weight, k_weight)
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise RuntimeError(f"q [T, H, D] and k [T, KV, D] wanted; got {tuple(q.shape)}, {tuple(k.shape)}")
-    T, H, D = q.shape
-    KV = k.shape[1]
+    shape, kshape = q.shape, k.shape
+    if len(shape) != 3 or len(kshape) != 3 or shape[0] != kshape[0] or shape[2] != kshape[2]:
+        raise RuntimeError(f"q [T, H, D] and k [T, KV, D] wanted; got {tuple(shape)}, {tuple(kshape)}")
+    T, H, D = shape
+    KV = kshape[1]
     if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise RuntimeError("cos and sin must be f32 [max_pos, R / 2]")
     if positions.shape != (T,) or positions.dtype not in (torch.int32, torch.int64):
@@ -269,29 +278,32 @@ def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     (q, qs), (k, ks) = _rows(q), _rows(k)
     cos, sin, qw, kw, pos = _solid(cos), _solid(sin), _solid(q_weight), _solid(k_weight), positions.contiguous()
     if q_out is None:
-        q_out, qos = q.new_empty((T, H, D)), H * D
+        q_out, qos = torch.empty_like(q, memory_format=torch.contiguous_format), H * D
     else:
-        _check_output(q_out, q.shape, q.dtype, (q, k), in_place_of=q)
+        _check_output(q_out, shape, q.dtype, (q, k), in_place_of=q)
         qos = _row_stride(q_out)
     if k_out is None:
-        k_out, kos = k.new_empty((T, KV, D)), KV * D
+        k_out, kos = torch.empty_like(k, memory_format=torch.contiguous_format), KV * D
     else:
-        _check_output(k_out, k.shape, k.dtype, (q, k, q_out), in_place_of=k)
+        _check_output(k_out, kshape, k.dtype, (q, k, q_out), in_place_of=k)
         kos = _row_stride(k_out)
-    _lib.check(_lib.lib().ragrt_enc_qk_norm_rope(
+    rc = _lib.lib().ragrt_enc_qk_norm_rope(
         q.data_ptr(), k.data_ptr(), qw if qw is None else qw.data_ptr(), kw if kw is None else kw.data_ptr(),
         cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), pos.element_size(), q_out.data_ptr(), k_out.data_ptr(), T, H,
-        KV, D, 2 * cos.shape[1], cos.shape[0], qs, ks, qos, kos, eps, bool(interleaved), dt, _stream()))
+        KV, D, 2 * cos.shape[1], cos.shape[0], qs, ks, qos, kos, eps, bool(interleaved), dt, _raw_stream(q))
+    if rc:
+        _lib.check(rc)
     return q_out, k_out
 
 
 def _ffn_args(x, w_gate, w_up, act):
     if act not in _ACTS:
         raise RuntimeError(f"unknown activation {act!r}: one of {sorted(_ACTS)}")
-    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != x.shape[1]:
-        raise RuntimeError(f"x [M, K], w_gate and w_up [F, K] wanted; got {tuple(x.shape)}, {tuple(w_gate.shape)}, "
+    shape, wshape = x.shape, w_gate.shape
+    if len(shape) != 2 or len(wshape) != 2 or wshape != w_up.shape or wshape[1] != shape[1]:
+        raise RuntimeError(f"x [M, K], w_gate and w_up [F, K] wanted; got {tuple(shape)}, {tuple(wshape)}, "
                            f"{tuple(w_up.shape)}")
-    return x.shape[0], w_gate.shape[0], x.shape[1]
+    return shape[0], wshape[0], shape[1]
 
 
 def gated_ffn(x, w_gate, w_up, act="silu", keep=False, out=None):
@@ -309,10 +321,12 @@ def gated_ffn(x, w_gate, w_up, act="silu", keep=False, out=None):
         _check_output(out, (M, F), x.dtype, (x, wg, wu))
     gate = up = None
     if keep:
-        gate, up = x.new_empty((M, F)), x.new_empty((M, F))
-    _lib.check(_lib.lib().ragrt_enc_gated_ffn(
+        gate, up = torch.empty_like(out), torch.empty_like(out)
+    rc = _lib.lib().ragrt_enc_gated_ffn(
         x.data_ptr(), wg.data_ptr(), wu.data_ptr(), out.data_ptr(), gate.data_ptr() if keep else None,
-        up.data_ptr() if keep else None, M, F, K, _ACTS[act], dt, _stream()))
+        up.data_ptr() if keep else None, M, F, K, _ACTS[act], dt, _raw_stream(x))
+    if rc:
+        _lib.check(rc)
     return (out, gate, up) if keep else out
 
 
@@ -326,12 +340,13 @@ def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu", need_dx=True, 
         raise RuntimeError(f"dh, gate and up must be {(M, F)}; got {tuple(dh.shape)}, {tuple(gate.shape)}, "
                            f"{tuple(up.shape)}")
     dh, x, wg, wu, gate, up = (_solid(t) for t in (dh, x, w_gate, w_up, gate, up))
-    dgate, dup = gate.new_empty((M, F)), up.new_empty((M, F))
-    dx = x.new_empty((M, K)) if need_dx else None
-    dwg, dwu = (wg.new_empty((F, K)), wu.new_empty((F, K))) if need_dw else (None, None)
+    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
+    dx = torch.empty_like(x) if need_dx else None
+    dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_dw else (None, None)
     _lib.check(_lib.lib().ragrt_enc_gated_ffn_backward(
-        _ptr(dh), _ptr(x), _ptr(wg), _ptr(wu), _ptr(gate), _ptr(up), _ptr(dgate), _ptr(dup), _ptr(dx), _ptr(dwg),
-        _ptr(dwu), M, F, K, _ACTS[act], dt, _stream()))
+        dh.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), gate.data_ptr(), up.data_ptr(), dgate.data_ptr(),
+        dup.data_ptr(), dx.data_ptr() if need_dx else None, dwg.data_ptr() if need_dw else None,
+        dwu.data_ptr() if need_dw else None, M, F, K, _ACTS[act], dt, _raw_stream(x)))
     return dx, dwg, dwu
 
 
