@@ -135,7 +135,6 @@ __device__ __noinline__ void attn_row(const AttnParams& p, int t, int h, int lo,
 
 constexpr int kAFirst = 4;                     // first softmax warp: TMA, MMA and search warp before them, one idle
 constexpr int kAItems = 4;                     // items whose tiles are in shared memory
-constexpr uint32_t kAWaitLimit = 1u << 26;
 // The reference maximum of a row moves only when it is exceeded by a factor of 2^8: until then the weights are
 // at most 256, well inside either type, and the accumulator is not rescaled.
 constexpr float kARescale = 8.0f;
@@ -166,6 +165,24 @@ struct AttnMaps {
     CUtensorMap q, k, v;
 };
 
+// Bounded wait: 2 s, not counting the time that a warp of the CTA spends in attn_row (abort[1]: how many
+// do), or until another role gave up (abort[0]).  In few instructions: the roles' code shares the
+// instruction cache, and this is in it some twenty times.
+__device__ __forceinline__ bool attn_wait(uint64_t* m, uint32_t parity, volatile int* abort) {
+    if (tc::mbar_try_wait_hint(m, parity, tc::kWaitHintNs)) return true;
+    uint32_t since, now;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(since));
+    for (uint32_t i = 0; i < (1u << 30); ++i) {
+        if (tc::mbar_try_wait_hint(m, parity, tc::kWaitHintNs)) return true;
+        if (abort[0]) return false;
+        asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(now));
+        if (abort[1]) since = now;
+        if (now - since > (uint32_t)tc::kWaitDeadlineNs) break;
+    }
+    abort[0] = 1;
+    return false;
+}
+
 // What the roles hand one another, behind the tiles in shared memory.
 template <int DP>
 struct AttnShared {
@@ -180,7 +197,7 @@ struct AttnShared {
     uint64_t odone[kTiles];                  // product with V done
     uint64_t drain;
     uint32_t tmem;
-    int abort;
+    int abort[2];                            // given up; warps in attn_row
 };
 
 // The blocks of an item: blocks 0 .. n - 1 from key kv0 on, tile t takes [jb[t], je[t]) of them.
@@ -219,7 +236,7 @@ struct AttnWalk {
         }
         if (kRelease && rec >= 0 && lead) tc::mbar_arrive(&sh->iempty[rec % kAItems]);
         ++rec;
-        if (!tc::mbar_wait_or_abort(&sh->ifull[rec % kAItems], (rec / kAItems) & 1, &sh->abort, kAWaitLimit)) return -1;
+        if (!attn_wait(&sh->ifull[rec % kAItems], (rec / kAItems) & 1, sh->abort)) return -1;
         b.get(sh, rec % kAItems);
         j = 0;
         return b.head >= 0;
@@ -267,7 +284,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     uint8_t* sV = sK + S * Cfg::kTileK;
     AttnShared<DP>* sh = reinterpret_cast<AttnShared<DP>*>(sV + S * Cfg::kTileK);
     static_assert(sizeof(AttnShared<DP>) <= 1024, "shared memory of the roles");
-    volatile int* abort = &sh->abort;
+    volatile int* abort = sh->abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -289,7 +306,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             tc::mbar_init(&sh->odone[t], 1);
         }
         tc::mbar_init(&sh->drain, 1);
-        sh->abort = 0;
+        sh->abort[0] = sh->abort[1] = 0;
         tc::mbar_fence_init();
     }
     if (warp == 1) {
@@ -315,7 +332,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             auto load = [&](const AttnBlocks<DP>& b, int j, int i, const CUtensorMap* map, uint8_t* ring, uint64_t* full,
                             uint64_t* empty) {
                 const int s = i % S;
-                if (i >= S && !tc::mbar_wait_or_abort(empty + s, (i / S - 1) & 1, abort, kAWaitLimit)) return false;
+                if (i >= S && !attn_wait(empty + s, (i / S - 1) & 1, abort)) return false;
                 tc::mbar_arrive_expect_tx(full + s, Cfg::kTileK);
                 for (int c = 0; c < DP / 64; ++c)
                     tc::tma_load_3d(ring + s * Cfg::kTileK + c * N * 128, map, 64 * c, b.head / per, b.kv0 + j * N,
@@ -339,7 +356,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 }
                 ++nk;
                 if (kw.j == 0) {                                  // a new item: its Q
-                    if (nq > 0 && !tc::mbar_wait_or_abort(&sh->qempty, (nq - 1) & 1, abort, kAWaitLimit)) {
+                    if (nq > 0 && !attn_wait(&sh->qempty, (nq - 1) & 1, abort)) {
                         failed = true;
                         break;
                     }
@@ -387,7 +404,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 const bool begun = vw.j > vw.b.jb[t];
 #pragma unroll
                 for (int x = 0; x < Cfg::kHalves; ++x) {
-                    const bool ok = tc::mbar_wait_or_abort(&sh->pready[t][x], np[t] & 1, abort, kAWaitLimit);
+                    const bool ok = attn_wait(&sh->pready[t][x], np[t] & 1, abort);
                     if (!__all_sync(0xFFFFFFFFu, ok)) return false;
                     tc::fence_after();
 #pragma unroll
@@ -400,8 +417,8 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 return true;
             };
             auto k_arrived = [&] {
-                const bool ok = tc::mbar_wait_or_abort(&sh->kfull[nk % S], (nk / S) & 1, abort, kAWaitLimit) &&
-                                (sw.j != 0 || tc::mbar_wait_or_abort(&sh->qfull, nq & 1, abort, kAWaitLimit));
+                const bool ok = attn_wait(&sh->kfull[nk % S], (nk / S) & 1, abort) &&
+                                (sw.j != 0 || attn_wait(&sh->qfull, nq & 1, abort));
                 if (!__all_sync(0xFFFFFFFFu, ok)) return false;
                 tc::fence_after();
                 return true;
@@ -416,7 +433,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 // one's products run while the other's weights are computed.
                 const bool apart = more > 0 && (kTiles == 1 || sw.j == 0);
                 if (there > 0) {
-                    const bool ok = tc::mbar_wait_or_abort(&sh->vfull[nv % S], (nv / S) & 1, abort, kAWaitLimit);
+                    const bool ok = attn_wait(&sh->vfull[nv % S], (nv / S) & 1, abort);
                     failed = !__all_sync(0xFFFFFFFFu, ok) || (kTiles > 1 && more > 0 && !apart && !k_arrived());
                     if (failed) break;
                     tc::fence_after();
@@ -476,7 +493,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 }
                 const int r = rec % kAItems;
                 const bool ok = rec < kAItems ||
-                                tc::mbar_wait_or_abort(&sh->iempty[r], (rec / kAItems - 1) & 1, abort, kAWaitLimit);
+                                attn_wait(&sh->iempty[r], (rec / kAItems - 1) & 1, abort);
                 if (!__all_sync(0xFFFFFFFFu, ok)) {
                     failed = true;
                     break;
@@ -503,7 +520,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         uint32_t blk = 0, outs = 0;                               // blocks and items of this tile
         for (int rec = 0; !failed; ++rec) {
             const int r = rec % kAItems;
-            bool ok = tc::mbar_wait_or_abort(&sh->ifull[r], (rec / kAItems) & 1, abort, kAWaitLimit);
+            bool ok = attn_wait(&sh->ifull[r], (rec / kAItems) & 1, abort);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 failed = true;
                 break;
@@ -523,7 +540,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             float m = -INFINITY, l = 0.f;
             const int b0 = tile == 0 ? b.jb[0] : b.jb[kTiles - 1], b1 = tile == 0 ? b.je[0] : b.je[kTiles - 1];
             for (int j = b0; j < b1; ++j, ++blk) {
-                ok = tc::mbar_wait_or_abort(&sh->sfull[tile], blk & 1, abort, kAWaitLimit);
+                ok = attn_wait(&sh->sfull[tile], blk & 1, abort);
                 if (!__all_sync(0xFFFFFFFFu, ok)) {
                     failed = true;
                     break;
@@ -637,7 +654,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 }
             }
             if (failed) break;
-            ok = tc::mbar_wait_or_abort(&sh->odone[tile], outs++ & 1, abort, kAWaitLimit);
+            ok = attn_wait(&sh->odone[tile], outs++ & 1, abort);
             if (!__all_sync(0xFFFFFFFFu, ok)) {
                 failed = true;
                 break;
@@ -667,9 +684,14 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 }
             }
             __syncwarp();                                         // a bad row's values above come before attn_row's
-            for (unsigned left = __ballot_sync(0xFFFFFFFFu, bad); left; left &= left - 1) {
-                const int src = __ffs(left) - 1;
-                attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), b.head, own.lo, __shfl_sync(0xFFFFFFFFu, hi, src));
+            unsigned left = __ballot_sync(0xFFFFFFFFu, bad);
+            if (left) {
+                if (lane == 0) atomicAdd(&sh->abort[1], 1);
+                for (; left; left &= left - 1) {
+                    const int src = __ffs(left) - 1;
+                    attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), b.head, own.lo, __shfl_sync(0xFFFFFFFFu, hi, src));
+                }
+                if (lane == 0) atomicAdd(&sh->abort[1], -1);
             }
         }
     }
