@@ -49,6 +49,7 @@ struct AttnTile {
 __device__ __forceinline__ AttnTile attn_tile(const AttnParams& p, int64_t slot, int lane) {
     int b = 0, n = p.B;                              // the sequence is among b .. b + n - 1
     bool any = true;
+#pragma unroll 1
     while (n > 1 && any) {
         const int step = (n + 31) >> 5;
         const int i = b + min(lane * step, n - 1);
@@ -72,6 +73,7 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnParams& p, int64_t slot,
 
 // Every entry of the table is looked at by one thread of the grid: bisection alone does not see them all.
 __device__ __forceinline__ void attn_check_table(const AttnParams& p, int lane) {
+#pragma unroll 1
     for (int64_t i = (int64_t)blockIdx.x * 32 + lane; i < p.B; i += (int64_t)gridDim.x * 32) {
         const int begin = __ldg(p.cu + i), end = __ldg(p.cu + i + 1);
         if (begin < 0 || end < begin || end > p.T) atomicExch(p.err, 6);
@@ -221,9 +223,9 @@ struct AttnBlocks {
     }
 };
 
-// A walk of a thread or a whole warp over the blocks of its CTA's items.  The last of a role's walks
-// gives the items' records back behind itself (by the lane with `lead` set).
-template <int DP, bool kRelease>
+// A walk of a thread or a whole warp over the blocks of its CTA's items; gives the items' records back
+// behind itself (by the lane with `lead` set).
+template <int DP>
 struct AttnWalk {
     AttnBlocks<DP> b;
     int rec = -1, j = 0;
@@ -234,7 +236,7 @@ struct AttnWalk {
             ++j;
             return 1;
         }
-        if (kRelease && rec >= 0 && lead) tc::mbar_arrive(&sh->iempty[rec % kAItems]);
+        if (rec >= 0 && lead) tc::mbar_arrive(&sh->iempty[rec % kAItems]);
         ++rec;
         if (!attn_wait(&sh->ifull[rec % kAItems], (rec / kAItems) & 1, sh->abort)) return -1;
         b.get(sh, rec % kAItems);
@@ -324,71 +326,69 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsFew));
         if (warp == 0 && lane == 0) {
             // -------------------------------------------------------- TMA producer
-            // K blocks run one ahead of V blocks, over all items' blocks, as the products want them
             const int per = p.heads / p.kv_heads;
-            AttnWalk<DP, false> kw;
-            AttnWalk<DP, true> vw;
-            int nk = 0, nv = 0, nq = 0, k = 1;
-            auto load = [&](const AttnBlocks<DP>& b, int j, int i, const CUtensorMap* map, uint8_t* ring, uint64_t* full,
-                            uint64_t* empty) {
-                const int s = i % S;
-                if (i >= S && !attn_wait(empty + s, (i / S - 1) & 1, abort)) return false;
-                tc::mbar_arrive_expect_tx(full + s, Cfg::kTileK);
-                for (int c = 0; c < DP / 64; ++c)
-                    tc::tma_load_3d(ring + s * Cfg::kTileK + c * N * 128, map, 64 * c, b.head / per, b.kv0 + j * N,
-                                    full + s);
+            AttnWalk<DP> walk;
+            int n = 0, nq = 0;                                    // blocks and items
+            auto slot = [&](uint64_t* full, uint64_t* empty) {
+                if (n >= S && !attn_wait(empty + n % S, (n / S - 1) & 1, abort)) return false;
+                tc::mbar_arrive_expect_tx(full + n % S, Cfg::kTileK);
                 return true;
             };
-            for (int pos = 0; !failed; ++pos) {
-                if (pos > 0) {
-                    const int v = vw.next(sh);
-                    if (v == 0) break;
-                    failed = v < 0 || !load(vw.b, vw.j, nv, &maps.v, sV, sh->vfull, sh->vempty);
-                    if (failed) break;
-                    ++nv;
+            auto load = [&](const CUtensorMap* map, uint8_t* ring, uint64_t* full) {
+                for (int c = 0; c < DP / 64; ++c)
+                    tc::tma_load_3d(ring + (n % S) * Cfg::kTileK + c * N * 128, map, 64 * c, walk.b.head / per,
+                                    walk.b.kv0 + walk.j * N, full + n % S);
+            };
+            for (;; ++n) {
+                const int there = walk.next(sh);
+                if (there <= 0) {
+                    failed = there < 0;
+                    break;
                 }
-                if (k > 0) k = kw.next(sh);
-                if (k < 0) failed = true;
-                if (k <= 0) continue;
-                if (!load(kw.b, kw.j, nk, &maps.k, sK, sh->kfull, sh->kempty)) {
+                if (!slot(sh->kfull, sh->kempty)) {
                     failed = true;
                     break;
                 }
-                ++nk;
-                if (kw.j == 0) {                                  // a new item: its Q
+                load(&maps.k, sK, sh->kfull);
+                if (walk.j == 0) {                                // a new item: its Q
                     if (nq > 0 && !attn_wait(&sh->qempty, (nq - 1) & 1, abort)) {
                         failed = true;
                         break;
                     }
                     // rows of a tile behind its sequence are another's: read along and not used
-                    const int r = kw.rec % kAItems;
                     tc::mbar_arrive_expect_tx(&sh->qfull, kTiles * Cfg::kTileQ);
                     for (int t = 0; t < kTiles; ++t)
                         for (int c = 0; c < DP / 64; ++c)
-                            tc::tma_load_3d(sQ + t * Cfg::kTileQ + c * kAM * 128, &maps.q, 64 * c, kw.b.head,
-                                            sh->tile[r][t].row0, &sh->qfull);
+                            tc::tma_load_3d(sQ + t * Cfg::kTileQ + c * kAM * 128, &maps.q, 64 * c, walk.b.head,
+                                            sh->tile[walk.rec % kAItems][t].row0, &sh->qfull);
                     ++nq;
                 }
+                if (!slot(sh->vfull, sh->vempty)) {
+                    failed = true;
+                    break;
+                }
+                load(&maps.v, sV, sh->vfull);
             }
             if (failed) {                                         // copies in flight end before the CTA does
                 if (nq > 0) (void)tc::mbar_wait_bounded(&sh->qfull, (nq - 1) & 1, 1u << 16);
-                for (int i = max(0, nk - S); i < nk; ++i)
+#pragma unroll 1
+                for (int i = max(0, n - S); i <= n; ++i) {
                     (void)tc::mbar_wait_bounded(&sh->kfull[i % S], (i / S) & 1, 1u << 16);
-                for (int i = max(0, nv - S); i < nv; ++i)
                     (void)tc::mbar_wait_bounded(&sh->vfull[i % S], (i / S) & 1, 1u << 16);
+                }
             }
         } else if (warp == 1) {
             // -------------------------------------------------------- MMA issuer, one lane of a warp in step
             constexpr uint32_t idS = tc::idesc_f16_f32(kAM, N) | idesc_type<T>();
             constexpr uint32_t idO = tc::idesc_f16_f32(kAM, DP) | idesc_type<T>() | kIdescBMn;
             const uint32_t lead = tc::elect_one();
-            AttnWalk<DP, false> sw;                               // scores run one block ahead of
-            AttnWalk<DP, true> vw;                                // the products with V
-            vw.lead = lead != 0;
+            AttnWalk<DP> walk;                                    // of the scores; the products with V are
+            int vj = 0, vjb[kTiles], vje[kTiles];                 // one block behind it, at vj
+            walk.lead = lead != 0;
             uint32_t np[kTiles] = {};                             // products of each tile
-            int nk = 0, nv = 0, nq = 0, more = 1;
+            int nk = 0, nv = 0, nq = 0;
             auto scores = [&](int t) {
-                if (sw.j < sw.b.jb[t] || sw.j >= sw.b.je[t]) return;
+                if (walk.j < walk.b.jb[t] || walk.j >= walk.b.je[t]) return;
                 // S takes the columns of the weights that the product just issued reads: the tensor pipe
                 // runs them one behind the other
                 const uint32_t q = tc::smem_u32(sQ + t * Cfg::kTileQ), k = tc::smem_u32(sK + (nk % S) * Cfg::kTileK);
@@ -399,9 +399,9 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 tc::mma_commit_if(lead, &sh->sfull[t]);
             };
             auto product = [&](int t) {
-                if (vw.j < vw.b.jb[t] || vw.j >= vw.b.je[t]) return true;
+                if (vj < vjb[t] || vj >= vje[t]) return true;
                 const uint32_t v = tc::smem_u32(sV + (nv % S) * Cfg::kTileK);
-                const bool begun = vw.j > vw.b.jb[t];
+                const bool begun = vj > vjb[t];
 #pragma unroll
                 for (int x = 0; x < Cfg::kHalves; ++x) {
                     const bool ok = attn_wait(&sh->pready[t][x], np[t] & 1, abort);
@@ -413,52 +413,56 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                                       tc::sw128_mnmajor_desc(v + 2048 * c, N * 128), idO, begun || c > 0);
                 }
                 ++np[t];
-                if (vw.j == vw.b.je[t] - 1) tc::mma_commit_if(lead, &sh->odone[t]);
+                if (vj == vje[t] - 1) tc::mma_commit_if(lead, &sh->odone[t]);
                 return true;
             };
             auto k_arrived = [&] {
                 const bool ok = attn_wait(&sh->kfull[nk % S], (nk / S) & 1, abort) &&
-                                (sw.j != 0 || attn_wait(&sh->qfull, nq & 1, abort));
+                                (walk.j != 0 || attn_wait(&sh->qfull, nq & 1, abort));
                 if (!__all_sync(0xFFFFFFFFu, ok)) return false;
                 tc::fence_after();
                 return true;
             };
-            for (int pos = 0;; ++pos) {
-                const int there = pos == 0 ? 0 : vw.next(sh);
-                if (more > 0) more = sw.next(sh);
-                failed = !__all_sync(0xFFFFFFFFu, there >= 0 && more >= 0);
-                if (failed || there + more == 0) break;
-                // Where the scores want a new Q, which may still be on its way, they come behind all
-                // products; else each tile's follow its product, which also keeps two tiles in turns:
-                // one's products run while the other's weights are computed.
-                const bool apart = more > 0 && (kTiles == 1 || sw.j == 0);
-                if (there > 0) {
+            // Within an item two tiles take turns, each one's scores behind its product: its products run
+            // while the other's weights are computed.  At an item's end, and with one tile, all products
+            // come first: the next item's record, K and Q may still be on their way.
+            bool first = true;
+            for (;;) {
+                const bool follow = kTiles > 1 && !first && walk.j + 1 < walk.b.n;
+                if (!first) {
+                    vj = walk.j;
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        vjb[t] = walk.b.jb[t];
+                        vje[t] = walk.b.je[t];
+                    }
+                    if (follow) ++walk.j;
                     const bool ok = attn_wait(&sh->vfull[nv % S], (nv / S) & 1, abort);
-                    failed = !__all_sync(0xFFFFFFFFu, ok) || (kTiles > 1 && more > 0 && !apart && !k_arrived());
+                    failed = !__all_sync(0xFFFFFFFFu, ok) || (follow && !k_arrived());
                     if (failed) break;
                     tc::fence_after();
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
                         failed = failed || !product(t);
-                        if (kTiles > 1 && !failed && more > 0 && !apart) scores(t);
+                        if (kTiles > 1 && !failed && follow) scores(t);
                     }
                     if (failed) break;
                     tc::mma_commit_if(lead, &sh->vempty[nv % S]);
                     ++nv;
                 }
-                if (more > 0) {
-                    if (apart) {
-                        failed = !k_arrived();
-                        if (failed) break;
+                first = false;
+                if (!follow) {
+                    const int more = walk.next(sh);
+                    failed = !__all_sync(0xFFFFFFFFu, more >= 0) || (more > 0 && !k_arrived());
+                    if (failed || more == 0) break;
 #pragma unroll
-                        for (int t = 0; t < kTiles; ++t) scores(t);
-                    }
-                    tc::mma_commit_if(lead, &sh->kempty[nk % S]);
-                    ++nk;
-                    if (sw.j == sw.b.n - 1) {
-                        tc::mma_commit_if(lead, &sh->qempty);
-                        ++nq;
-                    }
+                    for (int t = 0; t < kTiles; ++t) scores(t);
+                }
+                tc::mma_commit_if(lead, &sh->kempty[nk % S]);
+                ++nk;
+                if (walk.j == walk.b.n - 1) {
+                    tc::mma_commit_if(lead, &sh->qempty);
+                    ++nq;
                 }
             }
             if (failed) {                                         // the last products read shared memory
