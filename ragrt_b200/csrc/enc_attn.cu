@@ -190,7 +190,7 @@ template <int DP>
 struct AttnShared {
     static constexpr int kTiles = AttnCfg<DP>::kTiles, kStages = AttnCfg<DP>::kStages;
     AttnTile tile[kAItems][kTiles];
-    int head[kAItems];                       // < 0: no more items
+    int head[kAItems], group[kAItems];       // query and key head; head < 0: no more items
     uint64_t kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
     uint64_t qfull, qempty;
     uint64_t ifull[kAItems], iempty[kAItems];
@@ -205,9 +205,10 @@ struct AttnShared {
 // The blocks of an item: blocks 0 .. n - 1 from key kv0 on, tile t takes [jb[t], je[t]) of them.
 template <int DP>
 struct AttnBlocks {
-    int head = -1, kv0, n = 0, jb[AttnCfg<DP>::kTiles], je[AttnCfg<DP>::kTiles];
+    int head = -1, group, kv0, n = 0, jb[AttnCfg<DP>::kTiles], je[AttnCfg<DP>::kTiles];
     __device__ __forceinline__ void get(const AttnShared<DP>* sh, int r) {
         head = sh->head[r];
+        group = sh->group[r];
         kv0 = 0x7FFFFFFF;
         n = 0;
 #pragma unroll
@@ -326,7 +327,6 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsFew));
         if (warp == 0 && lane == 0) {
             // -------------------------------------------------------- TMA producer
-            const int per = p.heads / p.kv_heads;
             AttnWalk<DP> walk;
             int n = 0, nq = 0;                                    // blocks and items
             auto slot = [&](uint64_t* full, uint64_t* empty) {
@@ -336,7 +336,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             };
             auto load = [&](const CUtensorMap* map, uint8_t* ring, uint64_t* full) {
                 for (int c = 0; c < DP / 64; ++c)
-                    tc::tma_load_3d(ring + (n % S) * Cfg::kTileK + c * N * 128, map, 64 * c, walk.b.head / per,
+                    tc::tma_load_3d(ring + (n % S) * Cfg::kTileK + c * N * 128, map, 64 * c, walk.b.group,
                                     walk.b.kv0 + walk.j * N, full + n % S);
             };
             for (;; ++n) {
@@ -474,16 +474,16 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             // Heads fastest, and the last rows first: the tiles of a causal sequence grow along it.  The
             // CTAs take a round of items in one order and the next in the other, so that none always
             // gets a round's longest.  Items without a row are passed over.
-            const int groups = p.items / p.heads;
-            int rec = 0, group = -1;
+            const uint32_t heads = p.heads, per = heads / p.kv_heads, groups = p.items / heads, cta = blockIdx.x;
+            uint32_t rec = 0, group = 0xFFFFFFFFu;
             AttnTile tile[kTiles];
             bool any = false;
-            for (int round = 0; !failed; ++round) {
-                const int64_t i = (int64_t)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                const bool end = (int64_t)round * gridDim.x >= p.items;
+            for (uint32_t round = 0; !failed; ++round) {
+                const uint32_t base = round * gridDim.x, i = base + (round & 1 ? gridDim.x - 1 - cta : cta);
+                const bool end = base >= (uint32_t)p.items;
                 if (!end) {
-                    if (i >= p.items) continue;
-                    const int g = groups - 1 - (int)(i / p.heads);
+                    if (i >= (uint32_t)p.items) continue;
+                    const uint32_t g = groups - 1 - i / heads;
                     if (g != group) {
                         group = g;
                         any = false;
@@ -495,8 +495,8 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                     }
                     if (!any) continue;
                 }
-                const int r = rec % kAItems;
-                const bool ok = rec < kAItems ||
+                const uint32_t r = rec % kAItems;
+                const bool ok = rec < (uint32_t)kAItems ||
                                 attn_wait(&sh->iempty[r], (rec / kAItems - 1) & 1, abort);
                 if (!__all_sync(0xFFFFFFFFu, ok)) {
                     failed = true;
@@ -505,7 +505,8 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 if (lane == 0) {
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) sh->tile[r][t] = end ? AttnTile{0, 0, 0, 0} : tile[t];
-                    sh->head[r] = end ? -1 : (int)(i % p.heads);
+                    sh->head[r] = end ? -1 : (int)(i % heads);
+                    sh->group[r] = (int)(i % heads / per);
                     tc::mbar_arrive(&sh->ifull[r]);
                 }
                 ++rec;
