@@ -71,15 +71,6 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnParams& p, int64_t slot,
     return t;
 }
 
-// Every entry of the table is looked at by one thread of the grid: bisection alone does not see them all.
-__device__ __forceinline__ void attn_check_table(const AttnParams& p, int lane) {
-#pragma unroll 1
-    for (int64_t i = (int64_t)blockIdx.x * 32 + lane; i < p.B; i += (int64_t)gridDim.x * 32) {
-        const int begin = __ldg(p.cu + i), end = __ldg(p.cu + i + 1);
-        if (begin < 0 || end < begin || end > p.T) atomicExch(p.err, 6);
-    }
-}
-
 // bits below n of a word, n of any size
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 
@@ -136,7 +127,7 @@ __device__ __noinline__ void attn_row(const AttnParams& p, int t, int h, int lo,
 }
 
 constexpr int kAFirst = 4;                     // first softmax warp: TMA, MMA and search warp before them, one idle
-constexpr int kAItems = 4;                     // items whose tiles are in shared memory
+constexpr int kAItems = 2;                     // items whose tiles are in shared memory
 // The reference maximum of a row moves only when it is exceeded by a factor of 2^8: until then the weights are
 // at most 256, well inside either type, and the accumulator is not rescaled.
 constexpr float kARescale = 8.0f;
@@ -190,6 +181,7 @@ template <int DP>
 struct AttnShared {
     static constexpr int kTiles = AttnCfg<DP>::kTiles, kStages = AttnCfg<DP>::kStages;
     AttnTile tile[kAItems][kTiles];
+    uint4 answer;                            // to a request for the next item
     int head[kAItems], group[kAItems];       // query and key head; head < 0: no more items
     uint64_t kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
     uint64_t qfull, qempty;
@@ -197,7 +189,7 @@ struct AttnShared {
     uint64_t sfull[kTiles];                  // scores ready (MMA -> softmax)
     uint64_t pready[kTiles][AttnCfg<DP>::kHalves];       // weights written (softmax -> MMA)
     uint64_t odone[kTiles];                  // product with V done
-    uint64_t drain;
+    uint64_t drain, taken;
     uint32_t tmem;
     int abort[2];                            // given up; warps in attn_row
 };
@@ -309,6 +301,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             tc::mbar_init(&sh->odone[t], 1);
         }
         tc::mbar_init(&sh->drain, 1);
+        tc::mbar_init(&sh->taken, 1);
         sh->abort[0] = sh->abort[1] = 0;
         tc::mbar_fence_init();
     }
@@ -471,19 +464,30 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             }
         } else if (warp == 2) {
             // -------------------------------------------------------- the coming items
-            // Heads fastest, and the last rows first: the tiles of a causal sequence grow along it.  The
-            // CTAs take a round of items in one order and the next in the other, so that none always
-            // gets a round's longest.  Items without a row are passed over.
-            const uint32_t heads = p.heads, per = heads / p.kv_heads, groups = p.items / heads, cta = blockIdx.x;
-            uint32_t rec = 0, group = 0xFFFFFFFFu;
+            // The grid has a CTA for each item: heads fastest, and the last rows first, since the tiles of a
+            // causal sequence grow along it.  The CTAs that are running take over those that are not, one
+            // at a time, so that none is left with more than its share of long ones.  Items without a row
+            // are passed over.
+            const uint32_t heads = p.heads, per = heads / p.kv_heads, groups = p.items / heads;
+            uint32_t rec = 0, asked = 0, group = 0xFFFFFFFFu;
             AttnTile tile[kTiles];
             bool any = false;
-            for (uint32_t round = 0; !failed; ++round) {
-                const uint32_t base = round * gridDim.x, i = base + (round & 1 ? gridDim.x - 1 - cta : cta);
-                const bool end = base >= (uint32_t)p.items;
+            int64_t item = blockIdx.x;
+            for (;;) {
+                const bool end = item < 0;
                 if (!end) {
-                    if (i >= (uint32_t)p.items) continue;
-                    const uint32_t g = groups - 1 - i / heads;
+                    if (lane == 0) {
+                        tc::fence_proxy_async();                  // behind the reading of the answer before
+                        tc::take_ask(&sh->answer, &sh->taken);
+                    }
+                    // an entry of the table for each lane and item: that is all of them, which bisection
+                    // alone does not see
+                    const int64_t e = item * 32 + lane;
+                    if (e < p.B) {
+                        const int begin = __ldg(p.cu + e), stop = __ldg(p.cu + e + 1);
+                        if (begin < 0 || stop < begin || stop > p.T) atomicExch(p.err, 6);
+                    }
+                    const uint32_t g = groups - 1 - (uint32_t)item / heads;
                     if (g != group) {
                         group = g;
                         any = false;
@@ -493,26 +497,29 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                             any = any || tile[t].rows > 0;
                         }
                     }
-                    if (!any) continue;
                 }
-                const uint32_t r = rec % kAItems;
-                const bool ok = rec < (uint32_t)kAItems ||
-                                attn_wait(&sh->iempty[r], (rec / kAItems - 1) & 1, abort);
-                if (!__all_sync(0xFFFFFFFFu, ok)) {
-                    failed = true;
-                    break;
-                }
-                if (lane == 0) {
+                if (end || any) {
+                    const uint32_t r = rec % kAItems;
+                    const bool ok = rec < (uint32_t)kAItems || attn_wait(&sh->iempty[r], (rec / kAItems - 1) & 1, abort);
+                    failed = !__all_sync(0xFFFFFFFFu, ok);
+                    if (lane == 0 && !failed) {
 #pragma unroll
-                    for (int t = 0; t < kTiles; ++t) sh->tile[r][t] = end ? AttnTile{0, 0, 0, 0} : tile[t];
-                    sh->head[r] = end ? -1 : (int)(i % heads);
-                    sh->group[r] = (int)(i % heads / per);
-                    tc::mbar_arrive(&sh->ifull[r]);
+                        for (int t = 0; t < kTiles; ++t) sh->tile[r][t] = end ? AttnTile{0, 0, 0, 0} : tile[t];
+                        sh->head[r] = end ? -1 : (int)((uint32_t)item % heads);
+                        sh->group[r] = end ? 0 : (int)((uint32_t)item % heads / per);
+                        tc::mbar_arrive(&sh->ifull[r]);
+                    }
+                    ++rec;
                 }
-                ++rec;
                 if (end) break;
+                // also behind a failure: the answer must have come before the CTA goes
+                const bool ok = attn_wait(&sh->taken, asked++ & 1, abort) ||
+                                tc::mbar_wait_bounded(&sh->taken, (asked - 1) & 1, 1u << 20);
+                failed = failed || !__all_sync(0xFFFFFFFFu, ok);
+                if (failed) break;
+                item = tc::take_answer(&sh->answer);
+                __syncwarp();
             }
-            attn_check_table(p, lane);
         }
     } else {
         // ------------------------------------------------------------ softmax, a thread per row
@@ -722,8 +729,8 @@ int attn_launch(int dtype, AttnParams p, cudaStream_t stream) {
     const int64_t groups = ceil_div(p.T / kAM + (int64_t)p.B, AttnCfg<DP>::kTiles);
     if (groups * p.heads > 0x7FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many rows x heads");
     p.items = (int)(groups * p.heads);
-    return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)std::min(p.items, num_sms() * AttnCfg<DP>::kCtas)),
-                      dim3(AttnCfg<DP>::kThreads), AttnCfg<DP>::kSmem, stream, m, p);
+    return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)p.items), dim3(AttnCfg<DP>::kThreads), AttnCfg<DP>::kSmem,
+                      stream, m, p);
 }
 
 }  // namespace

@@ -390,3 +390,33 @@ __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_g
 
 }  // namespace tc
 }  // namespace ragrt
+
+// ------------------------------------------------------------------ work from the launch queue
+// A running CTA takes over a CTA of its own launch that has not begun (cluster launch control): one
+// thread asks, the 16-byte answer comes to shared memory and is counted on `bar`, and after an answer
+// without a CTA no more is asked for.
+namespace ragrt {
+namespace tc {
+
+__device__ __forceinline__ void take_ask(void* answer, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(answer)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// x index of the CTA taken over, or -1
+__device__ __forceinline__ int64_t take_answer(const void* answer) {
+    uint32_t got, x;
+    asm volatile(
+        "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\tld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}\n"
+        : "=r"(got), "=r"(x)
+        : "r"(smem_u32(answer))
+        : "memory");
+    return got ? (int64_t)x : -1;
+}
+
+}  // namespace tc
+}  // namespace ragrt
