@@ -26,6 +26,8 @@ feed-forward blocks (fp16 or bf16, no counterpart in the reference):
 The token ids, [Q] marker and [MASK] padding come from the checkpoint's own tokenizer, as in
 the reference; `encode_ids` takes already-tokenized input.
 """
+import ctypes
+
 import torch
 
 from . import _lib
@@ -146,6 +148,28 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 
+_bound = None
+
+
+def _bind():
+    """The host binding (csrc/enc_bind.cpp), given the entry points of the loaded library.  It serves the
+    calls whose operands can be used as they lie and answers None to the others, which the Python below
+    then copies or refuses."""
+    global _bound
+    if _bound is None:
+        L = _lib.lib()
+        try:
+            from . import _enc_bind
+        except ImportError as e:
+            raise RuntimeError("ragrt_b200/_enc_bind.so is missing or does not load: build it first "
+                               "(python -m ragrt_b200.build)") from e
+        _enc_bind.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            L.ragrt_enc_packed_attention, L.ragrt_enc_qk_norm_rope, L.ragrt_enc_gated_ffn,
+            L.ragrt_enc_gated_ffn_backward)))
+        _bound = _enc_bind
+    return _bound
+
+
 def _dtype16(*ts):
     """Type code of a call's 16-bit tensors (None for an absent one), which must agree."""
     want = ts[0].dtype
@@ -229,6 +253,10 @@ def packed_attention(q, k, v, cu_seqlens, causal=False, scale=None, out=None):
     its sequence up to itself.  scale defaults to D ** -0.5.  Rows outside every sequence are not
     written (undefined in a new `out`).  D a multiple of 8 up to 128.  A bad table raises the
     device error flag (6) and leaves rows unwritten.  Not differentiable."""
+    if out is None:
+        r = (_bound or _bind()).packed_attention(q, k, v, cu_seqlens, causal, scale)
+        if r is not None:
+            return _lib.check(r) if type(r) is int else r
     _need_cuda(q, k, v, cu_seqlens, out)
     dt = _dtype16(q, k, v)
     shape, kshape = q.shape, k.shape
@@ -261,6 +289,10 @@ def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     pairs (i, i + R / 2), or neighbours with `interleaved`.  q [T, H, D], k [T, KV, D] fp16 or bf16 ->
     (q_out, k_out), which may be q and k themselves.  D a multiple of 8 in [16, 256], R a multiple
     of 16.  A position outside the table reads its row 0 and raises the device error flag (5)."""
+    if q_out is None and k_out is None:
+        r = (_bound or _bind()).qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+        if r is not None:
+            return _lib.check(r) if type(r) is int else r
     _need_cuda(q, k, cos, sin, positions, q_weight, k_weight, q_out, k_out)
     dt = _dtype16(q, k, q_weight, k_weight)
     shape, kshape = q.shape, k.shape
@@ -311,6 +343,10 @@ def gated_ffn(x, w_gate, w_up, act="silu", keep=False, out=None):
     a stacked [2 F, K] matrix are read in place), fp16 or bf16, F and K multiples of 8; act "silu",
     "gelu" (erf form) or "gelu_tanh".  keep=True returns (h, gate, up) with the two products that
     gated_ffn_backward wants.  Not tracked by autograd."""
+    if out is None and act in _ACTS:
+        r = (_bound or _bind()).gated_ffn(x, w_gate, w_up, _ACTS[act], keep)
+        if r is not None:
+            return _lib.check(r) if type(r) is int else r
     _need_cuda(x, w_gate, w_up, out)
     dt = _dtype16(x, w_gate, w_up)
     M, F, K = _ffn_args(x, w_gate, w_up, act)
@@ -333,6 +369,10 @@ def gated_ffn(x, w_gate, w_up, act="silu", keep=False, out=None):
 def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu", need_dx=True, need_dw=True):
     """Gradients of gated_ffn from dh [M, F] and the kept gate and up: (dx [M, K], dw_gate [F, K],
     dw_up [F, K]) in the inputs' type, None for what is not needed.  Sums run in a fixed order."""
+    if act in _ACTS:
+        r = (_bound or _bind()).gated_ffn_backward(dh, x, w_gate, w_up, gate, up, _ACTS[act], need_dx, need_dw)
+        if r is not None:
+            return _lib.check(r) if type(r) is int else r
     _need_cuda(dh, x, w_gate, w_up, gate, up)
     dt = _dtype16(dh, x, w_gate, w_up, gate, up)
     M, F, K = _ffn_args(x, w_gate, w_up, act)
