@@ -33,6 +33,8 @@ struct RopeParams {
 };
 
 
+constexpr int kRopeWarps = 2;                    // small CTAs: a place is free again as soon as two tokens are done
+
 // 8 values of 16 bits <-> 4 fp32 pairs
 template <typename T>
 __device__ __forceinline__ void up8x2(const uint4& u, uint64_t (&f)[4]) {
@@ -58,7 +60,7 @@ __device__ __forceinline__ uint4 down8x2(const uint64_t (&f)[4]) {
 // A warp takes one token and one of `slabs` shares of its heads, kBatch of a lane's heads in flight at a
 // time.
 template <typename T, bool kNeighbours, int kBatch>
-__global__ void __launch_bounds__(256, 3) enc_qk_norm_rope(const RopeParams p, const int group) {
+__global__ void __launch_bounds__(32 * kRopeWarps, 24 / kRopeWarps) enc_qk_norm_rope(const RopeParams p, const int group) {
     pdl_wait_then_release();
     const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     if (unit >= (int64_t)p.T * p.slabs) return;
@@ -95,8 +97,8 @@ __global__ void __launch_bounds__(256, 3) enc_qk_norm_rope(const RopeParams p, c
             const int h = (r + i) * per + sub;
             const bool on = r + i < r1 && h < all;
             const T* src = (h < p.heads ? q : k) + h * p.dim;
-            ua[i] = on && has_a ? *reinterpret_cast<const uint4*>(src + a) : zero;
-            ub[i] = on && has_b ? *reinterpret_cast<const uint4*>(src + b) : zero;
+            ua[i] = on && has_a ? __ldcs(reinterpret_cast<const uint4*>(src + a)) : zero;
+            ub[i] = on && has_b ? __ldcs(reinterpret_cast<const uint4*>(src + b)) : zero;
         }
         if (r == r0) {                                      // the angles, behind the first heads' loads
             if (pos < 0 || pos >= p.max_pos) {
@@ -157,8 +159,8 @@ __global__ void __launch_bounds__(256, 3) enc_qk_norm_rope(const RopeParams p, c
             }
             if (on) {
                 T* dst = (is_q ? qo : ko) + h * p.dim;
-                if (has_a) *reinterpret_cast<uint4*>(dst + a) = down8x2<T>(x);
-                if (has_b) *reinterpret_cast<uint4*>(dst + b) = down8x2<T>(y);
+                if (has_a) __stcs(reinterpret_cast<uint4*>(dst + a), down8x2<T>(x));
+                if (has_b) __stcs(reinterpret_cast<uint4*>(dst + b), down8x2<T>(y));
             }
         }
     }
@@ -166,9 +168,9 @@ __global__ void __launch_bounds__(256, 3) enc_qk_norm_rope(const RopeParams p, c
 
 template <typename T, bool kNeighbours>
 int rope_launch(const RopeParams& p, int group, int batch, cudaStream_t stream) {
-    const int64_t blocks = ceil_div((int64_t)p.T * p.slabs, 8);
-    return batch == 3 ? enc_launch(enc_qk_norm_rope<T, kNeighbours, 3>, dim3((unsigned)blocks), dim3(256), 0, stream, p, group)
-                      : enc_launch(enc_qk_norm_rope<T, kNeighbours, 2>, dim3((unsigned)blocks), dim3(256), 0, stream, p, group);
+    const int64_t blocks = ceil_div((int64_t)p.T * p.slabs, kRopeWarps);
+    return batch == 3 ? enc_launch(enc_qk_norm_rope<T, kNeighbours, 3>, dim3((unsigned)blocks), dim3(32 * kRopeWarps), 0, stream, p, group)
+                      : enc_launch(enc_qk_norm_rope<T, kNeighbours, 2>, dim3((unsigned)blocks), dim3(32 * kRopeWarps), 0, stream, p, group);
 }
 
 }  // namespace
@@ -215,7 +217,7 @@ extern "C" int ragrt_enc_qk_norm_rope(const void* d_q, const void* d_k, const vo
     // token, which loads its angles once.
     const int warps = num_sms() * 16;
     const int slabs = (int)std::min<int64_t>(ceil_div(rounds, batch), std::max<int64_t>(1, warps / T));
-    RAGRT_REQUIRE(ceil_div((int64_t)T * slabs, 8) <= 0x7FFFFFFF, "too many tokens");
+    RAGRT_REQUIRE(ceil_div((int64_t)T * slabs, kRopeWarps) <= 0x7FFFFFFF, "too many tokens");
     RopeParams p{d_q, d_k, d_q_weight, d_k_weight, d_cos, d_sin, d_pos, d_q_out, d_k_out, q_stride, k_stride,
                  q_out_stride, k_out_stride, T, heads, kv_heads, head_dim, rot_dim, max_pos, pos_bytes == 8,
                  interleaved != 0, slabs, eps, err};
