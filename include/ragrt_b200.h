@@ -406,20 +406,20 @@ int ragrt_enc_qk_norm_rope(const void* d_q, const void* d_k, const void* d_q_wei
 /*
  * d_h [M, F] = act(d_x . d_w_gate^T) * (d_x . d_w_up^T), d_x [M, K], weights [F, K] (the halves of a
  * stacked [2 F, K] matrix will do): both projections, the activation and the product in one
- * kernel.  act 0: silu, 1: gelu (erf form), 2: gelu (tanh form).  d_gate / d_up [M, F] (or both NULL)
- * keep the two products for ragrt_enc_gated_ffn_backward.  F and K multiples of 8.
+ * kernel.  act 0: silu, 1: gelu (erf form), 2: gelu (tanh form).  d_gate / d_up f32 [M, F] (or both
+ * NULL) keep the two products for ragrt_enc_gated_ffn_backward.  F and K multiples of 8.
  */
-int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const void* d_w_up, void* d_h, void* d_gate,
-                        void* d_up, int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype, void* stream);
+int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const void* d_w_up, void* d_h, float* d_gate,
+                        float* d_up, int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype, void* stream);
 
 /*
  * Gradients of ragrt_enc_gated_ffn from d_dh [M, F] and the kept d_gate / d_up: d_dgate, d_dup [M, F]
- * (the gradients of the two products; always written, they may be d_gate and d_up themselves),
+ * (16 bits, the gradients of the two products; always written),
  * d_dx [M, K] (may be NULL), d_dw_gate and d_dw_up [F, K] (may both be NULL).  Overwrites, does
  * not add to, its outputs; the order of every sum is fixed.  M = 0 gives zero weight gradients.
  */
 int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* d_w_gate, const void* d_w_up,
-                                 const void* d_gate, const void* d_up, void* d_dgate, void* d_dup, void* d_dx,
+                                 const float* d_gate, const float* d_up, void* d_dgate, void* d_dup, void* d_dx,
                                  void* d_dw_gate, void* d_dw_up, int32_t M, int32_t F, int32_t K, int32_t act,
                                  int32_t dtype, void* stream);
 

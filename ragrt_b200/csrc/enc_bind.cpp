@@ -164,11 +164,11 @@ PyObject* gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t M = x->size(0), F = g->size(0), K = x->size(1);
         at::Tensor h = like(*x, {M, F}), gate, up;
         if (keep) {
-            gate = like(*x, {M, F});
-            up = like(*x, {M, F});
+            gate = at::empty({M, F}, h.options().dtype(at::kFloat));
+            up = at::empty({M, F}, h.options().dtype(at::kFloat));
         }
-        const int rc = f_ffn(x->data_ptr(), g->data_ptr(), u->data_ptr(), h.data_ptr(), keep ? gate.data_ptr() : nullptr,
-                             keep ? up.data_ptr() : nullptr, (int32_t)M, (int32_t)F, (int32_t)K, (int32_t)act, dt,
+        const int rc = f_ffn(x->data_ptr(), g->data_ptr(), u->data_ptr(), h.data_ptr(), keep ? (float*)gate.data_ptr() : nullptr,
+                             keep ? (float*)up.data_ptr() : nullptr, (int32_t)M, (int32_t)F, (int32_t)K, (int32_t)act, dt,
                              stream(dev));
         if (rc) return PyLong_FromLong(rc);
         if (!keep) return THPVariable_Wrap(std::move(h));
@@ -192,7 +192,7 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (dt < 0) Py_RETURN_NONE;
         const int64_t M = x->size(0), F = g->size(0), K = x->size(1);
         for (const at::Tensor* t : {dh, gate, up})
-            if (t->scalar_type() != x->scalar_type() || t->dim() != 2 || t->size(0) != M || t->size(1) != F || !solid(*t))
+            if (t->scalar_type() != (t == dh ? x->scalar_type() : at::kFloat) || t->dim() != 2 || t->size(0) != M || t->size(1) != F || !solid(*t))
                 Py_RETURN_NONE;
         at::Tensor dg = like(*x, {M, F}), du = like(*x, {M, F}), rx, rg, ru;
         if (dx) rx = like(*x, {M, K});
@@ -200,8 +200,8 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
             rg = like(*x, {F, K});
             ru = like(*x, {F, K});
         }
-        const int rc = f_ffn_backward(dh->data_ptr(), x->data_ptr(), g->data_ptr(), u->data_ptr(), gate->data_ptr(),
-                                      up->data_ptr(), dg.data_ptr(), du.data_ptr(), dx ? rx.data_ptr() : nullptr,
+        const int rc = f_ffn_backward(dh->data_ptr(), x->data_ptr(), g->data_ptr(), u->data_ptr(),
+                                      (const float*)gate->data_ptr(), (const float*)up->data_ptr(), dg.data_ptr(), du.data_ptr(), dx ? rx.data_ptr() : nullptr,
                                       dw ? rg.data_ptr() : nullptr, dw ? ru.data_ptr() : nullptr, (int32_t)M, (int32_t)F,
                                       (int32_t)K, (int32_t)act, dt, stream(dev));
         if (rc) return PyLong_FromLong(rc);

@@ -77,6 +77,21 @@ inline int enc_map_2d(CUtensorMap* m, int dtype, const void* base, int64_t rows,
     return RAGRT_OK;
 }
 
+// f32 [rows, cols] matrix (cols a multiple of 4), box [32 rows x 32 cols], 128-byte swizzle, for stores.
+inline int enc_map_f32(CUtensorMap* m, const void* base, int64_t rows, int64_t cols) {
+    EncodeTiledFn fn = enc_encode_fn();
+    if (!fn) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)cols * 4};
+    const cuuint32_t box[2] = {32u, 32u};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RAGRT_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return RAGRT_OK;
+}
+
 // 16-bit [rows, heads, dim] tensor, rows `stride` elements apart, box [box_rows x 1 x 64]: one head's
 // columns of box_rows rows; columns behind dim and rows behind the last read 0.
 inline int enc_map_heads(CUtensorMap* m, int dtype, const void* base, int64_t rows, int heads, int dim, int64_t stride,

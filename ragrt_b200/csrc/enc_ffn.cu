@@ -18,8 +18,10 @@
 //   ffn_act_backward        dg and du, elementwise.
 //
 // The weight matrices and x are read as they lie: an operand whose contraction index is the row of
-// its matrix is fed to the tensor cores MN-major.  Accumulators are fp32; g and u are rounded once
-// where they are kept, dg and du where they become operands, results at the end.
+// its matrix is fed to the tensor cores MN-major.  Accumulators are fp32.  g and u are kept in fp32: in 16
+// bits their rounding would add as much to the gradients' error as the results' own does (bf16: 3.1e-3 of
+// the gradients' norm instead of 2.4e-3, for 360 MB less to move in a step of 8192 x 2048 -> 5504).  dg and du
+// are rounded where they become operands, results at the end.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -310,15 +312,15 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
                 if (!rows || at >= tile.cols) break;
                 if (kMode == kForward && p.keep) {
 #pragma unroll 1
-                    for (int w = 0; w < 2; ++w) {
+                    for (int w = 0; w < 4; ++w) {       // g and u, 32 columns at a time
+                        float f[32];
+                        tc::ld32x32(taddr + (w >> 1) * (kFN / 2) + c0 + 32 * (w & 1), *reinterpret_cast<uint32_t(*)[32]>(f));
+                        tc::wait_ld();
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float f[32];
-                            tc::ld32x32(taddr + w * (kFN / 2) + c0 + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(f));
-                            tc::wait_ld();
-                            put(c, f);
-                        }
-                        send(&maps.out[1 + w], at, y);
+                        for (int q = 0; q < 32; q += 4)
+                            *reinterpret_cast<float4*>(out + lane * 128 + (((q / 4) ^ (lane & 7)) << 4)) =
+                                make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]);
+                        if (at + 32 * (w & 1) < tile.cols) send(&maps.out[1 + (w >> 1)], at + 32 * (w & 1), y);
                     }
                 }
 #pragma unroll
@@ -512,10 +514,17 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
                             *reinterpret_cast<uint4*>(static_cast<T*>(base) + at + off + q) =
                                 down8<T>(*reinterpret_cast<const float(*)[8]>(x + q));
                 };
+                auto keep = [&](void* base, const float (&x)[32]) {
+#pragma unroll
+                    for (int q = 0; q < 32; q += 4)
+                        if (tile.n0 + q < tile.cols)
+                            *reinterpret_cast<float4*>(static_cast<float*>(base) + at + q) =
+                                make_float4(x[q], x[q + 1], x[q + 2], x[q + 3]);
+                };
                 if (kMode == kForward) {
                     if (p.keep) {
-                        put(p.out[1], 0, f);
-                        put(p.out[2], 0, v);
+                        keep(p.out[1], f);
+                        keep(p.out[2], v);
                     }
                     ffn_gate(f, v, p.act);
                     put(p.out[0], 0, f);
@@ -599,8 +608,8 @@ __global__ void __launch_bounds__(256) ffn_rows(const T* __restrict__ x, const T
             if (lane == 0) {
                 const int64_t at = (int64_t)r * p.F + f0 + c;
                 if (p.keep) {
-                    static_cast<T*>(p.out[1])[at] = (T)v[0];
-                    static_cast<T*>(p.out[2])[at] = (T)v[1];
+                    static_cast<float*>(p.out[1])[at] = v[0];
+                    static_cast<float*>(p.out[2])[at] = v[1];
                 }
                 static_cast<T*>(p.out[0])[at] = (T)(ffn_act(v[0], p.act) * v[1]);
             }
@@ -619,15 +628,18 @@ int ffn_rows_launch(const void* x, const void* wg, const void* wu, const FfnPara
 
 // dg = dh * u * act'(g), du = dh * act(g); a thread per 8 values
 template <typename T>
-__global__ void __launch_bounds__(256) ffn_act_backward(const T* __restrict__ dh, const T* __restrict__ gate,
-                                                        const T* __restrict__ up, T* __restrict__ dg,
+__global__ void __launch_bounds__(256) ffn_act_backward(const T* __restrict__ dh, const float* __restrict__ gate,
+                                                        const float* __restrict__ up, T* __restrict__ dg,
                                                         T* __restrict__ du, int64_t n8, int act) {
     pdl_wait_then_release();
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (int64_t)gridDim.x * blockDim.x) {
         float d[8], g[8], u[8], x[8], y[8];
         up8<T>(reinterpret_cast<const uint4*>(dh)[i], d);
-        up8<T>(reinterpret_cast<const uint4*>(gate)[i], g);
-        up8<T>(reinterpret_cast<const uint4*>(up)[i], u);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            *reinterpret_cast<float4*>(g + 4 * h) = __ldcs(reinterpret_cast<const float4*>(gate) + 2 * i + h);
+            *reinterpret_cast<float4*>(u + 4 * h) = __ldcs(reinterpret_cast<const float4*>(up) + 2 * i + h);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float a, da;
@@ -650,9 +662,10 @@ int ffn_maps(FfnMaps& m, int mode, bool pair, int dtype, const FfnParams& p, con
             (rc = enc_map_2d(&m.b[0], dtype, wg, p.F, p.K, p.K, wrows)) ||
             (rc = enc_map_2d(&m.b[1], dtype, wu, p.F, p.K, p.K, wrows)))
             return rc;
-        if (pair)
-            for (int i = 0; i < (p.keep ? 3 : 1); ++i)
-                if ((rc = enc_map_2d(&m.out[i], dtype, p.out[i], p.M, p.F, p.F, 32))) return rc;
+        if (pair && ((rc = enc_map_2d(&m.out[0], dtype, p.out[0], p.M, p.F, p.F, 32)) ||
+                     (p.keep && ((rc = enc_map_f32(&m.out[1], p.out[1], p.M, p.F)) ||
+                                 (rc = enc_map_f32(&m.out[2], p.out[2], p.M, p.F))))))
+            return rc;
         return RAGRT_OK;
     }
     if (p.dx && ((rc = enc_map_2d(&m.a[0], dtype, dg, p.M, p.F, p.F, pair ? kFM / 2 : p.a_rows)) ||
@@ -729,8 +742,8 @@ int ffn_check(int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype) {
 
 using namespace ragrt;
 
-extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const void* d_w_up, void* d_h, void* d_gate,
-                                   void* d_up, int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype,
+extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const void* d_w_up, void* d_h, float* d_gate,
+                                   float* d_up, int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype,
                                    void* stream_) {
     int rc = ffn_check(M, F, K, act, dtype);
     if (rc) return rc;
@@ -754,7 +767,7 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
 }
 
 extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* d_w_gate,
-                                            const void* d_w_up, const void* d_gate, const void* d_up, void* d_dgate,
+                                            const void* d_w_up, const float* d_gate, const float* d_up, void* d_dgate,
                                             void* d_dup, void* d_dx, void* d_dw_gate, void* d_dw_up, int32_t M,
                                             int32_t F, int32_t K, int32_t act, int32_t dtype, void* stream_) {
     int rc = ffn_check(M, F, K, act, dtype);
@@ -781,10 +794,10 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
     const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n8, 256), (int64_t)num_sms() * 16);
     rc = dtype == RAGRT_BF16
              ? enc_launch(ffn_act_backward<__nv_bfloat16>, dim3(blocks), dim3(256), 0, stream,
-                          (const __nv_bfloat16*)d_dh, (const __nv_bfloat16*)d_gate, (const __nv_bfloat16*)d_up,
+                          (const __nv_bfloat16*)d_dh, d_gate, d_up,
                           (__nv_bfloat16*)d_dgate, (__nv_bfloat16*)d_dup, n8, (int)act)
              : enc_launch(ffn_act_backward<__half>, dim3(blocks), dim3(256), 0, stream, (const __half*)d_dh,
-                          (const __half*)d_gate, (const __half*)d_up, (__half*)d_dgate, (__half*)d_dup, n8, (int)act);
+                          d_gate, d_up, (__half*)d_dgate, (__half*)d_dup, n8, (int)act);
     if (rc) return rc;
     if (!d_dx && !d_dw_gate) return RAGRT_OK;
     FfnParams p{M, F, K, act, 0, d_dx != nullptr, d_dw_gate != nullptr, 0, {d_dx, d_dw_gate, d_dw_up}, err};

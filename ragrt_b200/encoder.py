@@ -341,8 +341,8 @@ def _ffn_args(x, w_gate, w_up, act):
 def gated_ffn(x, w_gate, w_up, act="silu", keep=False, out=None):
     """h [M, F] = act(x w_gate^T) * (x w_up^T) in one kernel: x [M, K], weights [F, K] (the halves of
     a stacked [2 F, K] matrix are read in place), fp16 or bf16, F and K multiples of 8; act "silu",
-    "gelu" (erf form) or "gelu_tanh".  keep=True returns (h, gate, up) with the two products that
-    gated_ffn_backward wants.  Not tracked by autograd."""
+    "gelu" (erf form) or "gelu_tanh".  keep=True returns (h, gate, up) with the two products in
+    fp32, which gated_ffn_backward wants.  Not tracked by autograd."""
     if out is None and act in _ACTS:
         r = (_bound or _bind()).gated_ffn(x, w_gate, w_up, _ACTS[act], keep)
         if r is not None:
@@ -357,7 +357,7 @@ def gated_ffn(x, w_gate, w_up, act="silu", keep=False, out=None):
         _check_output(out, (M, F), x.dtype, (x, wg, wu))
     gate = up = None
     if keep:
-        gate, up = torch.empty_like(out), torch.empty_like(out)
+        gate, up = torch.empty_like(out, dtype=torch.float32), torch.empty_like(out, dtype=torch.float32)
     rc = _lib.lib().ragrt_enc_gated_ffn(
         x.data_ptr(), wg.data_ptr(), wu.data_ptr(), out.data_ptr(), gate.data_ptr() if keep else None,
         up.data_ptr() if keep else None, M, F, K, _ACTS[act], dt, _raw_stream(x))
@@ -374,13 +374,15 @@ def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu", need_dx=True, 
         if r is not None:
             return _lib.check(r) if type(r) is int else r
     _need_cuda(dh, x, w_gate, w_up, gate, up)
-    dt = _dtype16(dh, x, w_gate, w_up, gate, up)
+    dt = _dtype16(dh, x, w_gate, w_up)
+    if gate.dtype is not torch.float32 or up.dtype is not torch.float32:
+        raise RuntimeError(f"gate and up must be fp32, as gated_ffn keeps them; got {gate.dtype} and {up.dtype}")
     M, F, K = _ffn_args(x, w_gate, w_up, act)
     if dh.shape != (M, F) or gate.shape != (M, F) or up.shape != (M, F):
         raise RuntimeError(f"dh, gate and up must be {(M, F)}; got {tuple(dh.shape)}, {tuple(gate.shape)}, "
                            f"{tuple(up.shape)}")
     dh, x, wg, wu, gate, up = (_solid(t) for t in (dh, x, w_gate, w_up, gate, up))
-    dgate, dup = torch.empty_like(gate), torch.empty_like(up)
+    dgate, dup = torch.empty_like(dh), torch.empty_like(dh)
     dx = torch.empty_like(x) if need_dx else None
     dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_dw else (None, None)
     _lib.check(_lib.lib().ragrt_enc_gated_ffn_backward(

@@ -94,11 +94,11 @@ def ffn64(x, wg, wu, act):
     h = a * u
     # the activation's exp is good to 2^-17 for arguments up to 88
     bh = 1.02 * (e * h.abs() + LIP * eg * u.abs() + (a.abs() + LIP * eg) * eu + 2.0 ** -16 * (g * u).abs() + tiny)
-    return h, g, u, bh, 1.02 * (e * g.abs() + eg + tiny), 1.02 * (e * u.abs() + eu + tiny)
+    return h, g, u, bh, 1.02 * eg, 1.02 * eu                 # g and u are kept in fp32
 
 
 def ffn_backward64(dh, x, wg, wu, gate, up, act):
-    """Gradients of the formula at the kept (rounded) gate and up, and their bounds: dg and du are
+    """Gradients of the formula at the kept gate and up, and their bounds: dg and du are
     rounded to the type before they are multiplied."""
     e, tiny = EPS[x.dtype], TINY[x.dtype]
     dh, x, wg, wu, g, u = (t.double() for t in (dh, x, wg, wu, gate, up))

@@ -159,8 +159,11 @@ def test_python_checks_of_gated_ffn(on_host):
         encoder.gated_ffn(x, w.bfloat16(), w)
     with pytest.raises(RuntimeError, match="out must be"):
         encoder.gated_ffn(x, w, w, out=h[:3])
+    kept = h.float()
     with pytest.raises(RuntimeError, match="must be"):
-        encoder.gated_ffn_backward(h[:, :64], x, w, w, h, h)
+        encoder.gated_ffn_backward(h[:, :64], x, w, w, kept, kept)
+    with pytest.raises(RuntimeError, match="fp32"):
+        encoder.gated_ffn_backward(h, x, w, w, h, h)
     square = torch.zeros(128, 64, dtype=H16)
     with pytest.raises(RuntimeError, match="overlaps"):
         encoder.gated_ffn(square, torch.zeros(64, 64, dtype=H16), torch.zeros(64, 64, dtype=H16), out=square)

@@ -300,12 +300,12 @@ def test_gated_ffn_gradients_against_differences(act):
     _, gate, up = encoder.gated_ffn(x, wg, wu, act=act, keep=True)
     grads = encoder.gated_ffn_backward(dh, x, wg, wu, gate, up, act=act)
     bounds = [b for _, b in L.ffn_backward64(dh, x, wg, wu, gate, up, act)]
-    e = L.EPS[torch.float16]
     base = [t.double() for t in (x, wg, wu)]
     g, u = gate.double().abs(), up.double().abs()
-    # the gradients are taken at the kept gate and up, which are rounded: dg and du move by at most this
-    dg = dh.double().abs() * (L.LIP * u * e + u * L.BEND * g * e) * 1.05
-    du = dh.double().abs() * L.LIP * g * e * 1.05
+    _, _, _, _, eg, eu = L.ffn64(x, wg, wu, act)
+    # the gradients are taken at the kept gate and up, which are off by eg and eu: dg and du move by at most this
+    dg = dh.double().abs() * (L.LIP * eu + u * L.BEND * eg) * 1.05
+    du = dh.double().abs() * L.LIP * eg * 1.05
     moved = [dg @ base[1].abs() + du @ base[2].abs(), dg.T @ base[0].abs(), du.T @ base[0].abs()]
 
     def loss(ts):
