@@ -635,7 +635,8 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                     announce(0);
                 } else {
                     float s[N];
-                    if (!idle && first >= own.lo && first + N <= wall) {
+                    const bool all = !idle && first >= own.lo && first + N <= wall;
+                    if (all) {
 #pragma unroll
                         for (int c = 0; c < N / 32; ++c)
                             tc::ld32x32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
@@ -656,12 +657,22 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                     (void)refer(mx);
                     const float ref = m == -INFINITY ? 0.f : m;
                     const uint64_t ref2 = pack2(-ref, -ref);
+                    if (all) {                                    // straight code: no step waits for a branch
 #pragma unroll
-                    for (int c = 0; c < N / 32; ++c) {
-                        uint32_t w[16] = {};
-                        if (seen(c)) l += attn_weights<T>(s + 32 * c, scale22, ref2, w);
-                        tc::st32x16(ts + 16 * c, w);
-                        if (c & 1) announce(c / 2);
+                        for (int c = 0; c < N / 32; ++c) {
+                            uint32_t w[16];
+                            l += attn_weights<T>(s + 32 * c, scale22, ref2, w);
+                            tc::st32x16(ts + 16 * c, w);
+                            if (c & 1) announce(c / 2);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < N / 32; ++c) {
+                            uint32_t w[16] = {};
+                            if (seen(c)) l += attn_weights<T>(s + 32 * c, scale22, ref2, w);
+                            tc::st32x16(ts + 16 * c, w);
+                            if (c & 1) announce(c / 2);
+                        }
                     }
                 }
             }
