@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/ragrt_b200.h"
@@ -49,18 +50,12 @@ bool fits(int64_t n) { return n >= 0 && n <= 0x7FFFFFFF; }
 at::Tensor like(const at::Tensor& t, at::IntArrayRef shape) { return at::empty(shape, t.options().requires_grad(false)); }
 void* stream(int device) { return (void*)at::cuda::getCurrentCUDAStream(device).stream(); }
 
-// A C++ exception (out of memory, above all) becomes Python's error.
+// A C++ exception becomes Python's error, as torch itself translates it (out of memory above all).
 template <typename F>
 PyObject* guarded(F f) {
-    try {
-        return f();
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
-    } catch (...) {
-        PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
-        return nullptr;
-    }
+    HANDLE_TH_ERRORS
+    return f();
+    END_HANDLE_TH_ERRORS
 }
 
 PyObject* bind(PyObject*, PyObject* args) {

@@ -266,7 +266,7 @@ def packed_attention(q, k, v, cu_seqlens, causal=False, scale=None, out=None):
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise RuntimeError("cu_seqlens must be int32 [B + 1]")
     if cu_seqlens.dtype is not torch.int32 or not cu_seqlens.is_contiguous():
-        cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        cu_seqlens = cu_seqlens.clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()
     (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
     T, H, D = shape
     if out is None:

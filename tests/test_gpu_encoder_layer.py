@@ -185,6 +185,64 @@ def test_attention_bad_table_raises_the_flag(table):
     assert flag() == 0
 
 
+@pytest.mark.parametrize("D", [16, 24, 40, 72, 104, 120])
+def test_attention_other_head_sizes(D):
+    lens = [70, 3, 140]
+    q, k, v = qkv_of(lens, 3, 1, D, torch.bfloat16, seed=D)
+    cu = L.cu_of(lens, "cuda")
+    want, bound = L.attention64(q, k, v, cu, True)
+    L.check(encoder.packed_attention(q, k, v, cu, causal=True), want, bound)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_many_short_and_empty_sequences(D, causal):
+    """More sequences than the search looks at in two steps, most of them of a few rows or none."""
+    g = torch.Generator().manual_seed(1)
+    lens = torch.randint(0, 4, (2500,), generator=g).tolist() + [0] * 600 + [130] + [0] * 700
+    q, k, v = qkv_of(lens, 2, 1, D, torch.float16, seed=20)
+    cu = L.cu_of(lens, "cuda")
+    want, bound = L.attention64(q, k, v, cu, causal)
+    L.check(encoder.packed_attention(q, k, v, cu, causal=causal), want, bound)
+    assert flag() == 0
+
+
+def test_attention_nothing_but_empty_sequences():
+    q, k, v = qkv_of([0], 2, 2, 64, torch.float16, seed=1, spare=300)
+    out = torch.full(q.shape, 5.0, dtype=torch.float16, device="cuda")
+    encoder.packed_attention(q, k, v, torch.zeros(400, dtype=torch.int32, device="cuda"), out=out)
+    assert (out == 5.0).all() and flag() == 0
+    assert encoder.packed_attention(q[:0], k[:0], v[:0], L.cu_of([0], "cuda")).shape == (0, 2, 64)
+    encoder.packed_attention(q, k, v, L.cu_of([], "cuda"), out=out)
+    assert (out == 5.0).all()
+
+
+def test_attention_64_bit_tables():
+    q, k, v = qkv_of([90, 11], 2, 2, 64, torch.float16, seed=12)
+    cu = L.cu_of([90, 11], "cuda")
+    assert torch.equal(encoder.packed_attention(q, k, v, cu.long()), encoder.packed_attention(q, k, v, cu))
+    flag()
+    far = torch.tensor([0, 90, 2 ** 32 + 101], device="cuda")          # does not come back as 101
+    encoder.packed_attention(q, k, v, far)
+    assert flag() == 6
+
+
+def test_attention_on_two_streams_at_once():
+    sets = [qkv_of([700, 40, 333], 4, 2, D, torch.float16, seed=D) for D in (64, 128)]
+    cu = L.cu_of([700, 40, 333], "cuda")
+    want = [encoder.packed_attention(*s, cu, causal=True) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(encoder.packed_attention(*s, cu, causal=True))
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 2])
+
+
 # ------------------------------------------------------------------------------------ norm + rotary
 def tables(n, R):
     a = torch.arange(n, device="cuda", dtype=torch.float64)[:, None] * 10000.0 ** (
@@ -228,6 +286,17 @@ def test_norm_rope_in_place_and_zero_rows():
     e = torch.empty(0, 12, 64, dtype=torch.float16, device="cuda")
     qz, kz = encoder.qk_norm_rope(e, e, cos, sin, pos[:0], w, w)
     assert qz.shape == (0, 12, 64) and kz.shape == (0, 12, 64)
+
+
+def test_norm_rope_of_queries_alone():
+    q, _, _ = qkv_of([50], 4, 1, 64, torch.float16, seed=3)
+    none = torch.empty(50, 0, 64, dtype=torch.float16, device="cuda")
+    cos, sin = tables(64, 64)
+    pos = torch.arange(50, device="cuda")
+    w = torch.ones(64, dtype=torch.float16, device="cuda")
+    qo, ko = encoder.qk_norm_rope(q, none, cos, sin, pos, w)
+    L.check(qo, *L.rms_rope64(q, w, cos, sin, pos, 1e-6, False))
+    assert ko.shape == (50, 0, 64)
 
 
 @pytest.mark.parametrize("pos", [-1, 512, 2 ** 40])
