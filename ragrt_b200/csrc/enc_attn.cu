@@ -688,6 +688,8 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             // the accumulator read.
             const float inv = 1.0f / l;
             T* dst = static_cast<T*>(p.out) + row * p.out_stride + (int64_t)b.head * p.dim;
+            // whole sectors where the rows allow it: half as many stores, each to 32 rows
+            const bool sectors = ((uintptr_t)p.out & 31) == 0 && p.out_stride % 16 == 0 && p.dim % 16 == 0;
             bool bad = false;
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
@@ -700,7 +702,13 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                     odd = fmaf(o[q], 0.f, odd);                   // NaN as soon as one is not finite
                 }
                 bad = bad || (mine && !(odd == 0.f));
-                if (mine) {
+                if (mine && sectors) {
+#pragma unroll
+                    for (int q = 0; q < 32; q += 16)
+                        if (c + q < p.dim)
+                            store32(dst + c + q, down8<T>(*reinterpret_cast<float(*)[8]>(o + q)),
+                                    down8<T>(*reinterpret_cast<float(*)[8]>(o + q + 8)));
+                } else if (mine) {
 #pragma unroll
                     for (int q = 0; q < 32; q += 8)
                         if (c + q < p.dim) *reinterpret_cast<uint4*>(dst + c + q) = down8<T>(*reinterpret_cast<float(*)[8]>(o + q));

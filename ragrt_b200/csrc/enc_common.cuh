@@ -166,6 +166,13 @@ __device__ __forceinline__ uint4 down8(const float (&f)[8]) {
     return u;
 }
 
+// 32 bytes at once, a whole sector (address a multiple of 32)
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+
 // ------------------------------------------------------------------ fp32 pairs
 // two fp32 values side by side, one instruction for both
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
