@@ -9,6 +9,18 @@
 //                      Warp 0 streams Q and the blocks of K and V by TMA, warp 1 issues the products
 //                      (S = Q K^T and O += P V, P from tensor memory), warp 2 finds the coming items'
 //                      sequences, and per tile four warps run the softmax, a thread per row.
+//                      Heads wider than 64 are bound by the turn of a tile: per 128 keys about 2,300 cycles of
+//                      softmax (two warps share an exponential unit that needs 1,024 for each), then P V and
+//                      the next Q K^T (16 products of about 95 cycles; a 128-row operand from shared memory
+//                      takes that long whatever the width of the other).  One sequence of 16,384 rows, 16
+//                      heads of 128, causal: 0.92 ms, 1,190 TFLOP/s.  Heads of up to 64 over short sequences
+//                      are bound by instruction issue and fetch: 1,024 passages of 20-180 rows, 12 heads:
+//                      195 us, 3.2 TB/s.  Tried and dropped: tiles over the rows as they lie, several sequences
+//                      in one (masks cost more than the rows saved: 263 us); 64-key blocks with two score
+//                      buffers for wide heads (1.59 ms: twice the products at the same 95 cycles); a quarter
+//                      of the exponentials as polynomials on the FMA units (0.97 ms: issue, not that unit,
+//                      is short); two tiles of one CTA with an issuing warp each (1.20 ms: they fall into
+//                      step and want the same units at the same time).
 //   attn_row           one row of one head by a warp, in fp32.  A weight of zero does not keep a NaN or
 //                      an infinity in a masked row of V out of a matrix product: rows that come out
 //                      of it not finite are computed once more by this, over their own keys alone.
