@@ -15,7 +15,11 @@
 //                           tiles where the large ones would leave SMs without work.
 //   ffn_rows                forward of up to four rows: a warp per pair of weight rows, fp32 on the CUDA
 //                           cores, bound by the weights' bytes.
-//   ffn_act_backward        dg and du, elementwise.
+//   ffn_act_backward        dg and du, elementwise; at memory speed (8192 x 5504: 97 us, 6.5 TB/s).
+//
+// Measured: 16384 x 2048 -> 8192 forward 688 us in a burst (1,600 TFLOP/s; 810 us, 1,360 TFLOP/s, under the
+// power cap); a training step of 8192 x 2048 -> 5504 237 us forward, 40 more for keeping g and u, 670
+// backward (cuBLAS for the three products alone: 251, 246 and 258 us).
 //
 // The weight matrices and x are read as they lie: an operand whose contraction index is the row of
 // its matrix is fed to the tensor cores MN-major.  Accumulators are fp32.  g and u are kept in fp32: in 16

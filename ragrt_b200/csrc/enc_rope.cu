@@ -7,7 +7,9 @@
 // The pass is bound by memory (each value is read once and written once).  A lane holds two 8-value
 // chunks of a head that rotate with one another, so that a head is ceil(dim / 16) lanes, the
 // rotation needs no exchange, the mean a few shuffles, and a lane's cos / sin stay in registers
-// while its warp walks the heads of one token.
+// while its warp walks the heads of one token.  Measured: 102,411 tokens of 24 heads of 64 (32 values
+// turned) 125 us, 5.0 TB/s; 32,768 tokens of 40 heads of 128 125 us, 5.5 TB/s.  What is left of the way to
+// a copy's 6.5 is issue: about 230 instructions per warp for 512 values.
 #include <algorithm>
 
 #include "enc_common.cuh"
