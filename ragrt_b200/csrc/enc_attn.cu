@@ -9,11 +9,11 @@
 //                      Warp 0 streams Q and the blocks of K and V by TMA, warp 1 issues the products
 //                      (S = Q K^T and O += P V, P from tensor memory), warp 2 finds the coming items'
 //                      sequences, and per tile four warps run the softmax, a thread per row.
-//                      Heads wider than 64 are bound by the turn of a tile: per 128 keys about 2,300 cycles of
+//                      CTAs of two tiles are bound by the turn of a tile: per 128 keys about 2,300 cycles of
 //                      softmax (two warps share an exponential unit that needs 1,024 for each), then P V and
 //                      the next Q K^T (16 products of about 95 cycles; a 128-row operand from shared memory
 //                      takes that long whatever the width of the other).  One sequence of 16,384 rows, 16
-//                      heads of 128, causal: 0.92 ms, 1,190 TFLOP/s.  Heads of up to 64 over short sequences
+//                      heads of 128, causal: 0.92 ms, 1,190 TFLOP/s.  CTAs of one tile, for short sequences,
 //                      are bound by instruction issue and fetch: 1,024 passages of 20-180 rows, 12 heads:
 //                      195 us, 3.2 TB/s.  Tried and dropped: tiles over the rows as they lie, several sequences
 //                      in one (masks cost more than the rows saved: 263 us); 64-key blocks with two score
@@ -144,25 +144,28 @@ constexpr int kAItems = 2;                     // items whose tiles are in share
 // at most 256, well inside either type, and the accumulator is not rescaled.
 constexpr float kARescale = 8.0f;
 
-// Heads of up to 64: CTAs of one tile, four to an SM, so that the many short steps of short sequences
-// (loads, products, weights, stores) of one run while another's wait.  Wider heads: two tiles that share
+// CTAs of one tile, several to an SM, so that the many short steps of short sequences (loads, products,
+// weights, stores) of one run while another's wait; and for long sequences CTAs of two tiles that share
 // K and V and take turns, one's products running while the other's weights are computed.
-template <int DP>
+template <int DP_, int kTiles_>
 struct AttnCfg {
-    static constexpr int kTiles = DP == 128 ? 2 : 1;
-    static constexpr int kCtas = DP == 128 ? 1 : 4;               // per SM
+    static constexpr int DP = DP_, kTiles = kTiles_;              // columns of a head, tiles
+    static constexpr int kCtas = kTiles == 2 ? 1 : DP == 128 ? 2 : 4;        // per SM
     static constexpr int kThreads = 32 * (kAFirst + 4 * kTiles);
-    static constexpr int kN = DP == 128 ? 128 : 64;               // keys per block
+    static constexpr int kN = kTiles == 2 ? 128 : 64;             // keys per block
     static constexpr int kHalves = kN / 64;                       // a block's weights are announced 64 at a time
-    static constexpr bool kSteps = DP != 128;                     // a row's scores are held 32 at a time, not a block's
+    static constexpr bool kSteps = kTiles == 1;                   // a row's scores are held 32 at a time, not a block's
     static constexpr int kTileQ = kAM * DP * 2;                   // bytes of a Q tile
     static constexpr int kTileK = kN * DP * 2;                    // bytes of a K or a V block
     static constexpr int kStages = 2;                             // K blocks, and V blocks, in flight
     static constexpr int kSmem = 1024 + kTiles * kTileQ + 2 * kStages * kTileK + 1024;
     static constexpr uint32_t kO = kTiles * kN;                   // first accumulator column: S and P lie before
-    static constexpr uint32_t kCols = kO + kTiles * DP;           // tensor-memory columns
+    static constexpr uint32_t kCols = 512 / kCtas;                // tensor-memory columns: a power of two
+    static_assert(kO + kTiles * DP <= kCols, "tensor memory");
     // The launch's registers, dealt out anew: a softmax thread holds its row of scores.
-    static constexpr int kRegs = DP == 128 ? 168 : 64, kRegsFew = DP == 128 ? 88 : 40, kRegsMany = DP == 128 ? 208 : 88;
+    static constexpr int kRegs = kTiles == 2 ? 168 : DP == 128 ? 128 : 64;
+    static constexpr int kRegsFew = kTiles == 2 ? 88 : DP == 128 ? 80 : 40;
+    static constexpr int kRegsMany = kTiles == 2 ? 208 : DP == 128 ? 176 : 88;
     static_assert(128 * kRegsFew + (kThreads - 128) * kRegsMany <= kThreads * kRegs, "more registers than the launch holds");
 };
 
@@ -189,9 +192,9 @@ __device__ __forceinline__ bool attn_wait(uint64_t* m, uint32_t parity, volatile
 }
 
 // What the roles hand one another, behind the tiles in shared memory.
-template <int DP>
+template <class Cfg>
 struct AttnShared {
-    static constexpr int kTiles = AttnCfg<DP>::kTiles, kStages = AttnCfg<DP>::kStages;
+    static constexpr int kTiles = Cfg::kTiles, kStages = Cfg::kStages;
     AttnTile tile[kAItems][kTiles];
     uint4 answer;                            // to a request for the next item
     int head[kAItems], group[kAItems];       // query and key head; head < 0: no more items
@@ -199,7 +202,7 @@ struct AttnShared {
     uint64_t qfull, qempty;
     uint64_t ifull[kAItems], iempty[kAItems];
     uint64_t sfull[kTiles];                  // scores ready (MMA -> softmax)
-    uint64_t pready[kTiles][AttnCfg<DP>::kHalves];       // weights written (softmax -> MMA)
+    uint64_t pready[kTiles][Cfg::kHalves];       // weights written (softmax -> MMA)
     uint64_t odone[kTiles];                  // product with V done
     uint64_t drain, taken;
     uint32_t tmem;
@@ -207,22 +210,22 @@ struct AttnShared {
 };
 
 // The blocks of an item: blocks 0 .. n - 1 from key kv0 on, tile t takes [jb[t], je[t]) of them.
-template <int DP>
+template <class Cfg>
 struct AttnBlocks {
-    int head = -1, group, kv0, n = 0, jb[AttnCfg<DP>::kTiles], je[AttnCfg<DP>::kTiles];
-    __device__ __forceinline__ void get(const AttnShared<DP>* sh, int r) {
+    int head = -1, group, kv0, n = 0, jb[Cfg::kTiles], je[Cfg::kTiles];
+    __device__ __forceinline__ void get(const AttnShared<Cfg>* sh, int r) {
         head = sh->head[r];
         group = sh->group[r];
         kv0 = 0x7FFFFFFF;
         n = 0;
 #pragma unroll
-        for (int t = 0; t < AttnCfg<DP>::kTiles; ++t)
+        for (int t = 0; t < Cfg::kTiles; ++t)
             if (sh->tile[r][t].rows > 0) kv0 = min(kv0, sh->tile[r][t].lo);
 #pragma unroll
-        for (int t = 0; t < AttnCfg<DP>::kTiles; ++t) {
+        for (int t = 0; t < Cfg::kTiles; ++t) {
             const bool any = sh->tile[r][t].rows > 0;
-            jb[t] = any ? (unsigned)(sh->tile[r][t].lo - kv0) / AttnCfg<DP>::kN : 0;
-            je[t] = any ? (unsigned)(sh->tile[r][t].hi - kv0 + AttnCfg<DP>::kN - 1) / AttnCfg<DP>::kN : 0;
+            jb[t] = any ? (unsigned)(sh->tile[r][t].lo - kv0) / Cfg::kN : 0;
+            je[t] = any ? (unsigned)(sh->tile[r][t].hi - kv0 + Cfg::kN - 1) / Cfg::kN : 0;
             n = max(n, je[t]);
         }
     }
@@ -230,13 +233,13 @@ struct AttnBlocks {
 
 // A walk of a thread or a whole warp over the blocks of its CTA's items; gives the items' records back
 // behind itself (by the lane with `lead` set).
-template <int DP>
+template <class Cfg>
 struct AttnWalk {
-    AttnBlocks<DP> b;
+    AttnBlocks<Cfg> b;
     int rec = -1, j = 0;
     bool lead = true;
     // On to the next block; 1: there is one, 0: no more, -1: gave up waiting.
-    __device__ __forceinline__ int next(AttnShared<DP>* sh) {
+    __device__ __forceinline__ int next(AttnShared<Cfg>* sh) {
         if (j + 1 < b.n) {
             ++j;
             return 1;
@@ -279,18 +282,17 @@ __device__ __forceinline__ float attn_weights(const float* s, uint64_t scale, ui
     return x + y;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(AttnCfg<DP>::kThreads, AttnCfg<DP>::kCtas)
+template <typename T, class Cfg>
+__global__ void __launch_bounds__(Cfg::kThreads, Cfg::kCtas)
 packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
-    using Cfg = AttnCfg<DP>;
-    constexpr int S = Cfg::kStages, N = Cfg::kN, kTiles = Cfg::kTiles;
+    constexpr int S = Cfg::kStages, N = Cfg::kN, kTiles = Cfg::kTiles, DP = Cfg::DP;
     extern __shared__ uint8_t attn_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)attn_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sQ = sm;
     uint8_t* sK = sm + kTiles * Cfg::kTileQ;
     uint8_t* sV = sK + S * Cfg::kTileK;
-    AttnShared<DP>* sh = reinterpret_cast<AttnShared<DP>*>(sV + S * Cfg::kTileK);
-    static_assert(sizeof(AttnShared<DP>) <= 1024, "shared memory of the roles");
+    AttnShared<Cfg>* sh = reinterpret_cast<AttnShared<Cfg>*>(sV + S * Cfg::kTileK);
+    static_assert(sizeof(AttnShared<Cfg>) <= 1024, "shared memory of the roles");
     volatile int* abort = sh->abort;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -332,7 +334,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsFew));
         if (warp == 0 && lane == 0) {
             // -------------------------------------------------------- TMA producer
-            AttnWalk<DP> walk;
+            AttnWalk<Cfg> walk;
             int n = 0, nq = 0;                                    // blocks and items
             auto slot = [&](uint64_t* full, uint64_t* empty) {
                 if (n >= S && !attn_wait(empty + n % S, (n / S - 1) & 1, abort)) return false;
@@ -387,7 +389,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             constexpr uint32_t idS = tc::idesc_f16_f32(kAM, N) | idesc_type<T>();
             constexpr uint32_t idO = tc::idesc_f16_f32(kAM, DP) | idesc_type<T>() | kIdescBMn;
             const uint32_t lead = tc::elect_one();
-            AttnWalk<DP> walk;                                    // of the scores; the products with V are
+            AttnWalk<Cfg> walk;                                    // of the scores; the products with V are
             int vj = 0, vjb[kTiles], vje[kTiles];                 // one block behind it, at vj
             walk.lead = lead != 0;
             uint32_t np[kTiles] = {};                             // products of each tile
@@ -549,7 +551,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                 failed = true;
                 break;
             }
-            AttnBlocks<DP> b;
+            AttnBlocks<Cfg> b;
             b.get(sh, r);
             const AttnTile own = sh->tile[r][tile];
             __syncwarp();
@@ -747,21 +749,31 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
     }
 }
 
-template <typename T, int DP>
+template <typename T, class Cfg>
 int attn_launch(int dtype, AttnParams p, cudaStream_t stream) {
     static std::atomic<uint64_t> done{0};
-    int rc = enc_allow_smem(packed_attn_mma<T, DP>, AttnCfg<DP>::kSmem, done);
+    int rc = enc_allow_smem(packed_attn_mma<T, Cfg>, Cfg::kSmem, done);
     if (rc) return rc;
     AttnMaps m;
     if ((rc = enc_map_heads(&m.q, dtype, p.q, p.T, p.heads, p.dim, p.q_stride, kAM)) ||
-        (rc = enc_map_heads(&m.k, dtype, p.k, p.T, p.kv_heads, p.dim, p.k_stride, AttnCfg<DP>::kN)) ||
-        (rc = enc_map_heads(&m.v, dtype, p.v, p.T, p.kv_heads, p.dim, p.v_stride, AttnCfg<DP>::kN)))
+        (rc = enc_map_heads(&m.k, dtype, p.k, p.T, p.kv_heads, p.dim, p.k_stride, Cfg::kN)) ||
+        (rc = enc_map_heads(&m.v, dtype, p.v, p.T, p.kv_heads, p.dim, p.v_stride, Cfg::kN)))
         return rc;
-    const int64_t groups = ceil_div(p.T / kAM + (int64_t)p.B, AttnCfg<DP>::kTiles);
+    const int64_t groups = ceil_div(p.T / kAM + (int64_t)p.B, Cfg::kTiles);
     if (groups * p.heads > 0x7FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many rows x heads");
     p.items = (int)(groups * p.heads);
-    return enc_launch(packed_attn_mma<T, DP>, dim3((unsigned)p.items), dim3(AttnCfg<DP>::kThreads), AttnCfg<DP>::kSmem,
-                      stream, m, p);
+    return enc_launch(packed_attn_mma<T, Cfg>, dim3((unsigned)p.items), dim3(Cfg::kThreads), Cfg::kSmem, stream, m, p);
+}
+
+template <typename T>
+int attn_launch_sized(int dtype, const AttnParams& p, cudaStream_t stream) {
+    // Two tiles where a row sees many keys: as far as the host knows, the mean length (half of it, causal).
+    // 65536 rows of 16 heads, one tile / two: heads of 128, full, length 100 226 / 345 us, 512 536 / 543, 768
+    // 733 / 640, 2048 1761 / 1214; causal, 1024 596 / 619, 2048 1026 / 828; heads of 64, full, 100 151 / 321,
+    // 1024 602 / 641, 2048 1114 / 1042; causal, 2048 668 / 729, 8192 (half the rows) 1124 / 881.
+    const bool wide = p.dim > 64, two = p.T / p.B / (p.causal ? 2 : 1) >= (wide ? 544 : 1536);
+    if (wide) return two ? attn_launch<T, AttnCfg<128, 2>>(dtype, p, stream) : attn_launch<T, AttnCfg<128, 1>>(dtype, p, stream);
+    return two ? attn_launch<T, AttnCfg<64, 2>>(dtype, p, stream) : attn_launch<T, AttnCfg<64, 1>>(dtype, p, stream);
 }
 
 }  // namespace
@@ -798,8 +810,5 @@ extern "C" int ragrt_enc_packed_attention(const void* d_q, const void* d_k, cons
     AttnParams p{d_q, d_k, d_v, d_out, d_cu_seqlens, q_stride, k_stride, v_stride, out_stride, T, B, heads, kv_heads,
                  head_dim, causal != 0, 0, scale, err};
     cudaStream_t stream = (cudaStream_t)stream_;
-    if (dtype == RAGRT_BF16)
-        return head_dim <= 64 ? attn_launch<__nv_bfloat16, 64>(dtype, p, stream)
-                              : attn_launch<__nv_bfloat16, 128>(dtype, p, stream);
-    return head_dim <= 64 ? attn_launch<__half, 64>(dtype, p, stream) : attn_launch<__half, 128>(dtype, p, stream);
+    return dtype == RAGRT_BF16 ? attn_launch_sized<__nv_bfloat16>(dtype, p, stream) : attn_launch_sized<__half>(dtype, p, stream);
 }

@@ -49,7 +49,9 @@ def test_attention(lens, heads, causal, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lens,heads,causal", [([4100], (2, 1, 128), True), ([3000, 1500], (1, 1, 64), False),
-                                               ([2048], (4, 2, 64), True)])
+                                               ([2048], (4, 2, 64), True), ([4000, 2300], (2, 1, 64), True),
+                                               ([700, 5, 1900], (3, 1, 96), False), ([1, 4200], (1, 1, 40), True),
+                                               ([130, 0, 3000, 129], (2, 2, 128), True), ([1200], (1, 1, 80), True)])
 def test_attention_long(lens, heads, causal, dtype):
     q, k, v = qkv_of(lens, *heads, dtype, seed=5)
     cu = L.cu_of(lens, "cuda")
@@ -58,9 +60,10 @@ def test_attention_long(lens, heads, causal, dtype):
 
 
 @pytest.mark.parametrize("causal", [False, True])
-def test_attention_growing_scores(causal):
+@pytest.mark.parametrize("n,D", [(700, 64), (700, 128), (3300, 64)])
+def test_attention_growing_scores(n, D, causal):
     """Scores that rise along the keys, far beyond one another: the running maximum moves in every block."""
-    n, H, D = 700, 2, 64
+    H = 2
     q, k, v = qkv_of([n], H, H, D, torch.bfloat16, seed=9)
     k = k.clone()
     k[..., 0] = torch.linspace(-60, 60, n, device="cuda")[:, None]
@@ -98,6 +101,24 @@ def test_attention_keeps_what_is_not_seen_out(causal, D, bad):
         seen[250:310] = False
     L.check(got[seen], clean[seen], bound[seen])
     assert (got[319:] == 7.0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_keeps_unseen_values_out_of_long_sequences(D):
+    """The same for the tiles of long sequences: a neighbour's NaN, and a later row's."""
+    lens = [3300, 900, 3300]
+    q, k, v = qkv_of(lens, 2, 1, D, torch.float16, seed=13)
+    cu = L.cu_of(lens, "cuda")
+    clean, bound = L.attention64(q, k, v, cu, True)
+    q, k, v = q.clone(), k.clone(), v.clone()
+    for t in (k, v):
+        t[3300:4200] = math.nan
+        t[7490:] = math.inf
+    seen = torch.ones(7500, dtype=torch.bool, device="cuda")
+    seen[3300:4200] = False
+    seen[7490:] = False
+    got = encoder.packed_attention(q, k, v, cu, causal=True)
+    L.check(got[seen], clean[seen], bound[seen])
 
 
 def test_attention_spread_of_a_bad_row_is_the_formulas():
@@ -228,8 +249,9 @@ def test_attention_64_bit_tables():
 
 
 def test_attention_on_two_streams_at_once():
-    sets = [qkv_of([700, 40, 333], 4, 2, D, torch.float16, seed=D) for D in (64, 128)]
-    cu = L.cu_of([700, 40, 333], "cuda")
+    lens = [3000, 40, 1733]                              # two tiles a CTA for heads of 128, one for 64
+    sets = [qkv_of(lens, 4, 2, D, torch.float16, seed=D) for D in (64, 128)]
+    cu = L.cu_of(lens, "cuda")
     want = [encoder.packed_attention(*s, cu, causal=True) for s in sets]
     streams = [torch.cuda.Stream() for _ in sets]
     torch.cuda.synchronize()
