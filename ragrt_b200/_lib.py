@@ -69,7 +69,8 @@ _SIGS = {
     "ragrt_enc_qk_norm_rope": (I32, [P, P, P, P, P, P, P, I32, P, P, I32, I32, I32, I32, I32, I32, I64, I64, I64, I64,
                                      C.c_float, I32, I32, P]),
     "ragrt_enc_gated_ffn": (I32, [P, P, P, P, P, P, I32, I32, I32, I32, I32, P]),
-    "ragrt_enc_gated_ffn_backward": (I32, [P, P, P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, P]),
+    "ragrt_enc_gated_ffn_backward": (I32, [P, P, P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, P, I64, P]),
+    "ragrt_enc_gated_ffn_workspace": (I64, [I32, I32, I32]),
 }
 
 _lib = None

@@ -20,6 +20,7 @@ decltype(&ragrt_enc_packed_attention) f_attention = nullptr;
 decltype(&ragrt_enc_qk_norm_rope) f_rope = nullptr;
 decltype(&ragrt_enc_gated_ffn) f_ffn = nullptr;
 decltype(&ragrt_enc_gated_ffn_backward) f_ffn_backward = nullptr;
+decltype(&ragrt_enc_gated_ffn_workspace) f_ffn_workspace = nullptr;
 
 // The current device, where the first tensor of a call lies on it; -1 otherwise.
 int device_of(PyObject* o) {
@@ -59,12 +60,13 @@ PyObject* guarded(F f) {
 }
 
 PyObject* bind(PyObject*, PyObject* args) {
-    unsigned long long a, r, f, b;
-    if (!PyArg_ParseTuple(args, "KKKK", &a, &r, &f, &b)) return nullptr;
+    unsigned long long a, r, f, b, w;
+    if (!PyArg_ParseTuple(args, "KKKKK", &a, &r, &f, &b, &w)) return nullptr;
     f_attention = (decltype(f_attention))a;
     f_rope = (decltype(f_rope))r;
     f_ffn = (decltype(f_ffn))f;
     f_ffn_backward = (decltype(f_ffn_backward))b;
+    f_ffn_workspace = (decltype(f_ffn_workspace))w;
     Py_RETURN_NONE;
 }
 
@@ -189,7 +191,9 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
         for (const at::Tensor* t : {dh, gate, up})
             if (t->scalar_type() != (t == dh ? x->scalar_type() : at::kFloat) || t->dim() != 2 || t->size(0) != M || t->size(1) != F || !solid(*t))
                 Py_RETURN_NONE;
-        at::Tensor dg = like(*x, {M, F}), du = like(*x, {M, F}), rx, rg, ru;
+        at::Tensor dg = like(*x, {M, F}), du = like(*x, {M, F}), rx, rg, ru, ws;
+        const int64_t bytes = dx ? f_ffn_workspace((int32_t)M, (int32_t)F, (int32_t)K) : 0;
+        if (bytes) ws = at::empty({bytes}, dg.options().dtype(at::kByte));
         if (dx) rx = like(*x, {M, K});
         if (dw) {
             rg = like(*x, {F, K});
@@ -198,7 +202,7 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int rc = f_ffn_backward(dh->data_ptr(), x->data_ptr(), g->data_ptr(), u->data_ptr(),
                                       (const float*)gate->data_ptr(), (const float*)up->data_ptr(), dg.data_ptr(), du.data_ptr(), dx ? rx.data_ptr() : nullptr,
                                       dw ? rg.data_ptr() : nullptr, dw ? ru.data_ptr() : nullptr, (int32_t)M, (int32_t)F,
-                                      (int32_t)K, (int32_t)act, dt, stream(dev));
+                                      (int32_t)K, (int32_t)act, dt, bytes ? ws.data_ptr() : nullptr, bytes, stream(dev));
         if (rc) return PyLong_FromLong(rc);
         auto wrap = [](bool has, at::Tensor& t) {
             if (has) return THPVariable_Wrap(std::move(t));

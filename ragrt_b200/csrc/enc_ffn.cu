@@ -64,14 +64,17 @@ struct FfnParams {
     int keep;                  // kForward: g and u are written too
     int dx, dw;                // kBackward: which gradients
     int a_rows;                // ffn_small: rows of x, dg, du that a load brings
+    int split;                 // ffn_small: parts of dx's contraction, each an entry of the list
+    float4* partial;           // their sums, [entry][quad of columns][row], what a warp's stores fill whole
     void* out[3];              // as in FfnMaps
     int* err;
 };
 
 // A tile of one of the products: output `out` (0, or 1 and 2 for the weight gradients), its rows x cols,
-// the tile's first row and column, and the length of the contraction in chunks of kFK (dx: of each half).
+// the tile's first row and column, the length of the contraction in chunks of kFK (dx: of each half), and
+// the chunks [i0, i1) to take (dx: those of du and Wu follow those of dg and Wg).
 struct FfnTile {
-    int out, rows, cols, m0, n0, chunks;
+    int out, rows, cols, m0, n0, chunks, i0, i1;
 };
 
 // Tile t of the list: dx first, the longest contraction, then dWg, dWu.  Within an output eight tile
@@ -82,7 +85,7 @@ struct FfnList {
     __device__ __forceinline__ FfnList(const FfnParams& p) {
         const int cols = kMode == kForward ? p.F : p.K;
         tn = (cols + kTileN - 1) / kTileN;
-        first = kMode == kForward || p.dx ? tn * ((p.M + kTileM - 1) / kTileM) : 0;
+        first = kMode == kForward || p.dx ? tn * ((p.M + kTileM - 1) / kTileM) * p.split : 0;
         per = kMode == kBackward && p.dw ? tn * ((p.F + kTileM - 1) / kTileM) : 0;
         total = first + 2 * per;
     }
@@ -98,6 +101,15 @@ struct FfnList {
         r.rows = dw ? p.F : p.M;
         r.cols = kMode == kForward ? p.F : p.K;
         r.chunks = ((kMode == kForward ? p.K : dw ? p.M : p.F) + kFK - 1) / kFK;
+        const int nk = kMode == kBackward && !dw ? 2 * r.chunks : r.chunks;
+        r.i0 = 0;
+        r.i1 = nk;
+        if (kMode == kBackward && !dw && p.split > 1) {
+            const int part = t % p.split;
+            t /= p.split;
+            r.i0 = (int)((int64_t)nk * part / p.split);
+            r.i1 = (int)((int64_t)nk * (part + 1) / p.split);
+        }
         const int tm = (r.rows + kTileM - 1) / kTileM;
         const int band = t / (8 * tn), in = t % (8 * tn), high = min(8, tm - 8 * band);
         r.m0 = (8 * band + in % high) * kTileM;
@@ -197,10 +209,9 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
             for (int t = pair; t < list.total && !failed; t += pairs) {
                 const FfnTile tile = list.get(p, t);
                 const bool dw = kMode == kBackward && tile.out > 0;
-                const int nk = kMode == kBackward && !dw ? 2 * tile.chunks : tile.chunks;
                 const int m0 = tile.m0 + rank * (kFM / 2);
                 const int n0 = tile.n0 + (kMode == kForward ? 0 : rank * (kFN / 2));
-                for (int i = 0; i < nk; ++i, ++g) {
+                for (int i = tile.i0; i < tile.i1; ++i, ++g) {
                     const int s = g % kFStages;
                     if (g >= kFStages && !tc::mbar_wait_or_abort(empty + s, ((g / kFStages) - 1) & 1, abort, kFWaitLimit)) {
                         failed = true;
@@ -240,7 +251,6 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
             for (int t = pair; t < list.total && !failed; t += pairs, ++j) {
                 const FfnTile tile = list.get(p, t);
                 const bool dw = kMode == kBackward && tile.out > 0;
-                const int nk = kMode == kBackward && !dw ? 2 * tile.chunks : tile.chunks;
                 const uint32_t idesc = tc::idesc_f16_f32(kFM, kFN) | idesc_type<T>() | (dw ? kIdescAMn : 0u) |
                                        (kMode == kBackward ? kIdescBMn : 0u);
                 const uint32_t step = dw ? 2048 : 32;
@@ -250,7 +260,7 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
                 if (failed) break;
                 tc::fence_after();
                 const uint32_t d = tbase + (uint32_t)(b * kFN);
-                for (int i = 0; i < nk; ++i, ++g) {
+                for (int i = tile.i0; i < tile.i1; ++i, ++g) {
                     const int s = g % kFStages;
                     ok = tc::mbar_wait_or_abort(full + s, (g / kFStages) & 1, abort, kFWaitLimit);
                     failed = !__all_sync(0xFFFFFFFFu, ok);
@@ -263,7 +273,7 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
                         tc::mma_ss2_if(lead, d, tc::sw128_mnmajor_desc(a + step * k, 8192),
                                        kMode == kBackward ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192)
                                                           : tc::sw128_kmajor_desc(bb + 32 * k),
-                                       idesc, (i | k) != 0 ? 1u : 0u);
+                                       idesc, i != tile.i0 || k != 0 ? 1u : 0u);
                     tc::mma_commit2_if(lead, empty + s);
                 }
                 if (!failed) tc::mma_commit2_if(lead, accf + b);
@@ -423,8 +433,7 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
             for (int t = blockIdx.x; t < list.total && !failed; t += gridDim.x) {
                 const FfnTile tile = list.get(p, t);
                 const bool dw = kMode == kBackward && tile.out > 0;
-                const int nk = kMode == kBackward && !dw ? 2 * tile.chunks : tile.chunks;
-                for (int i = 0; i < nk; ++i, ++g) {
+                for (int i = tile.i0; i < tile.i1; ++i, ++g) {
                     const int s = g % kSStages;
                     if (g >= kSStages && !tc::mbar_wait_or_abort(empty + s, ((g / kSStages) - 1) & 1, abort, kFWaitLimit)) {
                         failed = true;
@@ -459,7 +468,6 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
         for (int t = blockIdx.x; t < list.total && !failed; t += gridDim.x, ++j) {
             const FfnTile tile = list.get(p, t);
             const bool dw = kMode == kBackward && tile.out > 0;
-            const int nk = kMode == kBackward && !dw ? 2 * tile.chunks : tile.chunks;
             const uint32_t idesc = tc::idesc_f16_f32(kFM / 2, kSN) | idesc_type<T>() | (dw ? kIdescAMn : 0u) |
                                    (kMode == kBackward ? kIdescBMn : 0u);
             const uint32_t step = dw ? 2048 : 32;
@@ -468,7 +476,7 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
             failed = !__all_sync(0xFFFFFFFFu, ok);
             if (failed) break;
             tc::fence_after();
-            for (int i = 0; i < nk; ++i, ++g) {
+            for (int i = tile.i0; i < tile.i1; ++i, ++g) {
                 const int s = g % kSStages;
                 ok = tc::mbar_wait_or_abort(full + s, (g / kSStages) & 1, abort, kFWaitLimit);
                 failed = !__all_sync(0xFFFFFFFFu, ok);
@@ -480,7 +488,7 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
                     tc::mma_ss_if(lead, tbase + (uint32_t)(b * kSN), tc::sw128_mnmajor_desc(a + step * k, 8192),
                                   kMode == kBackward ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192)
                                                      : tc::sw128_kmajor_desc(bb + 32 * k),
-                                  idesc, (i | k) != 0 ? 1u : 0u);
+                                  idesc, i != tile.i0 || k != 0 ? 1u : 0u);
                 tc::mma_commit_if(lead, empty + s);
             }
             if (!failed) tc::mma_commit_if(lead, accf + b);
@@ -509,7 +517,14 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
             tc::fence_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(acce + b);
-            if (row < tile.rows) {
+            if (kMode == kBackward && tile.out == 0 && p.split > 1) {
+                float4* to = p.partial + (int64_t)t * (kSN / 4 * kFM / 2) + quad * 32 + lane;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    to[q * (kFM / 2)] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+                    to[(8 + q) * (kFM / 2)] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                }
+            } else if (row < tile.rows) {
                 const int64_t at = (int64_t)row * tile.cols + tile.n0;
                 auto put = [&](void* base, int off, const float (&x)[32]) {
 #pragma unroll
@@ -546,6 +561,31 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
         tc::fence_after();
         tc::tmem_dealloc(tbase, 2 * kSN);
     }
+}
+
+// dx from the parts' sums, in their order; a thread per 8 values.
+template <typename T>
+__global__ void __launch_bounds__(256) ffn_dx_join(const __grid_constant__ FfnParams p) {
+    pdl_wait_then_release();
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    const int r = i % (kFM / 2), c = i / (kFM / 2) % (kSN / 8) * 8, t = i / (kFM / 2 * kSN / 8);
+    FfnParams whole = p;
+    whole.split = 1;
+    whole.dw = 0;
+    const FfnList<kBackward, kFM / 2, kSN> list(whole);
+    if (t >= list.total) return;
+    const FfnTile tile = list.get(whole, t);
+    const int row = tile.m0 + r, col = tile.n0 + c;
+    if (row >= tile.rows || col >= tile.cols) return;
+    float sum[8] = {};
+    const float4* from = p.partial + (int64_t)t * p.split * (kSN / 4 * kFM / 2) + c / 4 * (kFM / 2) + r;
+#pragma unroll 4
+    for (int s = 0; s < p.split; ++s, from += kSN / 4 * kFM / 2) {
+        const float4 a = __ldcs(from), b = __ldcs(from + kFM / 2);
+        sum[0] += a.x; sum[1] += a.y; sum[2] += a.z; sum[3] += a.w;
+        sum[4] += b.x; sum[5] += b.y; sum[6] += b.z; sum[7] += b.w;
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out[0]) + (int64_t)row * tile.cols + col) = down8<T>(sum);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -692,6 +732,28 @@ int64_t ffn_tiles(int mode, const FfnParams& p, int tile_m, int tile_n) {
     return ((p.dx ? ceil_div(p.M, tile_m) : 0) + (p.dw ? 2 * ceil_div(p.F, tile_m) : 0)) * ceil_div(p.K, tile_n);
 }
 
+// Parts of dx's contraction; 1: whole.  Where dx has fewer tiles than there are SMs, its time is that of the 2F steps
+// of one tile, 0.3 us per chunk; parts of 8 chunks or more share them out (shorter: 60 rows 512 -> 512 in two 10.1 us
+// instead of 8.2), two CTAs per SM from 64 chunks on (2000 rows 256 -> 1024 in two 14.6 us, in four 16.8).
+// With the weight gradients in the same launch of small tiles while these are few; else dx has a launch of its own
+// (apart), if its chain shrinks by 64 chunks (a pair's tiles for all: 1500 rows 768 -> 2048 32 us, apart 40).
+// dx with its elementwise kernel / all gradients, whole -> in parts, us: 25 rows 768 -> 2048 20.5 / 22.0 -> 9.9 / 11.5;
+// 128 rows 2048 -> 5504 50.1 / 68.2 -> 17.4 / 39.2; 300 rows 62.6 / 76.7 -> 31.4 / 56.3; 25 rows 4096 -> 8192
+// 86.2 / 124.3 -> 35.0 / 80.3; 1000 rows 768 -> 2048 24.8 / 29.8 -> 19.8 / 27.8 (cuBLAS's dx: 9.4, 16.5, 18.5, 25.6, 10.7).
+int ffn_split(int M, int F, int K, bool dw, bool& apart) {
+    const int64_t tiles = ceil_div(M, kFM / 2) * ceil_div(K, kSN), sms = num_sms(), nk = 2 * ceil_div(F, kFK);
+    apart = true;
+    if (tiles > sms || nk < 32) return 1;
+    const int64_t most = std::min<int64_t>(8, nk / 8);
+    const int64_t alone = std::min(most, (nk >= 64 ? 2 * sms : sms) / tiles);
+    if (!dw) return (int)alone;
+    if (2 * ceil_div(F, kFM / 2) * ceil_div(K, kSN) * ceil_div(M, kFK) <= 48 * sms) {
+        apart = false;
+        return (int)std::min(alone, std::max<int64_t>(2, sms / tiles));
+    }
+    return nk - nk / alone >= 64 ? (int)alone : 1;
+}
+
 template <typename T, int kMode>
 int ffn_launch(int dtype, FfnParams p, const void* x, const void* wg, const void* wu, const void* dg, const void* du,
                cudaStream_t stream) {
@@ -699,7 +761,8 @@ int ffn_launch(int dtype, FfnParams p, const void* x, const void* wg, const void
     int rc;
     const int64_t sms = num_sms(), pairs = sms / 2;
     const int64_t large = ffn_tiles(kMode, p, kFM, kMode == kForward ? kFN / 2 : kFN);
-    const int64_t small = ffn_tiles(kMode, p, kFM / 2, kMode == kForward ? kSN / 2 : kSN);
+    int64_t small = ffn_tiles(kMode, p, kFM / 2, kMode == kForward ? kSN / 2 : kSN);
+    if (p.dx) small += (p.split - 1) * ceil_div(p.M, kFM / 2) * ceil_div(p.K, kSN);
     bool pair;
     if (kMode == kForward) {
         // small tiles while they are one round of two CTAs per SM: 128 rows 2048 -> 5504 (172 tiles) 12.9 us
@@ -714,7 +777,7 @@ int ffn_launch(int dtype, FfnParams p, const void* x, const void* wg, const void
         const int64_t of_dx = 2 * ceil_div(p.F, kFK), of_dw = ceil_div(p.M, kFK);
         const int64_t n_dx = p.dx ? ceil_div(p.M, kFM) * ceil_div(p.K, kFN) : 0;
         const int64_t sum = n_dx * of_dx + (large - n_dx) * of_dw;
-        pair = 5 * sum >= pairs * std::max(p.dx ? of_dx : 0, p.dw ? of_dw : 0);
+        pair = p.split == 1 && 5 * sum >= pairs * std::max(p.dx ? of_dx : 0, p.dw ? of_dw : 0);
     }
     if (std::max(large, small) > 0x3FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many tiles");
     // few rows: a load brings no more of them than there are (one row of 2048 -> 5504 10.6 us; with
@@ -730,6 +793,29 @@ int ffn_launch(int dtype, FfnParams p, const void* x, const void* wg, const void
     static std::atomic<uint64_t> done{0};
     if ((rc = enc_allow_smem(ffn_small<T, kMode>, kSSmem, done))) return rc;
     return enc_launch(ffn_small<T, kMode>, dim3((unsigned)std::min(small, 2 * sms)), dim3(kSThreads), kSSmem, stream, m, p);
+}
+
+constexpr int64_t kPart = kFM / 2 * kSN * 4;         // bytes of one part's sums
+
+template <typename T>
+int ffn_backward(int dtype, FfnParams p, const void* x, const void* wg, const void* wu, const void* dg, const void* du,
+                 void* ws, int64_t ws_bytes, cudaStream_t stream) {
+    const int64_t tiles = ceil_div(p.M, kFM / 2) * ceil_div(p.K, kSN);
+    bool apart = true;
+    if (p.dx && ws)
+        p.split = (int)std::max<int64_t>(1, std::min<int64_t>(ffn_split(p.M, p.F, p.K, p.dw != 0, apart),
+                                                              ws_bytes / (tiles * kPart)));
+    if (p.split == 1) return ffn_launch<T, kBackward>(dtype, p, x, wg, wu, dg, du, stream);
+    FfnParams d = p;
+    if (apart) d.dw = 0;
+    d.partial = (float4*)ws;
+    int rc = ffn_launch<T, kBackward>(dtype, d, x, wg, wu, dg, du, stream);
+    if (rc) return rc;
+    rc = enc_launch(ffn_dx_join<T>, dim3((unsigned)(tiles * (kFM / 2 * kSN / 8 / 256))), dim3(256), 0, stream, d);
+    if (rc || d.dw == p.dw) return rc;
+    p.dx = 0;
+    p.split = 1;
+    return ffn_launch<T, kBackward>(dtype, p, x, wg, wu, dg, du, stream);
 }
 
 int ffn_check(int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype) {
@@ -760,7 +846,7 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
     cudaStream_t stream = (cudaStream_t)stream_;
-    FfnParams p{M, F, K, act, d_gate != nullptr, 0, 0, 0, {d_h, d_gate, d_up}, err};
+    FfnParams p{M, F, K, act, d_gate != nullptr, 0, 0, 0, 1, nullptr, {d_h, d_gate, d_up}, err};
     // One row at any size: 2048 -> 5504 5.8 us, on the tensor cores 11.0.  Up to four where the weights are few: 4
     // rows 768 -> 2048 4.4 us against 5.2, 2048 -> 4096 9.1 against 10.2; 2048 -> 5504 12.8 against 11.0.
     if (M == 1 || (M <= kFewRows && (int64_t)F * K <= (1 << 23))) {
@@ -775,7 +861,8 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
 extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* d_w_gate,
                                             const void* d_w_up, const float* d_gate, const float* d_up, void* d_dgate,
                                             void* d_dup, void* d_dx, void* d_dw_gate, void* d_dw_up, int32_t M,
-                                            int32_t F, int32_t K, int32_t act, int32_t dtype, void* stream_) {
+                                            int32_t F, int32_t K, int32_t act, int32_t dtype, void* d_ws,
+                                            int64_t ws_bytes, void* stream_) {
     int rc = ffn_check(M, F, K, act, dtype);
     if (rc) return rc;
     cudaStream_t stream = (cudaStream_t)stream_;
@@ -792,7 +879,7 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
     RAGRT_REQUIRE(!d_dw_gate || d_x, "the weight gradients need x");
     RAGRT_REQUIRE((((uintptr_t)d_dh | (uintptr_t)d_x | (uintptr_t)d_w_gate | (uintptr_t)d_w_up | (uintptr_t)d_gate |
                     (uintptr_t)d_up | (uintptr_t)d_dgate | (uintptr_t)d_dup | (uintptr_t)d_dx | (uintptr_t)d_dw_gate |
-                    (uintptr_t)d_dw_up) & 15) == 0,
+                    (uintptr_t)d_dw_up | (uintptr_t)d_ws) & 15) == 0,
                   "gated_ffn_backward operands must be 16-byte aligned");
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
@@ -806,8 +893,15 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
                           d_gate, d_up, (__half*)d_dgate, (__half*)d_dup, n8, (int)act);
     if (rc) return rc;
     if (!d_dx && !d_dw_gate) return RAGRT_OK;
-    FfnParams p{M, F, K, act, 0, d_dx != nullptr, d_dw_gate != nullptr, 0, {d_dx, d_dw_gate, d_dw_up}, err};
+    FfnParams p{M, F, K, act, 0, d_dx != nullptr, d_dw_gate != nullptr, 0, 1, nullptr, {d_dx, d_dw_gate, d_dw_up}, err};
     return dtype == RAGRT_BF16
-               ? ffn_launch<__nv_bfloat16, kBackward>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, stream)
-               : ffn_launch<__half, kBackward>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, stream);
+               ? ffn_backward<__nv_bfloat16>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, d_ws, ws_bytes, stream)
+               : ffn_backward<__half>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, d_ws, ws_bytes, stream);
+}
+
+extern "C" int64_t ragrt_enc_gated_ffn_workspace(int32_t M, int32_t F, int32_t K) {
+    if (M < 1 || F < 8 || K < 8) return 0;
+    bool apart;
+    const int split = ffn_split(M, F, K, false, apart);          // never more with the weight gradients
+    return split == 1 ? 0 : ceil_div(M, kFM / 2) * ceil_div(K, kSN) * split * kPart;
 }

@@ -165,7 +165,7 @@ def _bind():
                                "(python -m ragrt_b200.build)") from e
         _enc_bind.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             L.ragrt_enc_packed_attention, L.ragrt_enc_qk_norm_rope, L.ragrt_enc_gated_ffn,
-            L.ragrt_enc_gated_ffn_backward)))
+            L.ragrt_enc_gated_ffn_backward, L.ragrt_enc_gated_ffn_workspace)))
         _bound = _enc_bind
     return _bound
 
@@ -385,10 +385,12 @@ def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu", need_dx=True, 
     dgate, dup = torch.empty_like(dh), torch.empty_like(dh)
     dx = torch.empty_like(x) if need_dx else None
     dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_dw else (None, None)
+    nbytes = _lib.lib().ragrt_enc_gated_ffn_workspace(M, F, K) if need_dx else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _lib.check(_lib.lib().ragrt_enc_gated_ffn_backward(
         dh.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), gate.data_ptr(), up.data_ptr(), dgate.data_ptr(),
         dup.data_ptr(), dx.data_ptr() if need_dx else None, dwg.data_ptr() if need_dw else None,
-        dwu.data_ptr() if need_dw else None, M, F, K, _ACTS[act], dt, _raw_stream(x)))
+        dwu.data_ptr() if need_dw else None, M, F, K, _ACTS[act], dt, ws.data_ptr(), ws.numel(), _raw_stream(x)))
     return dx, dwg, dwu
 
 

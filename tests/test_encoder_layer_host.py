@@ -62,12 +62,13 @@ def test_gated_ffn_refusals():
                        ((P, None, P, P, None, None, 4, 64, 64, 0, 0, None), b"null"),
                        ((P, P + 2, P, P, None, None, 4, 64, 64, 0, 0, None), b"aligned")]:
         assert f(*args) == -1 and what in last(), what
-    for args, what in [((P,) * 11 + (4, 60, 64, 0, 0, None), b"multiples of 8"),
-                       ((P,) * 10 + (None, 4, 64, 64, 0, 0, None), b"together"),
-                       ((None,) + (P,) * 10 + (4, 64, 64, 0, 0, None), b"null"),
-                       ((P, None) + (P,) * 9 + (4, 64, 64, 0, 0, None), b"need x"),
-                       ((P, P, None) + (P,) * 8 + (4, 64, 64, 0, 0, None), b"needs the weights"),
-                       ((P + 8,) + (P,) * 10 + (4, 64, 64, 0, 0, None), b"aligned")]:
+    for args, what in [((P,) * 11 + (4, 60, 64, 0, 0, None, 0, None), b"multiples of 8"),
+                       ((P,) * 10 + (None, 4, 64, 64, 0, 0, None, 0, None), b"together"),
+                       ((None,) + (P,) * 10 + (4, 64, 64, 0, 0, None, 0, None), b"null"),
+                       ((P, None) + (P,) * 9 + (4, 64, 64, 0, 0, None, 0, None), b"need x"),
+                       ((P, P, None) + (P,) * 8 + (4, 64, 64, 0, 0, None, 0, None), b"needs the weights"),
+                       ((P + 8,) + (P,) * 10 + (4, 64, 64, 0, 0, None, 0, None), b"aligned"),
+                       ((P,) * 11 + (4, 64, 64, 0, 0, P + 4, 64, None), b"aligned")]:
         assert b(*args) == -1 and what in last(), what
 
 

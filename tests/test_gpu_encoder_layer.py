@@ -343,7 +343,8 @@ def ffn_inputs(M, F, K, dtype, seed):
 
 
 SHAPES = [(1, 128, 64), (1, 2056, 768), (3, 8, 8), (17, 264, 72), (128, 128, 128), (129, 136, 776), (200, 1160, 768),
-          (300, 64, 1000), (1000, 520, 264), (8, 1024, 2048), (9, 1000, 520), (64, 776, 512)]
+          (300, 64, 1000), (1000, 520, 264), (8, 1024, 2048), (9, 1000, 520), (64, 776, 512), (2500, 328, 520),
+          (130, 1400, 136), (270, 18312, 264)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -414,6 +415,30 @@ def test_gated_ffn_gradients_against_differences(act):
         room = ((bounds[i] + moved[i]) * d.abs()).sum().item()
         size = (grads[i].double() * d).abs().sum().item()
         assert abs(got - want) <= room + 1e-6 * size
+
+
+def test_gated_ffn_backward_with_less_scratch_or_none():
+    """dx's contraction in as many parts as the scratch allows: one, two, all; never differently twice."""
+    M, F, K = 70, 1096, 136
+    x, wg, wu, dh = ffn_inputs(M, F, K, torch.float16, 21)
+    _, gate, up = encoder.gated_ffn(x, wg, wu, keep=True)
+    want, bound = L.ffn_backward64(dh, x, wg, wu, gate, up, "silu")[0]
+    lib = _lib.lib()
+    full = lib.ragrt_enc_gated_ffn_workspace(M, F, K)
+    assert 0 < full <= torch.cuda.get_device_properties(0).multi_processor_count * 128 * 128 * 4
+    tmp = torch.empty_like(dh), torch.empty_like(dh)
+    for nbytes in (0, 1000, 3 * 128 * 64 * 4, 2 * 3 * 128 * 64 * 4, full):
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")
+        got = []
+        for _ in range(2):
+            dx = torch.full_like(x, 9.0)
+            _lib.check(lib.ragrt_enc_gated_ffn_backward(
+                dh.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), gate.data_ptr(), up.data_ptr(),
+                tmp[0].data_ptr(), tmp[1].data_ptr(), dx.data_ptr(), None, None, M, F, K, 0, 0,
+                ws.data_ptr() if nbytes else None, nbytes, torch.cuda.current_stream().cuda_stream))
+            got.append(dx)
+        L.check(got[0], want, bound)
+        assert torch.equal(got[0], got[1])
 
 
 def test_gated_ffn_partial_gradients_and_no_rows():
