@@ -342,6 +342,20 @@ def ffn_inputs(M, F, K, dtype, seed):
     return x, w[:F], w[F:], dh
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 72, 128])
+@pytest.mark.parametrize("others", [[], [700, 1], [3000]])
+def test_attention_of_a_single_key_is_its_value(others, dim, dtype):
+    """Whatever the score: rows that see one key, alone in a sequence or first of a causal one."""
+    lens = [1, 1, 5, 1] + others + [1]
+    cu = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    q, k, v = [torch.randn(cu[-1], h, dim, generator=g, device="cuda").to(dtype) for h in (6, 2, 2)]
+    out = encoder.packed_attention(q, k, v, torch.tensor(cu, dtype=torch.int32, device="cuda"), causal=True)
+    first = [a for a, n in zip(cu, lens) if n]
+    assert torch.equal(out[first], v[first].repeat_interleave(3, 1))
+
+
 SHAPES = [(1, 128, 64), (1, 2056, 768), (3, 8, 8), (17, 264, 72), (128, 128, 128), (129, 136, 776), (200, 1160, 768),
           (300, 64, 1000), (1000, 520, 264), (8, 1024, 2048), (9, 1000, 520), (64, 776, 512), (2500, 328, 520),
           (130, 1400, 136), (270, 18312, 264)]
