@@ -418,7 +418,8 @@ int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const void* d_w_u
  * d_dx [M, K] (may be NULL), d_dw_gate and d_dw_up [F, K] (may both be NULL).  Overwrites, does
  * not add to, its outputs; the order of every sum is fixed.  M = 0 gives zero weight gradients.
  * d_ws (ws_bytes, may be NULL / 0): scratch for small M, where dx's contraction is split over more CTAs
- * and joined in fp32 (ragrt_enc_gated_ffn_workspace bytes; fewer parts when there are fewer).
+ * and joined in fp32 (ragrt_enc_gated_ffn_workspace bytes; fewer parts when there are fewer).  Calls that
+ * may overlap on the GPU, on two streams or in two graphs, need a scratch each, as they need outputs of their own.
  */
 int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* d_w_gate, const void* d_w_up,
                                  const float* d_gate, const float* d_up, void* d_dgate, void* d_dup, void* d_dx,

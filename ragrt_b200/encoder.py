@@ -233,16 +233,17 @@ def _overlap(a, b):
 
 
 def _check_output(out, shape, dtype, inputs, in_place_of=None):
-    """`out` has the shape and type, can be written in place and is apart from the inputs."""
+    """`out` has the shape and type, can be written in place and is apart from the inputs; it may be
+    `in_place_of` itself."""
     if out.shape != shape or out.dtype != dtype:
         raise RuntimeError(f"out must be {tuple(shape)} {dtype}; got {tuple(out.shape)} {out.dtype}")
     if not (_row_stride(out) if out.dim() == 3 else out.is_contiguous() and not out.data_ptr() & 15):
         raise RuntimeError("out must be written in place: solid rows, 16-byte aligned, strides in multiples of 8")
     for t in inputs:
-        if not _overlap(out, t):
-            continue
-        if t is in_place_of and out.data_ptr() == t.data_ptr() and _row_stride(out) == _row_stride(t):
-            continue
+        if _overlap(out, t):
+            raise RuntimeError("out overlaps an input")
+    t = in_place_of
+    if t is not None and _overlap(out, t) and (out.data_ptr() != t.data_ptr() or _row_stride(out) != _row_stride(t)):
         raise RuntimeError("out overlaps an input")
 
 
@@ -288,7 +289,8 @@ def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     cos / sin [max_pos, R / 2] f32 at positions [T] (int32 or int64) of each head's first R values:
     pairs (i, i + R / 2), or neighbours with `interleaved`.  q [T, H, D], k [T, KV, D] fp16 or bf16 ->
     (q_out, k_out), which may be q and k themselves.  D a multiple of 8 in [16, 256], R a multiple
-    of 16.  A position outside the table reads its row 0 and raises the device error flag (5)."""
+    of 16.  A position outside the table reads its row 0 and raises the device error flag (5).  Not
+    differentiable."""
     if q_out is None and k_out is None:
         r = (_bound or _bind()).qk_norm_rope(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
         if r is not None:
@@ -312,12 +314,12 @@ def qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e
     if q_out is None:
         q_out, qos = torch.empty_like(q, memory_format=torch.contiguous_format), H * D
     else:
-        _check_output(q_out, shape, q.dtype, (q, k), in_place_of=q)
+        _check_output(q_out, shape, q.dtype, (k,), in_place_of=q)
         qos = _row_stride(q_out)
     if k_out is None:
         k_out, kos = torch.empty_like(k, memory_format=torch.contiguous_format), KV * D
     else:
-        _check_output(k_out, kshape, k.dtype, (q, k, q_out), in_place_of=k)
+        _check_output(k_out, kshape, k.dtype, (q, q_out), in_place_of=k)
         kos = _row_stride(k_out)
     rc = _lib.lib().ragrt_enc_qk_norm_rope(
         q.data_ptr(), k.data_ptr(), qw if qw is None else qw.data_ptr(), kw if kw is None else kw.data_ptr(),

@@ -135,6 +135,15 @@ def test_overlap_of_column_blocks_and_shifted_rows(on_host):
         encoder.qk_norm_rope(block(0, 0, 256), block(0, 256, 128), cos, cos, pos, k_out=block(0, 128, 128))
 
 
+def test_one_tensor_as_query_and_key_in_place(on_host):
+    """Neither may be written over the other, nor the two outputs over one another."""
+    q, other = torch.zeros(8, 4, 64, dtype=H16), torch.zeros(8, 4, 64, dtype=H16)
+    cos, pos = torch.zeros(4, 32), torch.zeros(8, dtype=torch.int64)
+    for outs in (dict(q_out=q), dict(k_out=q), dict(q_out=q, k_out=q), dict(q_out=other, k_out=other)):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            encoder.qk_norm_rope(q, q, cos, cos, pos, **outs)
+
+
 def test_python_checks_of_norm_rope(on_host):
     q, k = torch.zeros(8, 4, 64, dtype=H16), torch.zeros(8, 2, 64, dtype=H16)
     cos = torch.zeros(16, 32)
