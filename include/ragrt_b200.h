@@ -426,7 +426,7 @@ int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* 
                                  void* d_dw_gate, void* d_dw_up, int32_t M, int32_t F, int32_t K, int32_t act,
                                  int32_t dtype, void* d_ws, int64_t ws_bytes, void* stream);
 
-/* Bytes of scratch that ragrt_enc_gated_ffn_backward can use for these sizes (0: none; 9.7 MB at most). */
+/* Bytes of scratch that ragrt_enc_gated_ffn_backward can use for these sizes (0: none; 19.4 MB at most). */
 int64_t ragrt_enc_gated_ffn_workspace(int32_t M, int32_t F, int32_t K);
 
 /* Library version string. */

@@ -376,19 +376,24 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
     }
 }
 
-// ------------------------------------------------------------------ 128 x 64 tiles
-constexpr int kSN = 64;                        // accumulator columns
+// ------------------------------------------------------------------ 128-row tiles of one CTA, two to an SM
 constexpr int kSTileA = kFM / 2 * kFK * 2;
-constexpr int kSTileB = kSN * kFK * 2;
-constexpr int kSStages = 4;
-constexpr int kSSmem = 1024 + kSStages * (kSTileA + kSTileB) + 256;
+template <int kMode, int kN_>
+struct SmallCfg {
+    static constexpr int kN = kN_;                               // accumulator columns
+    static constexpr int kOutCols = kMode == kForward ? kN / 2 : kN;
+    static constexpr int kTileB = kN * kFK * 2;
+    static constexpr int kStages = kN == 64 ? 4 : 3;
+    static constexpr int kSmem = 1024 + kStages * (kSTileA + kTileB) + 256;
+};
 constexpr int kFewRows = 4;                    // rows that ffn_rows takes at most
 constexpr int kSThreads = 192;                 // TMA warp, MMA warp, 4 epilogue warps
 
-template <typename T, int kMode>
+template <typename T, int kMode, int kN>
 __global__ void __launch_bounds__(kSThreads, 2)
 ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams p) {
-    constexpr int kOutCols = kMode == kForward ? kSN / 2 : kSN;
+    typedef SmallCfg<kMode, kN> Cfg;
+    constexpr int kOutCols = Cfg::kOutCols, kSStages = Cfg::kStages, kSTileB = Cfg::kTileB;
     extern __shared__ uint8_t ffn_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)ffn_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sA = sm;
@@ -417,7 +422,7 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
         tc::mbar_fence_init();
     }
     if (warp == 1) {
-        tc::tmem_alloc(tslot, 2 * kSN);
+        tc::tmem_alloc(tslot, 2 * kN);
         tc::tmem_relinquish();
     }
     tc::fence_before();
@@ -454,7 +459,8 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
                         tc::tma_load_2d(db, &maps.b[0], k, tile.n0, full + s);
                         tc::tma_load_2d(db + kSTileB / 2, &maps.b[1], k, tile.n0, full + s);
                     } else {
-                        tc::tma_load_2d(db, &maps.b[dw ? 2 : (int)second], tile.n0, k, full + s);
+                        for (int c = 0; c < kN / 64; ++c)
+                            tc::tma_load_2d(db + 8192 * c, &maps.b[dw ? 2 : (int)second], tile.n0 + 64 * c, k, full + s);
                     }
                 }
             }
@@ -468,7 +474,7 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
         for (int t = blockIdx.x; t < list.total && !failed; t += gridDim.x, ++j) {
             const FfnTile tile = list.get(p, t);
             const bool dw = kMode == kBackward && tile.out > 0;
-            const uint32_t idesc = tc::idesc_f16_f32(kFM / 2, kSN) | idesc_type<T>() | (dw ? kIdescAMn : 0u) |
+            const uint32_t idesc = tc::idesc_f16_f32(kFM / 2, kN) | idesc_type<T>() | (dw ? kIdescAMn : 0u) |
                                    (kMode == kBackward ? kIdescBMn : 0u);
             const uint32_t step = dw ? 2048 : 32;
             const int b = j & 1;
@@ -485,7 +491,7 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
                 const uint32_t a = tc::smem_u32(sA + s * kSTileA), bb = tc::smem_u32(sB + s * kSTileB);
 #pragma unroll
                 for (int k = 0; k < kFK / 16; ++k)
-                    tc::mma_ss_if(lead, tbase + (uint32_t)(b * kSN), tc::sw128_mnmajor_desc(a + step * k, 8192),
+                    tc::mma_ss_if(lead, tbase + (uint32_t)(b * kN), tc::sw128_mnmajor_desc(a + step * k, 8192),
                                   kMode == kBackward ? tc::sw128_mnmajor_desc(bb + 2048 * k, 8192)
                                                      : tc::sw128_kmajor_desc(bb + 32 * k),
                                   idesc, i != tile.i0 || k != 0 ? 1u : 0u);
@@ -509,47 +515,61 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
                 break;
             }
             tc::fence_after();
-            const uint32_t taddr = tbase + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kSN);
-            float f[32], v[32];
-            tc::ld32x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(f));
-            tc::ld32x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(v));
-            tc::wait_ld();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(acce + b);
-            if (kMode == kBackward && tile.out == 0 && p.split > 1) {
-                float4* to = p.partial + (int64_t)t * (kSN / 4 * kFM / 2) + quad * 32 + lane;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    to[q * (kFM / 2)] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
-                    to[(8 + q) * (kFM / 2)] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            const uint32_t taddr = tbase + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kN);
+#pragma unroll 1
+            for (int c0 = 0; c0 < kN; c0 += 64) {
+                float f[32], v[32];
+                tc::ld32x32(taddr + c0, *reinterpret_cast<uint32_t(*)[32]>(f));
+                tc::ld32x32(taddr + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(v));
+                tc::wait_ld();
+                if (c0 + 64 == kN) {
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(acce + b);
                 }
-            } else if (row < tile.rows) {
-                const int64_t at = (int64_t)row * tile.cols + tile.n0;
-                auto put = [&](void* base, int off, const float (&x)[32]) {
+                if (kMode == kBackward && tile.out == 0 && p.split > 1) {
+                    float4* to = p.partial + ((int64_t)t * (kN / 4) + c0 / 4) * (kFM / 2) + quad * 32 + lane;
 #pragma unroll
-                    for (int q = 0; q < 32; q += 8)
-                        if (tile.n0 + off + q < tile.cols)       // cols is a multiple of 8
-                            *reinterpret_cast<uint4*>(static_cast<T*>(base) + at + off + q) =
-                                down8<T>(*reinterpret_cast<const float(*)[8]>(x + q));
-                };
-                auto keep = [&](void* base, const float (&x)[32]) {
-#pragma unroll
-                    for (int q = 0; q < 32; q += 4)
-                        if (tile.n0 + q < tile.cols)
-                            *reinterpret_cast<float4*>(static_cast<float*>(base) + at + q) =
-                                make_float4(x[q], x[q + 1], x[q + 2], x[q + 3]);
-                };
-                if (kMode == kForward) {
-                    if (p.keep) {
-                        keep(p.out[1], f);
-                        keep(p.out[2], v);
+                    for (int q = 0; q < 8; ++q) {
+                        to[q * (kFM / 2)] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+                        to[(8 + q) * (kFM / 2)] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
                     }
-                    ffn_gate(f, v, p.act);
-                    put(p.out[0], 0, f);
-                } else {
-                    put(p.out[tile.out], 0, f);
-                    put(p.out[tile.out], 32, v);
+                } else if (row < tile.rows) {
+                    const int64_t at = (int64_t)row * tile.cols + tile.n0;
+                    auto put = [&](void* base, int off, const float (&x)[32]) {
+                        T* dst = static_cast<T*>(base) + at + off;
+                        if (tile.cols % 16 == 0 && ((uintptr_t)base & 31) == 0) {       // whole sectors
+#pragma unroll
+                            for (int q = 0; q < 32; q += 16)
+                                if (tile.n0 + off + q < tile.cols)
+                                    store32(dst + q, down8<T>(*reinterpret_cast<const float(*)[8]>(x + q)),
+                                            down8<T>(*reinterpret_cast<const float(*)[8]>(x + q + 8)));
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 32; q += 8)
+                                if (tile.n0 + off + q < tile.cols)       // cols is a multiple of 8
+                                    *reinterpret_cast<uint4*>(dst + q) =
+                                        down8<T>(*reinterpret_cast<const float(*)[8]>(x + q));
+                        }
+                    };
+                    auto keep = [&](void* base, const float (&x)[32]) {
+#pragma unroll
+                        for (int q = 0; q < 32; q += 4)
+                            if (tile.n0 + q < tile.cols)
+                                *reinterpret_cast<float4*>(static_cast<float*>(base) + at + q) =
+                                    make_float4(x[q], x[q + 1], x[q + 2], x[q + 3]);
+                    };
+                    if (kMode == kForward) {
+                        if (p.keep) {
+                            keep(p.out[1], f);
+                            keep(p.out[2], v);
+                        }
+                        ffn_gate(f, v, p.act);
+                        put(p.out[0], 0, f);
+                    } else {
+                        put(p.out[tile.out], c0, f);
+                        put(p.out[tile.out], c0 + 32, v);
+                    }
                 }
             }
         }
@@ -559,28 +579,28 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
     __syncthreads();
     if (warp == 1) {
         tc::fence_after();
-        tc::tmem_dealloc(tbase, 2 * kSN);
+        tc::tmem_dealloc(tbase, 2 * kN);
     }
 }
 
 // dx from the parts' sums, in their order; a thread per 8 values.
-template <typename T>
+template <typename T, int kN>
 __global__ void __launch_bounds__(256) ffn_dx_join(const __grid_constant__ FfnParams p) {
     pdl_wait_then_release();
     const int i = blockIdx.x * 256 + threadIdx.x;
-    const int r = i % (kFM / 2), c = i / (kFM / 2) % (kSN / 8) * 8, t = i / (kFM / 2 * kSN / 8);
+    const int r = i % (kFM / 2), c = i / (kFM / 2) % (kN / 8) * 8, t = i / (kFM / 2 * kN / 8);
     FfnParams whole = p;
     whole.split = 1;
     whole.dw = 0;
-    const FfnList<kBackward, kFM / 2, kSN> list(whole);
+    const FfnList<kBackward, kFM / 2, kN> list(whole);
     if (t >= list.total) return;
     const FfnTile tile = list.get(whole, t);
     const int row = tile.m0 + r, col = tile.n0 + c;
     if (row >= tile.rows || col >= tile.cols) return;
     float sum[8] = {};
-    const float4* from = p.partial + (int64_t)t * p.split * (kSN / 4 * kFM / 2) + c / 4 * (kFM / 2) + r;
+    const float4* from = p.partial + (int64_t)t * p.split * (kN / 4 * kFM / 2) + c / 4 * (kFM / 2) + r;
 #pragma unroll 4
-    for (int s = 0; s < p.split; ++s, from += kSN / 4 * kFM / 2) {
+    for (int s = 0; s < p.split; ++s, from += kN / 4 * kFM / 2) {
         const float4 a = __ldcs(from), b = __ldcs(from + kFM / 2);
         sum[0] += a.x; sum[1] += a.y; sum[2] += a.z; sum[3] += a.w;
         sum[4] += b.x; sum[5] += b.y; sum[6] += b.z; sum[7] += b.w;
@@ -701,7 +721,7 @@ int ffn_maps(FfnMaps& m, int mode, bool pair, int dtype, const FfnParams& p, con
              const void* dg, const void* du) {
     int rc;
     if (mode == kForward) {
-        const int wrows = pair ? kFN / 2 : kSN / 2;
+        const int wrows = pair ? kFN / 2 : SmallCfg<kForward, 64>::kOutCols;
         if ((rc = enc_map_2d(&m.a[0], dtype, x, p.M, p.K, p.K, pair ? kFM / 2 : p.a_rows)) ||
             (rc = enc_map_2d(&m.b[0], dtype, wg, p.F, p.K, p.K, wrows)) ||
             (rc = enc_map_2d(&m.b[1], dtype, wu, p.F, p.K, p.K, wrows)))
@@ -732,37 +752,90 @@ int64_t ffn_tiles(int mode, const FfnParams& p, int tile_m, int tile_n) {
     return ((p.dx ? ceil_div(p.M, tile_m) : 0) + (p.dw ? 2 * ceil_div(p.F, tile_m) : 0)) * ceil_div(p.K, tile_n);
 }
 
-// Parts of dx's contraction; 1: whole.  Where dx has fewer tiles than there are SMs, its time is that of the 2F steps
-// of one tile, 0.3 us per chunk; parts of 8 chunks or more share them out (shorter: 60 rows 512 -> 512 in two 10.1 us
-// instead of 8.2), two CTAs per SM from 64 chunks on (2000 rows 256 -> 1024 in two 14.6 us, in four 16.8).
-// With the weight gradients in the same launch of small tiles while these are few; else dx has a launch of its own
-// (apart), if its chain shrinks by 64 chunks (a pair's tiles for all: 1500 rows 768 -> 2048 32 us, apart 40).
-// dx with its elementwise kernel / all gradients, whole -> in parts, us: 25 rows 768 -> 2048 20.5 / 22.0 -> 9.9 / 11.5;
-// 128 rows 2048 -> 5504 50.1 / 68.2 -> 17.4 / 39.2; 300 rows 62.6 / 76.7 -> 31.4 / 56.3; 25 rows 4096 -> 8192
-// 86.2 / 124.3 -> 35.0 / 80.3; 1000 rows 768 -> 2048 24.8 / 29.8 -> 19.8 / 27.8 (cuBLAS's dx: 9.4, 16.5, 18.5, 25.6, 10.7).
-int ffn_split(int M, int F, int K, bool dw, bool& apart) {
-    const int64_t tiles = ceil_div(M, kFM / 2) * ceil_div(K, kSN), sms = num_sms(), nk = 2 * ceil_div(F, kFK);
-    apart = true;
-    if (tiles > sms || nk < 32) return 1;
-    const int64_t most = std::min<int64_t>(8, nk / 8);
-    const int64_t alone = std::min(most, (nk >= 64 ? 2 * sms : sms) / tiles);
-    if (!dw) return (int)alone;
-    if (2 * ceil_div(F, kFM / 2) * ceil_div(K, kSN) * ceil_div(M, kFK) <= 48 * sms) {
-        apart = false;
-        return (int)std::min(alone, std::max<int64_t>(2, sms / tiles));
+// How the gradients run on 128-row tiles: their width, the parts that dx's contraction is cut into (1: whole), and
+// whether dx has a launch of its own (apart).
+struct FfnPlan {
+    int width, split;
+    bool apart;
+};
+
+int64_t ffn_dx_tiles(int M, int K, int width) { return ceil_div(M, kFM / 2) * ceil_div(K, width); }
+int64_t ffn_part_bytes(int width) { return (int64_t)(kFM / 2) * width * 4; }
+
+// The parts of least time, as the longest share of a CTA in chunks of the contraction: dx's parts and then `per` tiles
+// of of_dw chunks, dealt out to two CTAs per SM in turn.  A tile of the weight gradients takes 16 chunks at least, its
+// epilogue; a part 4 more; every entry of the list costs the SM 2; the joining kernel 8 and one per 64 parts.  Parts of
+// 8 chunks or more, at most two per SM in all (and 16 of a tile).  Against all counts, measured for 20 shapes from 25 x
+// 768 -> 2048 to 256 x 4096 -> 8192: within 5 % of the best for dx, 13 % for all gradients.
+int ffn_parts(int64_t tiles, int64_t nk, int64_t per, int64_t of_dw) {
+    const int64_t ctas = 2 * num_sms();
+    int best = 1;
+    int64_t least = 0;
+    for (int64_t s = 1; s <= 16 && (s == 1 || (s <= nk / 8 && s * tiles <= ctas)); ++s) {
+        auto share = [&](int64_t c) {
+            const int64_t n = ceil_div(std::max<int64_t>(tiles * s + per - c, 0), ctas);
+            const int64_t dx = ceil_div(std::max<int64_t>(tiles * s - c, 0), ctas);
+            return dx * (ceil_div(nk, s) + 4) + (n - dx) * std::max<int64_t>(of_dw, 16);
+        };
+        const int64_t time = std::max(share(0), share(tiles * s % ctas)) + (s > 1 ? 8 + tiles * s / 64 : 0) +
+                             2 * (tiles * s + per) / num_sms();
+        if (s == 1 || time < least) {
+            best = (int)s;
+            least = time;
+        }
     }
-    return nk - nk / alone >= 64 ? (int)alone : 1;
+    return best;
+}
+
+// dx is cut where it has fewer tiles than there are SMs: its time is that of the 2 F steps of one tile then, 0.3 us
+// a chunk.  Not under 32 chunks (60 rows 512 -> 512 in two parts 10.1 us, whole 8.2).  The weight gradients join its
+// launch while they are 27 chunks per SM or fewer; else dx runs apart if its chain shrinks by 64 chunks, or is left
+// whole (1500 rows 768 -> 2048: large tiles for all 32 us, dx apart 36).  With their elementwise kernel, whole and in
+// parts, dx / all gradients: 25 rows 768 -> 2048 20.8 / 22.0 and 9.9 / 11.5 us, 128 rows 2048 -> 5504 50 / 68 and 16.5 /
+// 32, 300 rows 63 / 77 and 30 / 54, 25 rows 4096 -> 8192 86 / 124 and 34 / 76, 1000 rows 768 -> 2048 24 / 30 and 20 / 24
+// (cuBLAS's dx: 9.3, 17, 18.5, 26, 10.7).
+// Tiles of 64 columns where those are one round of CTAs and 64 chunks per SM; else of 128, whose products take no
+// longer (100 cycles: the 128-row operand comes from shared memory at that rate): all gradients of 1000 rows 768 ->
+// 2048 by 64 27.8 us, by 128 24.4; 128 rows 2048 -> 5504 39.2 and 32.0; 1200 rows 384 -> 1536 17.4 and 18.9; dx alone
+// of 25 rows 768 -> 2048 9.9 and 10.4, of 256 rows 4096 -> 8192 60 and 52.
+FfnPlan ffn_plan(int M, int F, int K, bool dx, bool dw) {
+    const int64_t sms = num_sms(), nk = 2 * ceil_div(F, kFK), of_dw = ceil_div(M, kFK);
+    FfnPlan plan{64, 1, false};
+    for (const int width : {64, 128}) {
+        const int64_t tiles = dx ? ffn_dx_tiles(M, K, width) : 0;
+        const int64_t per = dw ? 2 * ceil_div(F, kFM / 2) * ceil_div(K, width) : 0;
+        plan = FfnPlan{width, 1, false};
+        if (tiles > 0 && tiles <= sms && nk >= 32) {
+            plan.apart = dw && per * of_dw * width / 128 > 27 * sms;
+            plan.split = ffn_parts(tiles, nk, plan.apart ? 0 : per, of_dw);
+            if (plan.apart && nk - nk / plan.split < 64) plan.split = 1;
+        }
+        if (plan.split == 1) plan.apart = false;
+        const int64_t rest = plan.apart ? 0 : per;
+        if (tiles * plan.split + rest <= 2 * sms && tiles * nk + rest * of_dw <= 64 * sms) break;
+    }
+    return plan;
+}
+
+template <typename T, int kMode, int kN>
+int ffn_launch_small(const FfnMaps& m, const FfnParams& p, int64_t entries, cudaStream_t stream) {
+    typedef SmallCfg<kMode, kN> Cfg;
+    static std::atomic<uint64_t> done{0};
+    const int rc = enc_allow_smem(ffn_small<T, kMode, kN>, Cfg::kSmem, done);
+    if (rc) return rc;
+    return enc_launch(ffn_small<T, kMode, kN>, dim3((unsigned)std::min<int64_t>(entries, 2 * num_sms())),
+                      dim3(kSThreads), Cfg::kSmem, stream, m, p);
 }
 
 template <typename T, int kMode>
-int ffn_launch(int dtype, FfnParams p, const void* x, const void* wg, const void* wu, const void* dg, const void* du,
-               cudaStream_t stream) {
+int ffn_launch(int dtype, FfnParams p, int width, const void* x, const void* wg, const void* wu, const void* dg,
+               const void* du, cudaStream_t stream) {
     FfnMaps m = {};
     int rc;
     const int64_t sms = num_sms(), pairs = sms / 2;
     const int64_t large = ffn_tiles(kMode, p, kFM, kMode == kForward ? kFN / 2 : kFN);
-    int64_t small = ffn_tiles(kMode, p, kFM / 2, kMode == kForward ? kSN / 2 : kSN);
-    if (p.dx) small += (p.split - 1) * ceil_div(p.M, kFM / 2) * ceil_div(p.K, kSN);
+    int64_t small = ffn_tiles(kMode, p, kFM / 2, kMode == kForward ? width / 2 : width);
+    if (p.dx) small += (p.split - 1) * ffn_dx_tiles(p.M, p.K, width);
     bool pair;
     if (kMode == kForward) {
         // small tiles while they are one round of two CTAs per SM: 128 rows 2048 -> 5504 (172 tiles) 12.9 us
@@ -790,32 +863,31 @@ int ffn_launch(int dtype, FfnParams p, const void* x, const void* wg, const void
         return enc_launch(ffn_pair<T, kMode>, dim3((unsigned)(2 * std::min(large, pairs))), dim3(kFThreads), kFSmem,
                           stream, m, p);
     }
-    static std::atomic<uint64_t> done{0};
-    if ((rc = enc_allow_smem(ffn_small<T, kMode>, kSSmem, done))) return rc;
-    return enc_launch(ffn_small<T, kMode>, dim3((unsigned)std::min(small, 2 * sms)), dim3(kSThreads), kSSmem, stream, m, p);
+    if constexpr (kMode == kBackward)
+        if (width == 128) return ffn_launch_small<T, kMode, 128>(m, p, small, stream);
+    return ffn_launch_small<T, kMode, 64>(m, p, small, stream);
 }
-
-constexpr int64_t kPart = kFM / 2 * kSN * 4;         // bytes of one part's sums
 
 template <typename T>
 int ffn_backward(int dtype, FfnParams p, const void* x, const void* wg, const void* wu, const void* dg, const void* du,
                  void* ws, int64_t ws_bytes, cudaStream_t stream) {
-    const int64_t tiles = ceil_div(p.M, kFM / 2) * ceil_div(p.K, kSN);
-    bool apart = true;
-    if (p.dx && ws)
-        p.split = (int)std::max<int64_t>(1, std::min<int64_t>(ffn_split(p.M, p.F, p.K, p.dw != 0, apart),
-                                                              ws_bytes / (tiles * kPart)));
-    if (p.split == 1) return ffn_launch<T, kBackward>(dtype, p, x, wg, wu, dg, du, stream);
+    const FfnPlan plan = ffn_plan(p.M, p.F, p.K, p.dx != 0, p.dw != 0);
+    const int64_t tiles = ffn_dx_tiles(p.M, p.K, plan.width);
+    const int64_t room = ws ? ws_bytes / (tiles * ffn_part_bytes(plan.width)) : 0;
+    p.split = (int)std::max<int64_t>(1, std::min<int64_t>(plan.split, room));
+    if (p.split == 1) return ffn_launch<T, kBackward>(dtype, p, plan.width, x, wg, wu, dg, du, stream);
     FfnParams d = p;
-    if (apart) d.dw = 0;
+    if (plan.apart) d.dw = 0;
     d.partial = (float4*)ws;
-    int rc = ffn_launch<T, kBackward>(dtype, d, x, wg, wu, dg, du, stream);
+    int rc = ffn_launch<T, kBackward>(dtype, d, plan.width, x, wg, wu, dg, du, stream);
     if (rc) return rc;
-    rc = enc_launch(ffn_dx_join<T>, dim3((unsigned)(tiles * (kFM / 2 * kSN / 8 / 256))), dim3(256), 0, stream, d);
+    const dim3 blocks((unsigned)(tiles * (kFM / 2) * plan.width / 8 / 256));
+    rc = plan.width == 64 ? enc_launch(ffn_dx_join<T, 64>, blocks, dim3(256), 0, stream, d)
+                          : enc_launch(ffn_dx_join<T, 128>, blocks, dim3(256), 0, stream, d);
     if (rc || d.dw == p.dw) return rc;
     p.dx = 0;
     p.split = 1;
-    return ffn_launch<T, kBackward>(dtype, p, x, wg, wu, dg, du, stream);
+    return ffn_launch<T, kBackward>(dtype, p, plan.width, x, wg, wu, dg, du, stream);
 }
 
 int ffn_check(int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype) {
@@ -854,8 +926,8 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
                                    : ffn_rows_launch<__half>(d_x, d_w_gate, d_w_up, p, stream);
     }
     return dtype == RAGRT_BF16
-               ? ffn_launch<__nv_bfloat16, kForward>(dtype, p, d_x, d_w_gate, d_w_up, nullptr, nullptr, stream)
-               : ffn_launch<__half, kForward>(dtype, p, d_x, d_w_gate, d_w_up, nullptr, nullptr, stream);
+               ? ffn_launch<__nv_bfloat16, kForward>(dtype, p, 64, d_x, d_w_gate, d_w_up, nullptr, nullptr, stream)
+               : ffn_launch<__half, kForward>(dtype, p, 64, d_x, d_w_gate, d_w_up, nullptr, nullptr, stream);
 }
 
 extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* d_w_gate,
@@ -901,7 +973,11 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
 
 extern "C" int64_t ragrt_enc_gated_ffn_workspace(int32_t M, int32_t F, int32_t K) {
     if (M < 1 || F < 8 || K < 8) return 0;
-    bool apart;
-    const int split = ffn_split(M, F, K, false, apart);          // never more with the weight gradients
-    return split == 1 ? 0 : ceil_div(M, kFM / 2) * ceil_div(K, kSN) * split * kPart;
+    int64_t most = 0;
+    for (const bool dw : {false, true}) {
+        const FfnPlan plan = ffn_plan(M, F, K, true, dw);
+        if (plan.split > 1)
+            most = std::max(most, ffn_dx_tiles(M, K, plan.width) * plan.split * ffn_part_bytes(plan.width));
+    }
+    return most;
 }

@@ -358,7 +358,8 @@ def test_attention_of_a_single_key_is_its_value(others, dim, dtype):
 
 SHAPES = [(1, 128, 64), (1, 2056, 768), (3, 8, 8), (17, 264, 72), (128, 128, 128), (129, 136, 776), (200, 1160, 768),
           (300, 64, 1000), (1000, 520, 264), (8, 1024, 2048), (9, 1000, 520), (64, 776, 512), (2500, 328, 520),
-          (130, 1400, 136), (270, 18312, 264)]
+          (130, 1400, 136), (270, 18312, 264), (400, 22000, 264),
+          (140, 2824, 1032)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
