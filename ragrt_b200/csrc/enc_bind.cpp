@@ -192,7 +192,7 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
             if (t->scalar_type() != (t == dh ? x->scalar_type() : at::kFloat) || t->dim() != 2 || t->size(0) != M || t->size(1) != F || !solid(*t))
                 Py_RETURN_NONE;
         at::Tensor dg = like(*x, {M, F}), du = like(*x, {M, F}), rx, rg, ru, ws;
-        const int64_t bytes = dx ? f_ffn_workspace((int32_t)M, (int32_t)F, (int32_t)K) : 0;
+        const int64_t bytes = dx || dw ? f_ffn_workspace((int32_t)M, (int32_t)F, (int32_t)K) : 0;
         if (bytes) ws = at::empty({bytes}, dg.options().dtype(at::kByte));
         if (dx) rx = like(*x, {M, K});
         if (dw) {

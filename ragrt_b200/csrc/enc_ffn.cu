@@ -11,8 +11,10 @@
 //                           halves add up in the accumulator), and both weight gradients, contracted
 //                           over the rows of x: one list of tiles.  Persistent pairs of CTAs
 //                           (cta_group::2) on 256 x 256 accumulators, each CTA loading and draining its half.
-//   ffn_small<T, ...>       the same on 128 x 64 accumulators, two single CTAs per SM: more and shorter
-//                           tiles where the large ones would leave SMs without work.
+//   ffn_small<T, ...>       the same on accumulators of 128 x 64, or 128 for the gradients, two single CTAs per
+//                           SM: more and shorter tiles where the large ones would leave SMs without work,
+//                           and contractions cut into parts where even these are few.
+//   ffn_join                those parts' sums, in fp32 and in their order.
 //   ffn_rows                forward of up to four rows: a warp per pair of weight rows, fp32 on the CUDA
 //                           cores, bound by the weights' bytes.
 //   ffn_act_backward        dg and du, elementwise; at memory speed (8192 x 5504: 97 us, 6.5 TB/s).
@@ -64,7 +66,7 @@ struct FfnParams {
     int keep;                  // kForward: g and u are written too
     int dx, dw;                // kBackward: which gradients
     int a_rows;                // ffn_small: rows of x, dg, du that a load brings
-    int split;                 // ffn_small: parts of dx's contraction, each an entry of the list
+    int split, split_dw;       // ffn_small: parts of dx's and the weight gradients' contraction, each an entry
     float4* partial;           // their sums, [entry][quad of columns][row], what a warp's stores fill whole
     void* out[3];              // as in FfnMaps
     int* err;
@@ -86,7 +88,7 @@ struct FfnList {
         const int cols = kMode == kForward ? p.F : p.K;
         tn = (cols + kTileN - 1) / kTileN;
         first = kMode == kForward || p.dx ? tn * ((p.M + kTileM - 1) / kTileM) * p.split : 0;
-        per = kMode == kBackward && p.dw ? tn * ((p.F + kTileM - 1) / kTileM) : 0;
+        per = kMode == kBackward && p.dw ? tn * ((p.F + kTileM - 1) / kTileM) * p.split_dw : 0;
         total = first + 2 * per;
     }
     __device__ __forceinline__ FfnTile get(const FfnParams& p, int t) const {
@@ -104,11 +106,12 @@ struct FfnList {
         const int nk = kMode == kBackward && !dw ? 2 * r.chunks : r.chunks;
         r.i0 = 0;
         r.i1 = nk;
-        if (kMode == kBackward && !dw && p.split > 1) {
-            const int part = t % p.split;
-            t /= p.split;
-            r.i0 = (int)((int64_t)nk * part / p.split);
-            r.i1 = (int)((int64_t)nk * (part + 1) / p.split);
+        const int split = dw ? p.split_dw : p.split;
+        if (kMode == kBackward && split > 1) {
+            const int part = t % split;
+            t /= split;
+            r.i0 = (int)((int64_t)nk * part / split);
+            r.i1 = (int)((int64_t)nk * (part + 1) / split);
         }
         const int tm = (r.rows + kTileM - 1) / kTileM;
         const int band = t / (8 * tn), in = t % (8 * tn), high = min(8, tm - 8 * band);
@@ -527,8 +530,9 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(acce + b);
                 }
-                if (kMode == kBackward && tile.out == 0 && p.split > 1) {
-                    float4* to = p.partial + ((int64_t)t * (kN / 4) + c0 / 4) * (kFM / 2) + quad * 32 + lane;
+                if (kMode == kBackward && (tile.out == 0 ? p.split : p.split_dw) > 1) {
+                    const int entry = p.split > 1 ? t : t - list.first;
+                    float4* to = p.partial + ((int64_t)entry * (kN / 4) + c0 / 4) * (kFM / 2) + quad * 32 + lane;
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
                         to[q * (kFM / 2)] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
@@ -583,29 +587,33 @@ ffn_small(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParam
     }
 }
 
-// dx from the parts' sums, in their order; a thread per 8 values.
+// Gradients from their parts' sums, in the parts' order; a thread per 8 values, the tiles of what is not split left out.
 template <typename T, int kN>
-__global__ void __launch_bounds__(256) ffn_dx_join(const __grid_constant__ FfnParams p) {
+__global__ void __launch_bounds__(256) ffn_join(const __grid_constant__ FfnParams p) {
     pdl_wait_then_release();
     const int i = blockIdx.x * 256 + threadIdx.x;
-    const int r = i % (kFM / 2), c = i / (kFM / 2) % (kN / 8) * 8, t = i / (kFM / 2 * kN / 8);
+    const int r = i % (kFM / 2), c = i / (kFM / 2) % (kN / 8) * 8;
     FfnParams whole = p;
-    whole.split = 1;
-    whole.dw = 0;
+    if (p.split == 1) whole.dx = 0;
+    if (p.split_dw == 1) whole.dw = 0;
+    whole.split = whole.split_dw = 1;
     const FfnList<kBackward, kFM / 2, kN> list(whole);
+    const int t = i / (kFM / 2 * kN / 8);
     if (t >= list.total) return;
     const FfnTile tile = list.get(whole, t);
     const int row = tile.m0 + r, col = tile.n0 + c;
     if (row >= tile.rows || col >= tile.cols) return;
+    const int parts = tile.out == 0 ? p.split : p.split_dw;
+    const int entry = tile.out == 0 ? t * p.split : list.first * p.split + (t - list.first) * p.split_dw;
     float sum[8] = {};
-    const float4* from = p.partial + (int64_t)t * p.split * (kN / 4 * kFM / 2) + c / 4 * (kFM / 2) + r;
+    const float4* from = p.partial + (int64_t)entry * (kN / 4 * kFM / 2) + c / 4 * (kFM / 2) + r;
 #pragma unroll 4
-    for (int s = 0; s < p.split; ++s, from += kN / 4 * kFM / 2) {
+    for (int s = 0; s < parts; ++s, from += kN / 4 * kFM / 2) {
         const float4 a = __ldcs(from), b = __ldcs(from + kFM / 2);
         sum[0] += a.x; sum[1] += a.y; sum[2] += a.z; sum[3] += a.w;
         sum[4] += b.x; sum[5] += b.y; sum[6] += b.z; sum[7] += b.w;
     }
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.out[0]) + (int64_t)row * tile.cols + col) = down8<T>(sum);
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out[tile.out]) + (int64_t)row * tile.cols + col) = down8<T>(sum);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -752,14 +760,15 @@ int64_t ffn_tiles(int mode, const FfnParams& p, int tile_m, int tile_n) {
     return ((p.dx ? ceil_div(p.M, tile_m) : 0) + (p.dw ? 2 * ceil_div(p.F, tile_m) : 0)) * ceil_div(p.K, tile_n);
 }
 
-// How the gradients run on 128-row tiles: their width, the parts that dx's contraction is cut into (1: whole), and
-// whether dx has a launch of its own (apart).
+// How the gradients run on 128-row tiles: their width, the parts that the contraction of dx and of the weight gradients
+// is cut into (1: whole), and whether dx has a launch of its own (apart).
 struct FfnPlan {
-    int width, split;
+    int width, split, split_dw;
     bool apart;
 };
 
 int64_t ffn_dx_tiles(int M, int K, int width) { return ceil_div(M, kFM / 2) * ceil_div(K, width); }
+int64_t ffn_dw_tiles(int F, int K, int width) { return 2 * ceil_div(F, kFM / 2) * ceil_div(K, width); }
 int64_t ffn_part_bytes(int width) { return (int64_t)(kFM / 2) * width * 4; }
 
 // The parts of least time, as the longest share of a CTA in chunks of the contraction: dx's parts and then `per` tiles
@@ -787,6 +796,26 @@ int ffn_parts(int64_t tiles, int64_t nk, int64_t per, int64_t of_dw) {
     return best;
 }
 
+// Whether the weight gradients' contraction, over the rows, is cut: where many rows meet small matrices, so that even
+// the 128 x 128 tiles are no more than the SMs.  An SM takes 0.41 us for a chunk of those, a pair as long for one of 256 x
+// 256 (so twice the rate); the former are spread evenly by the cut and pay 8 us for it, the latter's longest share counts.
+// All gradients whole and cut: 16000 rows 256 -> 256 87 and 25.5 us, 16384 rows 384 -> 1536 187 and 153, 4000 rows 512 ->
+// 512 32 and 25; not cut by this rule: 8192 rows 512 -> 2048 110, 3000 rows 512 -> 1024 26.
+bool ffn_cut_dw(int M, int F, int K, bool dx) {
+    const int64_t sms = num_sms(), pairs = sms / 2, nk = 2 * ceil_div(F, kFK), of_dw = ceil_div(M, kFK);
+    const int64_t per = ffn_dw_tiles(F, K, 128);
+    if (per > sms || of_dw < 32) return false;
+    const int64_t n_dx = dx ? ceil_div(M, kFM) * ceil_div(K, kFN) : 0, n_dw = 2 * ceil_div(F, kFM) * ceil_div(K, kFN);
+    auto share = [&](int64_t c) {
+        const int64_t n = ceil_div(std::max<int64_t>(n_dx + n_dw - c, 0), pairs);
+        const int64_t d = ceil_div(std::max<int64_t>(n_dx - c, 0), pairs);
+        return d * nk + (n - d) * of_dw;
+    };
+    const int64_t large = std::max(share(0), share(n_dx % pairs));
+    const int64_t small = ((dx ? ffn_dx_tiles(M, K, 128) * nk : 0) + per * of_dw) / sms + 20;
+    return 10 * small < 9 * large;
+}
+
 // dx is cut where it has fewer tiles than there are SMs: its time is that of the 2 F steps of one tile then, 0.3 us
 // a chunk.  Not under 32 chunks (60 rows 512 -> 512 in two parts 10.1 us, whole 8.2).  The weight gradients join its
 // launch while they are 27 chunks per SM or fewer; else dx runs apart if its chain shrinks by 64 chunks, or is left
@@ -800,11 +829,17 @@ int ffn_parts(int64_t tiles, int64_t nk, int64_t per, int64_t of_dw) {
 // of 25 rows 768 -> 2048 9.9 and 10.4, of 256 rows 4096 -> 8192 60 and 52.
 FfnPlan ffn_plan(int M, int F, int K, bool dx, bool dw) {
     const int64_t sms = num_sms(), nk = 2 * ceil_div(F, kFK), of_dw = ceil_div(M, kFK);
-    FfnPlan plan{64, 1, false};
+    FfnPlan plan{64, 1, 1, false};
+    if (dw && ffn_cut_dw(M, F, K, dx)) {
+        const int64_t tiles = dx ? ffn_dx_tiles(M, K, 128) : 0, per = ffn_dw_tiles(F, K, 128);
+        plan.width = 128;
+        plan.split_dw = (int)std::min({(int64_t)16, of_dw / 8, 2 * sms / per});
+        if (tiles > 0 && tiles <= sms) plan.split = (int)std::max<int64_t>(1, std::min({(int64_t)16, nk / 16, sms / tiles}));
+        return plan;
+    }
     for (const int width : {64, 128}) {
-        const int64_t tiles = dx ? ffn_dx_tiles(M, K, width) : 0;
-        const int64_t per = dw ? 2 * ceil_div(F, kFM / 2) * ceil_div(K, width) : 0;
-        plan = FfnPlan{width, 1, false};
+        const int64_t tiles = dx ? ffn_dx_tiles(M, K, width) : 0, per = dw ? ffn_dw_tiles(F, K, width) : 0;
+        plan = FfnPlan{width, 1, 1, false};
         if (tiles > 0 && tiles <= sms && nk >= 32) {
             plan.apart = dw && per * of_dw * width / 128 > 27 * sms;
             plan.split = ffn_parts(tiles, nk, plan.apart ? 0 : per, of_dw);
@@ -836,6 +871,7 @@ int ffn_launch(int dtype, FfnParams p, int width, const void* x, const void* wg,
     const int64_t large = ffn_tiles(kMode, p, kFM, kMode == kForward ? kFN / 2 : kFN);
     int64_t small = ffn_tiles(kMode, p, kFM / 2, kMode == kForward ? width / 2 : width);
     if (p.dx) small += (p.split - 1) * ffn_dx_tiles(p.M, p.K, width);
+    if (p.dw) small += (p.split_dw - 1) * ffn_dw_tiles(p.F, p.K, width);
     bool pair;
     if (kMode == kForward) {
         // small tiles while they are one round of two CTAs per SM: 128 rows 2048 -> 5504 (172 tiles) 12.9 us
@@ -850,7 +886,7 @@ int ffn_launch(int dtype, FfnParams p, int width, const void* x, const void* wg,
         const int64_t of_dx = 2 * ceil_div(p.F, kFK), of_dw = ceil_div(p.M, kFK);
         const int64_t n_dx = p.dx ? ceil_div(p.M, kFM) * ceil_div(p.K, kFN) : 0;
         const int64_t sum = n_dx * of_dx + (large - n_dx) * of_dw;
-        pair = p.split == 1 && 5 * sum >= pairs * std::max(p.dx ? of_dx : 0, p.dw ? of_dw : 0);
+        pair = p.split == 1 && p.split_dw == 1 && 5 * sum >= pairs * std::max(p.dx ? of_dx : 0, p.dw ? of_dw : 0);
     }
     if (std::max(large, small) > 0x3FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many tiles");
     // few rows: a load brings no more of them than there are (one row of 2048 -> 5504 10.6 us; with
@@ -872,18 +908,22 @@ template <typename T>
 int ffn_backward(int dtype, FfnParams p, const void* x, const void* wg, const void* wu, const void* dg, const void* du,
                  void* ws, int64_t ws_bytes, cudaStream_t stream) {
     const FfnPlan plan = ffn_plan(p.M, p.F, p.K, p.dx != 0, p.dw != 0);
-    const int64_t tiles = ffn_dx_tiles(p.M, p.K, plan.width);
-    const int64_t room = ws ? ws_bytes / (tiles * ffn_part_bytes(plan.width)) : 0;
-    p.split = (int)std::max<int64_t>(1, std::min<int64_t>(plan.split, room));
-    if (p.split == 1) return ffn_launch<T, kBackward>(dtype, p, plan.width, x, wg, wu, dg, du, stream);
+    const int64_t tiles = p.dx ? ffn_dx_tiles(p.M, p.K, plan.width) : 0;
+    const int64_t per = p.dw ? ffn_dw_tiles(p.F, p.K, plan.width) : 0;
+    int64_t room = ws ? ws_bytes / ffn_part_bytes(plan.width) : 0;           // parts
+    if (tiles) p.split = (int)std::max<int64_t>(1, std::min<int64_t>(plan.split, room / tiles));
+    if (p.split > 1) room -= tiles * p.split;
+    if (per) p.split_dw = (int)std::max<int64_t>(1, std::min<int64_t>(plan.split_dw, room / per));
+    if (p.split == 1 && p.split_dw == 1) return ffn_launch<T, kBackward>(dtype, p, plan.width, x, wg, wu, dg, du, stream);
     FfnParams d = p;
     if (plan.apart) d.dw = 0;
     d.partial = (float4*)ws;
     int rc = ffn_launch<T, kBackward>(dtype, d, plan.width, x, wg, wu, dg, du, stream);
     if (rc) return rc;
-    const dim3 blocks((unsigned)(tiles * (kFM / 2) * plan.width / 8 / 256));
-    rc = plan.width == 64 ? enc_launch(ffn_dx_join<T, 64>, blocks, dim3(256), 0, stream, d)
-                          : enc_launch(ffn_dx_join<T, 128>, blocks, dim3(256), 0, stream, d);
+    const int64_t joined = (p.split > 1 ? tiles : 0) + (p.split_dw > 1 ? per : 0);
+    const dim3 blocks((unsigned)(joined * (kFM / 2) * plan.width / 8 / 256));
+    rc = plan.width == 64 ? enc_launch(ffn_join<T, 64>, blocks, dim3(256), 0, stream, d)
+                          : enc_launch(ffn_join<T, 128>, blocks, dim3(256), 0, stream, d);
     if (rc || d.dw == p.dw) return rc;
     p.dx = 0;
     p.split = 1;
@@ -918,7 +958,7 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
     int* err = device_error_flag();
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
     cudaStream_t stream = (cudaStream_t)stream_;
-    FfnParams p{M, F, K, act, d_gate != nullptr, 0, 0, 0, 1, nullptr, {d_h, d_gate, d_up}, err};
+    FfnParams p{M, F, K, act, d_gate != nullptr, 0, 0, 0, 1, 1, nullptr, {d_h, d_gate, d_up}, err};
     // One row at any size: 2048 -> 5504 5.8 us, on the tensor cores 11.0.  Up to four where the weights are few: 4
     // rows 768 -> 2048 4.4 us against 5.2, 2048 -> 4096 9.1 against 10.2; 2048 -> 5504 12.8 against 11.0.
     if (M == 1 || (M <= kFewRows && (int64_t)F * K <= (1 << 23))) {
@@ -965,7 +1005,7 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
                           d_gate, d_up, (__half*)d_dgate, (__half*)d_dup, n8, (int)act);
     if (rc) return rc;
     if (!d_dx && !d_dw_gate) return RAGRT_OK;
-    FfnParams p{M, F, K, act, 0, d_dx != nullptr, d_dw_gate != nullptr, 0, 1, nullptr, {d_dx, d_dw_gate, d_dw_up}, err};
+    FfnParams p{M, F, K, act, 0, d_dx != nullptr, d_dw_gate != nullptr, 0, 1, 1, nullptr, {d_dx, d_dw_gate, d_dw_up}, err};
     return dtype == RAGRT_BF16
                ? ffn_backward<__nv_bfloat16>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, d_ws, ws_bytes, stream)
                : ffn_backward<__half>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, d_ws, ws_bytes, stream);
@@ -974,10 +1014,11 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
 extern "C" int64_t ragrt_enc_gated_ffn_workspace(int32_t M, int32_t F, int32_t K) {
     if (M < 1 || F < 8 || K < 8) return 0;
     int64_t most = 0;
-    for (const bool dw : {false, true}) {
-        const FfnPlan plan = ffn_plan(M, F, K, true, dw);
-        if (plan.split > 1)
-            most = std::max(most, ffn_dx_tiles(M, K, plan.width) * plan.split * ffn_part_bytes(plan.width));
+    for (const int want : {1, 2, 3}) {                               // dx, weights, both
+        const FfnPlan plan = ffn_plan(M, F, K, want & 1, want & 2);
+        const int64_t parts = (want & 1 && plan.split > 1 ? ffn_dx_tiles(M, K, plan.width) * plan.split : 0) +
+                              (want & 2 && plan.split_dw > 1 ? ffn_dw_tiles(F, K, plan.width) * plan.split_dw : 0);
+        most = std::max(most, parts * ffn_part_bytes(plan.width));
     }
     return most;
 }

@@ -359,7 +359,7 @@ def test_attention_of_a_single_key_is_its_value(others, dim, dtype):
 SHAPES = [(1, 128, 64), (1, 2056, 768), (3, 8, 8), (17, 264, 72), (128, 128, 128), (129, 136, 776), (200, 1160, 768),
           (300, 64, 1000), (1000, 520, 264), (8, 1024, 2048), (9, 1000, 520), (64, 776, 512), (2500, 328, 520),
           (130, 1400, 136), (270, 18312, 264), (400, 22000, 264),
-          (140, 2824, 1032)]
+          (140, 2824, 1032), (4104, 264, 264), (2100, 1032, 72)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -454,6 +454,34 @@ def test_gated_ffn_backward_with_less_scratch_or_none():
             got.append(dx)
         L.check(got[0], want, bound)
         assert torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("M,F,K", [(4104, 264, 136), (2100, 1032, 72)])
+def test_gated_ffn_weight_gradients_with_less_scratch_or_none(M, F, K):
+    """As above for the contraction over many rows; alone, beside dx, and with what dx leaves of the scratch."""
+    dtype = torch.bfloat16
+    x, wg, wu, dh = ffn_inputs(M, F, K, dtype, 22)
+    _, gate, up = encoder.gated_ffn(x, wg, wu, keep=True)
+    wants = L.ffn_backward64(dh, x, wg, wu, gate, up, "silu")
+    lib = _lib.lib()
+    full = lib.ragrt_enc_gated_ffn_workspace(M, F, K)
+    part = 128 * 128 * 4
+    assert full >= 2 * part
+    tmp = torch.empty_like(dh), torch.empty_like(dh)
+    for nbytes in (0, part, full // 3, full - part, full):
+        ws = torch.full((max(nbytes, 16) + 64,), 77, dtype=torch.uint8, device="cuda")
+        for with_dx in (False, True):
+            got = [torch.full_like(t, 9.0) for t in (x, wg, wu)]
+            _lib.check(lib.ragrt_enc_gated_ffn_backward(
+                dh.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), gate.data_ptr(), up.data_ptr(),
+                tmp[0].data_ptr(), tmp[1].data_ptr(), got[0].data_ptr() if with_dx else None, got[1].data_ptr(),
+                got[2].data_ptr(), M, F, K, 0, 1, ws.data_ptr() if nbytes else None, nbytes,
+                torch.cuda.current_stream().cuda_stream))
+            for g, (want, bound), what in list(zip(got, wants, ("dx", "dwg", "dwu")))[0 if with_dx else 1:]:
+                L.check(g, want, bound, what)
+            if not with_dx:
+                assert bool((got[0] == 9.0).all())
+        assert bool((ws[nbytes:] == 77).all())
 
 
 def test_gated_ffn_partial_gradients_and_no_rows():
