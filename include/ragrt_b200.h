@@ -418,16 +418,18 @@ int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const void* d_w_u
  * d_dx [M, K] (may be NULL), d_dw_gate and d_dw_up [F, K] (may both be NULL).  Overwrites, does
  * not add to, its outputs; the order of every sum is fixed.  M = 0 gives zero weight gradients.
  * d_ws (ws_bytes, may be NULL / 0): scratch where a contraction (dx's for few rows, the weight gradients' for
- * many rows and small matrices) is split over more CTAs and joined in fp32 (ragrt_enc_gated_ffn_workspace bytes; fewer parts when there are fewer).  Calls that
- * may overlap on the GPU, on two streams or in two graphs, need a scratch each, as they need outputs of their own.
+ * many rows and small matrices) is split over more CTAs and joined in fp32
+ * (ragrt_enc_gated_ffn_workspace bytes; fewer parts when there are fewer).  Calls that may overlap
+ * on the GPU, on two streams or in two graphs, need a scratch each, as they need outputs of their own.
  */
 int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, const void* d_w_gate, const void* d_w_up,
                                  const float* d_gate, const float* d_up, void* d_dgate, void* d_dup, void* d_dx,
                                  void* d_dw_gate, void* d_dw_up, int32_t M, int32_t F, int32_t K, int32_t act,
                                  int32_t dtype, void* d_ws, int64_t ws_bytes, void* stream);
 
-/* Bytes of scratch that ragrt_enc_gated_ffn_backward can use for these sizes (0: none; 38.8 MB at most). */
-int64_t ragrt_enc_gated_ffn_workspace(int32_t M, int32_t F, int32_t K);
+/* Bytes of scratch that ragrt_enc_gated_ffn_backward can use for these sizes, for dx (dx != 0) and the
+ * weight gradients (dw != 0); 0: none; 38.8 MB at most. */
+int64_t ragrt_enc_gated_ffn_workspace(int32_t M, int32_t F, int32_t K, int32_t dx, int32_t dw);
 
 /* Library version string. */
 const char* ragrt_version(void);

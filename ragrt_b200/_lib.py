@@ -70,7 +70,7 @@ _SIGS = {
                                      C.c_float, I32, I32, P]),
     "ragrt_enc_gated_ffn": (I32, [P, P, P, P, P, P, I32, I32, I32, I32, I32, P]),
     "ragrt_enc_gated_ffn_backward": (I32, [P, P, P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, P, I64, P]),
-    "ragrt_enc_gated_ffn_workspace": (I64, [I32, I32, I32]),
+    "ragrt_enc_gated_ffn_workspace": (I64, [I32, I32, I32, I32, I32]),
 }
 
 _lib = None

@@ -8,6 +8,7 @@
 // status.  The library's entry points come by address (bind), from the one ctypes has loaded.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -48,7 +49,11 @@ int64_t row_stride(const at::Tensor& t) {
     return t.stride(0) >= H * D && t.stride(0) % 8 == 0 ? t.stride(0) : 0;
 }
 bool fits(int64_t n) { return n >= 0 && n <= 0x7FFFFFFF; }
-at::Tensor like(const at::Tensor& t, at::IntArrayRef shape) { return at::empty(shape, t.options().requires_grad(false)); }
+// A new tensor on t's device, straight from the allocator of torch's CUDA tensors.
+at::Tensor fresh(const at::Tensor& t, at::IntArrayRef shape, at::ScalarType type) {
+    return at::Tensor(at::detail::empty_cuda(shape, type, t.device(), std::nullopt));
+}
+at::Tensor like(const at::Tensor& t, at::IntArrayRef shape) { return fresh(t, shape, t.scalar_type()); }
 void* stream(int device) { return (void*)at::cuda::getCurrentCUDAStream(device).stream(); }
 
 // A C++ exception becomes Python's error, as torch itself translates it (out of memory above all).
@@ -161,8 +166,8 @@ PyObject* gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t M = x->size(0), F = g->size(0), K = x->size(1);
         at::Tensor h = like(*x, {M, F}), gate, up;
         if (keep) {
-            gate = at::empty({M, F}, h.options().dtype(at::kFloat));
-            up = at::empty({M, F}, h.options().dtype(at::kFloat));
+            gate = fresh(*x, {M, F}, at::kFloat);
+            up = fresh(*x, {M, F}, at::kFloat);
         }
         const int rc = f_ffn(x->data_ptr(), g->data_ptr(), u->data_ptr(), h.data_ptr(), keep ? (float*)gate.data_ptr() : nullptr,
                              keep ? (float*)up.data_ptr() : nullptr, (int32_t)M, (int32_t)F, (int32_t)K, (int32_t)act, dt,
@@ -191,18 +196,21 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
         for (const at::Tensor* t : {dh, gate, up})
             if (t->scalar_type() != (t == dh ? x->scalar_type() : at::kFloat) || t->dim() != 2 || t->size(0) != M || t->size(1) != F || !solid(*t))
                 Py_RETURN_NONE;
-        at::Tensor dg = like(*x, {M, F}), du = like(*x, {M, F}), rx, rg, ru, ws;
-        const int64_t bytes = dx || dw ? f_ffn_workspace((int32_t)M, (int32_t)F, (int32_t)K) : 0;
-        if (bytes) ws = at::empty({bytes}, dg.options().dtype(at::kByte));
+        // dg, du and the parts' sums, in one piece
+        const int64_t bytes = f_ffn_workspace((int32_t)M, (int32_t)F, (int32_t)K, dx, dw), n = (M * F * 2 + 15) / 16 * 16;
+        const at::Tensor scratch = fresh(*x, {2 * n + bytes}, at::kByte);
+        char* own = (char*)scratch.data_ptr();
+        at::Tensor rx, rg, ru;
         if (dx) rx = like(*x, {M, K});
         if (dw) {
             rg = like(*x, {F, K});
             ru = like(*x, {F, K});
         }
         const int rc = f_ffn_backward(dh->data_ptr(), x->data_ptr(), g->data_ptr(), u->data_ptr(),
-                                      (const float*)gate->data_ptr(), (const float*)up->data_ptr(), dg.data_ptr(), du.data_ptr(), dx ? rx.data_ptr() : nullptr,
-                                      dw ? rg.data_ptr() : nullptr, dw ? ru.data_ptr() : nullptr, (int32_t)M, (int32_t)F,
-                                      (int32_t)K, (int32_t)act, dt, bytes ? ws.data_ptr() : nullptr, bytes, stream(dev));
+                                      (const float*)gate->data_ptr(), (const float*)up->data_ptr(), own, own + n,
+                                      dx ? rx.data_ptr() : nullptr, dw ? rg.data_ptr() : nullptr,
+                                      dw ? ru.data_ptr() : nullptr, (int32_t)M, (int32_t)F, (int32_t)K, (int32_t)act,
+                                      dt, bytes ? own + 2 * n : nullptr, bytes, stream(dev));
         if (rc) return PyLong_FromLong(rc);
         auto wrap = [](bool has, at::Tensor& t) {
             if (has) return THPVariable_Wrap(std::move(t));

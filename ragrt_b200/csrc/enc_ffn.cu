@@ -776,20 +776,19 @@ int64_t ffn_part_bytes(int width) { return (int64_t)(kFM / 2) * width * 4; }
 // epilogue; a part 4 more; every entry of the list costs the SM 2; the joining kernel 8 and one per 64 parts.  Parts of
 // 8 chunks or more, at most two per SM in all (and 16 of a tile).  Against all counts, measured for 20 shapes from 25 x
 // 768 -> 2048 to 256 x 4096 -> 8192: within 5 % of the best for dx, 13 % for all gradients.
-int ffn_parts(int64_t tiles, int64_t nk, int64_t per, int64_t of_dw) {
-    const int64_t ctas = 2 * num_sms();
-    int best = 1;
-    int64_t least = 0;
-    for (int64_t s = 1; s <= 16 && (s == 1 || (s <= nk / 8 && s * tiles <= ctas)); ++s) {
-        auto share = [&](int64_t c) {
-            const int64_t n = ceil_div(std::max<int64_t>(tiles * s + per - c, 0), ctas);
-            const int64_t dx = ceil_div(std::max<int64_t>(tiles * s - c, 0), ctas);
-            return dx * (ceil_div(nk, s) + 4) + (n - dx) * std::max<int64_t>(of_dw, 16);
+int ffn_parts(int tiles, int nk, int per, int of_dw) {
+    const int sms = num_sms(), ctas = 2 * sms;
+    int best = 1, least = 0;
+    for (int s = 1; s <= 16 && (s == 1 || (s <= nk / 8 && s * tiles <= ctas)); ++s) {
+        // a CTA's first entry is one of dx, its own number if it has one; then come the others in turn
+        const int parts = tiles * s, part = (nk + s - 1) / s + 4;
+        auto share = [&](int c) {
+            const int n = (std::max(parts + per - c, 0) + ctas - 1) / ctas, dx = c < parts ? 1 : 0;
+            return dx * part + (n - dx) * std::max(of_dw, 16);
         };
-        const int64_t time = std::max(share(0), share(tiles * s % ctas)) + (s > 1 ? 8 + tiles * s / 64 : 0) +
-                             2 * (tiles * s + per) / num_sms();
+        const int time = std::max(share(0), share(parts % ctas)) + (s > 1 ? 8 + parts / 64 : 0) + 2 * (parts + per) / sms;
         if (s == 1 || time < least) {
-            best = (int)s;
+            best = s;
             least = time;
         }
     }
@@ -842,7 +841,7 @@ FfnPlan ffn_plan(int M, int F, int K, bool dx, bool dw) {
         plan = FfnPlan{width, 1, 1, false};
         if (tiles > 0 && tiles <= sms && nk >= 32) {
             plan.apart = dw && per * of_dw * width / 128 > 27 * sms;
-            plan.split = ffn_parts(tiles, nk, plan.apart ? 0 : per, of_dw);
+            plan.split = ffn_parts((int)tiles, (int)nk, plan.apart ? 0 : (int)per, (int)of_dw);
             if (plan.apart && nk - nk / plan.split < 64) plan.split = 1;
         }
         if (plan.split == 1) plan.apart = false;
@@ -1011,14 +1010,10 @@ extern "C" int ragrt_enc_gated_ffn_backward(const void* d_dh, const void* d_x, c
                : ffn_backward<__half>(dtype, p, d_x, d_w_gate, d_w_up, d_dgate, d_dup, d_ws, ws_bytes, stream);
 }
 
-extern "C" int64_t ragrt_enc_gated_ffn_workspace(int32_t M, int32_t F, int32_t K) {
+extern "C" int64_t ragrt_enc_gated_ffn_workspace(int32_t M, int32_t F, int32_t K, int32_t dx, int32_t dw) {
     if (M < 1 || F < 8 || K < 8) return 0;
-    int64_t most = 0;
-    for (const int want : {1, 2, 3}) {                               // dx, weights, both
-        const FfnPlan plan = ffn_plan(M, F, K, want & 1, want & 2);
-        const int64_t parts = (want & 1 && plan.split > 1 ? ffn_dx_tiles(M, K, plan.width) * plan.split : 0) +
-                              (want & 2 && plan.split_dw > 1 ? ffn_dw_tiles(F, K, plan.width) * plan.split_dw : 0);
-        most = std::max(most, parts * ffn_part_bytes(plan.width));
-    }
-    return most;
+    const FfnPlan plan = ffn_plan(M, F, K, dx != 0, dw != 0);
+    const int64_t parts = (dx && plan.split > 1 ? ffn_dx_tiles(M, K, plan.width) * plan.split : 0) +
+                          (dw && plan.split_dw > 1 ? ffn_dw_tiles(F, K, plan.width) * plan.split_dw : 0);
+    return parts * ffn_part_bytes(plan.width);
 }

@@ -387,7 +387,7 @@ def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu", need_dx=True, 
     dgate, dup = torch.empty_like(dh), torch.empty_like(dh)
     dx = torch.empty_like(x) if need_dx else None
     dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if need_dw else (None, None)
-    nbytes = _lib.lib().ragrt_enc_gated_ffn_workspace(M, F, K) if need_dx or need_dw else 0
+    nbytes = _lib.lib().ragrt_enc_gated_ffn_workspace(M, F, K, bool(need_dx), bool(need_dw))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _lib.check(_lib.lib().ragrt_enc_gated_ffn_backward(
         dh.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), gate.data_ptr(), up.data_ptr(), dgate.data_ptr(),

@@ -439,7 +439,7 @@ def test_gated_ffn_backward_with_less_scratch_or_none():
     _, gate, up = encoder.gated_ffn(x, wg, wu, keep=True)
     want, bound = L.ffn_backward64(dh, x, wg, wu, gate, up, "silu")[0]
     lib = _lib.lib()
-    full = lib.ragrt_enc_gated_ffn_workspace(M, F, K)
+    full = lib.ragrt_enc_gated_ffn_workspace(M, F, K, 1, 0)
     assert 0 < full <= torch.cuda.get_device_properties(0).multi_processor_count * 128 * 128 * 4
     tmp = torch.empty_like(dh), torch.empty_like(dh)
     for nbytes in (0, 1000, 3 * 128 * 64 * 4, 2 * 3 * 128 * 64 * 4, full):
@@ -464,7 +464,7 @@ def test_gated_ffn_weight_gradients_with_less_scratch_or_none(M, F, K):
     _, gate, up = encoder.gated_ffn(x, wg, wu, keep=True)
     wants = L.ffn_backward64(dh, x, wg, wu, gate, up, "silu")
     lib = _lib.lib()
-    full = lib.ragrt_enc_gated_ffn_workspace(M, F, K)
+    full = lib.ragrt_enc_gated_ffn_workspace(M, F, K, 1, 1)
     part = 128 * 128 * 4
     assert full >= 2 * part
     tmp = torch.empty_like(dh), torch.empty_like(dh)
