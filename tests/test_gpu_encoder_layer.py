@@ -484,6 +484,43 @@ def test_gated_ffn_weight_gradients_with_less_scratch_or_none(M, F, K):
         assert bool((ws[nbytes:] == 77).all())
 
 
+def test_gated_ffn_gradients_in_parts_on_two_streams_and_in_graphs():
+    """The parts' sums of calls that run side by side, or are replayed, do not meet."""
+    sets = []
+    for seed, (M, F, K) in enumerate([(130, 1400, 136), (2100, 1032, 72), (400, 22000, 264)]):
+        x, wg, wu, dh = ffn_inputs(M, F, K, torch.bfloat16, 30 + seed)
+        _, gate, up = encoder.gated_ffn(x, wg, wu, keep=True)
+        assert _lib.lib().ragrt_enc_gated_ffn_workspace(M, F, K, 1, 1) > 0
+        sets.append((dh, x, wg, wu, gate, up))
+    want = [encoder.gated_ffn_backward(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(10):
+        got = []
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(encoder.gated_ffn_backward(*s))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(g, w))
+    graphs = []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = encoder.gated_ffn_backward(*s)
+        graphs.append((g, out))
+    for _ in range(3):
+        for st, (g, out) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for (g, out), w in zip(graphs, want):
+            assert all(torch.equal(a, b) for a, b in zip(out, w))
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+
+
 def test_gated_ffn_partial_gradients_and_no_rows():
     x, wg, wu, dh = ffn_inputs(130, 136, 72, torch.float16, 3)
     _, gate, up = encoder.gated_ffn(x, wg, wu, keep=True)
