@@ -179,6 +179,10 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)tc::cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const FfnList<kMode, kFM, kOutCols> list(p);
+    // The tiles are dealt out in turn, those of the last round, which does not reach all pairs, from the last pair on:
+    // the first ones hold one tile of dx more, and those are longer.
+    const int last = list.total / pairs * pairs;
+    auto after = [&](int t) { return t + pairs < last ? t + pairs : t < last ? last + pairs - 1 - pair : list.total; };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFStages; ++s) {
@@ -209,7 +213,7 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
         // ------------------------------------------------------------ TMA producer
         if (lane == 0) {
             int g = 0;
-            for (int t = pair; t < list.total && !failed; t += pairs) {
+            for (int t = pair; t < list.total && !failed; t = after(t)) {
                 const FfnTile tile = list.get(p, t);
                 const bool dw = kMode == kBackward && tile.out > 0;
                 const int m0 = tile.m0 + rank * (kFM / 2);
@@ -251,7 +255,7 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
         if (rank == 0) {
             const uint32_t lead = tc::elect_one();
             int g = 0, j = 0;
-            for (int t = pair; t < list.total && !failed; t += pairs, ++j) {
+            for (int t = pair; t < list.total && !failed; t = after(t), ++j) {
                 const FfnTile tile = list.get(p, t);
                 const bool dw = kMode == kBackward && tile.out > 0;
                 const uint32_t idesc = tc::idesc_f16_f32(kFM, kFN) | idesc_type<T>() | (dw ? kIdescAMn : 0u) |
@@ -311,7 +315,7 @@ ffn_pair(const __grid_constant__ FfnMaps maps, const __grid_constant__ FfnParams
             __syncwarp();
         };
         int j = 0;
-        for (int t = pair; t < list.total; t += pairs, ++j) {
+        for (int t = pair; t < list.total; t = after(t), ++j) {
             const FfnTile tile = list.get(p, t);
             const int b = j & 1;
             const int y = tile.m0 + rank * (kFM / 2) + quad * 32;
