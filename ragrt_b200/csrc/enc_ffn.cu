@@ -20,8 +20,9 @@
 //   ffn_act_backward        dg and du, elementwise; at memory speed (8192 x 5504: 97 us, 6.5 TB/s).
 //
 // Measured: 16384 x 2048 -> 8192 forward 688 us in a burst (1,600 TFLOP/s; 810 us, 1,360 TFLOP/s, under the
-// power cap); a training step of 8192 x 2048 -> 5504 237 us forward, 40 more for keeping g and u, 670
-// backward (cuBLAS for the three products alone: 251, 246 and 258 us).
+// power cap); a training step of 8192 x 2048 -> 5504 236 us forward, 36 more for keeping g and u, 645
+// backward, 99 of them elementwise (cuBLAS for the three products alone: 248, 202 and 226 us; one behind the other for
+// longer, at the power cap, 301, 286 and 306, and the backward pass here 694).
 //
 // The weight matrices and x are read as they lie: an operand whose contraction index is the row of
 // its matrix is fed to the tensor cores MN-major.  Accumulators are fp32.  g and u are kept in fp32: in 16
