@@ -88,7 +88,8 @@ __global__ void __launch_bounds__(32 * kRopeWarps, 24 / kRopeWarps) enc_qk_norm_
     T* ko = static_cast<T*>(p.ko) + t * p.ko_stride - p.heads * p.dim;
     const int all = p.heads + p.kv_heads;
     const int rounds = (all + per - 1) / per;               // heads in steps of a warp's worth
-    const int r0 = rounds * slab / p.slabs, r1 = rounds * (slab + 1) / p.slabs;
+    // of a token with a million heads the product passes 32 bits
+    const int r0 = (int)((int64_t)rounds * slab / p.slabs), r1 = (int)((int64_t)rounds * (slab + 1) / p.slabs);
     const float inv_dim = 1.0f / (float)p.dim;
     const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
     float c[8], s[8];
