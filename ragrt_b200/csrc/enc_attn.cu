@@ -626,6 +626,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                                 for (int q = 0; q < 16; ++q) r16[q] = __float_as_uint(__uint_as_float(r16[q]) * alpha);
                                 tc::st32x16(to + 16 * c, r16);
                             }
+                            tc::wait_st();      // the next step of 32 keys may read it again, to move it once more
                         }
                     }
                     return alpha;

@@ -45,3 +45,31 @@ def test_norm_rope_of_one_token_with_a_million_heads():
         for x, y in ((q, qo), (k, ko)):
             L.check(y[:, at:at + 1000], *L.rms_rope64(x[:, at:at + 1000], w, cos, sin, pos, 1e-6, False))
     assert flag() == 0
+
+
+# ------------------------------------------------------------------------------------ attention
+def by_scores(scores, v, D, dtype):
+    """q, k, v of one head whose row 0 onwards have score `scores[j]` (in powers of two) for key j."""
+    n = scores.shape[0]
+    q = torch.zeros(n, 1, D, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    k = torch.zeros(n, 1, D, dtype=dtype, device="cuda")
+    k[:, 0, 0] = scores.to(dtype)
+    return q, k, v.to(dtype)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_reference_moves_twice_in_a_block(D, causal):
+    """The maximum rises by more than 2^8 in both 32-key halves of one block, again and again: the accumulator is
+    scaled twice between two products.  Early values are so large that a factor left out shows."""
+    n = 320
+    j = torch.arange(n, device="cuda")
+    scores = (10.0 * (j // 32)).to(torch.bfloat16)          # 2^10 per step: exact
+    v = torch.randn(n, 1, D, generator=gen(1), device="cuda") * torch.exp2(-10.0 * (j // 32))[:, None, None]
+    q, k, v = by_scores(scores, v, D, torch.bfloat16)
+    cu = L.cu_of([n], "cuda")
+    scale = math.log(2.0)
+    want, bound = L.attention64(q, k, v, cu, causal, scale=scale)
+    for _ in range(20):
+        L.check(encoder.packed_attention(q, k, v, cu, causal=causal, scale=scale), want, bound)
