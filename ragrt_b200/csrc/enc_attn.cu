@@ -21,9 +21,11 @@
 //                      of the exponentials as polynomials on the FMA units (0.97 ms: issue, not that unit,
 //                      is short); two tiles of one CTA with an issuing warp each (1.20 ms: they fall into
 //                      step and want the same units at the same time).
-//   attn_row           one row of one head by a warp, in fp32.  A weight of zero does not keep a NaN or
-//                      an infinity in a masked row of V out of a matrix product: rows that come out
-//                      of it not finite are computed once more by this, over their own keys alone.
+//   attn_odd_rows      A weight of zero does not keep a NaN or an infinity in a masked row of V out of a
+//                      matrix product.  Of the rows that come out of it not finite this finds those that
+//                      are so by the formula, and what they are;
+//   attn_row           computes the others once more, over their own keys alone: one row of one head by
+//                      a warp, in fp32.
 #include <algorithm>
 
 #include "enc_common.cuh"
@@ -138,6 +140,75 @@ __device__ __noinline__ void attn_row(const AttnParams& p, int t, int h, int lo,
         if (lane + 32 * c < p.dim) dst[lane + 32 * c] = (T)(o[c] / l);
 }
 
+// Rows of one head, of a warp, whose output is not finite although the sum of their weights is: bit i of `rows` is
+// row row0 + i, which sees the keys [lo, end) (causal: [lo, row0 + i]).  A column in which a row of V that is seen is
+// not finite is NaN, or the infinity that all such rows agree on, by the formula.  A column without any has it from
+// a row of V that may not be seen, through a weight of zero: the rows returned, which are to be computed again.  A
+// row of V that is not finite does that to the rows before it in its tile alone, and there only in columns in which
+// no row before it was: few rows of a causal sequence.  It does it to all rows of a full sequence that ends less than
+// a block of keys before it.  The warp looks at each seen row of V once.  8192 rows, 8 heads of 128, causal, 0.19 ms
+// when all is finite: one NaN in an early row of V 0.69 ms, the later half of V NaN 0.89 (all such rows computed
+// again: 105 and 81).  No branch but the whole warp's and no vote: those made the kernel hold a convergence barrier's
+// state in memory across the call (1024 passages 194 -> 203 us).
+template <typename T>
+__device__ __noinline__ unsigned attn_odd_rows(const AttnParams& p, int h, int row0, unsigned rows, int lo, int end) {
+    constexpr uint32_t kExp = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u, kStep = kExp & (0u - kExp);
+    const int lane = threadIdx.x & 31, vec = lane & 15;                           // 8 values of every other row
+    const bool there = vec < p.dim / 8;
+    const T* v = static_cast<const T*>(p.v) + (int64_t)(h / (p.heads / p.kv_heads)) * p.dim + (there ? 8 * vec : 0);
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    uint32_t up = 0, down = 0, nan = 0;               // bit e: a seen row's value e is +inf, -inf, NaN
+    auto halves = [&](const uint4& u, auto f) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f(e, (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+    };
+    auto odd = [&](uint32_t w) { return (w & (kExp * 0x10001u)) + kStep * 0x10001u; };         // its top bits: not finite
+    int done = lo;
+    unsigned again = 0;
+    for (; rows; rows &= rows - 1) {                  // the branches are the whole warp's throughout
+        const int row = row0 + __ffs(rows) - 1, hi = p.causal ? row + 1 : end;
+#pragma unroll 1
+        for (; done < hi; done += 8) {
+            uint4 u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = done + 2 * i + (lane >> 4);
+                u[i] = there && j < hi ? __ldg(reinterpret_cast<const uint4*>(v + j * p.v_stride)) : zero;
+            }
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= odd(u[i].x) | odd(u[i].y) | odd(u[i].z) | odd(u[i].w);
+            if (__reduce_or_sync(0xFFFFFFFFu, any & 0x80008000u) == 0) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                halves(u[i], [&](int e, uint32_t x) {
+                    const uint32_t is = (x & kExp) == kExp ? 1u << e : 0u, not_inf = (x & 0x7FFFu & ~kExp) ? is : 0u;
+                    nan |= not_inf;
+                    down |= (x >> 15) ? is & ~not_inf : 0u;
+                    up |= (x >> 15) ? 0u : is & ~not_inf;
+                });
+        }
+        done = hi;
+        up |= __shfl_xor_sync(0xFFFFFFFFu, up, 16);
+        down |= __shfl_xor_sync(0xFFFFFFFFu, down, 16);
+        nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 16);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.out_stride + (int64_t)h * p.dim) + vec;
+        const uint32_t all = up | down | nan;
+        const uint4 was = there ? *dst : zero;
+        uint32_t w[4] = {}, left = 0;                 // left: not finite, and none of the seen rows is
+        halves(was, [&](int e, uint32_t x) {
+            const bool known = (all >> e) & 1u, is_nan = ((nan | (up & down)) >> e) & 1u;
+            left |= (x & kExp) == kExp && !known ? 1u : 0u;
+            x = !known ? x : is_nan ? 0x7FFFu : (down >> e) & 1u ? kExp | 0x8000u : kExp;
+            w[e >> 1] |= x << (16 * (e & 1));
+        });
+        if (__reduce_or_sync(0xFFFFFFFFu, left)) again |= rows & (0u - rows);
+        else if (there && lane < 16) *dst = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return again;
+}
+
 constexpr int kAFirst = 4;                     // first softmax warp: TMA, MMA and search warp before them, one idle
 constexpr int kAItems = 2;                     // items whose tiles are in shared memory
 // The reference maximum of a row moves only when it is exceeded by a factor of 2^8: until then the weights are
@@ -173,8 +244,8 @@ struct AttnMaps {
     CUtensorMap q, k, v;
 };
 
-// Bounded wait: 2 s, not counting the time that a warp of the CTA spends in attn_row (abort[1]: how many
-// do), or until another role gave up (abort[0]).  In few instructions: the roles' code shares the
+// Bounded wait: 2 s, not counting the time that a warp of the CTA spends in attn_odd_rows and attn_row (abort[1]:
+// how many do), or until another role gave up (abort[0]).  In few instructions: the roles' code shares the
 // instruction cache, and this is in it some twenty times.
 __device__ __forceinline__ bool attn_wait(uint64_t* m, uint32_t parity, volatile int* abort) {
     if (tc::mbar_try_wait_hint(m, parity, tc::kWaitHintNs)) return true;
@@ -206,7 +277,7 @@ struct AttnShared {
     uint64_t odone[kTiles];                  // product with V done
     uint64_t drain, taken;
     uint32_t tmem;
-    int abort[2];                            // given up; warps in attn_row
+    int abort[2];                            // given up; warps that mend rows
 };
 
 // The blocks of an item: blocks 0 .. n - 1 from key kv0 on, tile t takes [jb[t], je[t]) of them.
@@ -744,11 +815,13 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                         if (c + q < p.dim) *reinterpret_cast<uint4*>(dst + c + q) = down8<T>(*reinterpret_cast<float(*)[8]>(o + q));
                 }
             }
-            __syncwarp();                                         // a bad row's values above come before attn_row's
-            unsigned left = __ballot_sync(0xFFFFFFFFu, bad);
+            __syncwarp();                                         // the rows' values above come before what mends them
+            // A sum of weights that is NaN or 0 (a score is NaN or infinite, or all are -inf) makes all of the row NaN
+            // by the formula, as it is already.
+            unsigned left = __ballot_sync(0xFFFFFFFFu, bad && inv < INFINITY);
             if (left) {
                 if (lane == 0) atomicAdd(&sh->abort[1], 1);
-                for (; left; left &= left - 1) {
+                for (left = attn_odd_rows<T>(p, b.head, row - lane, left, own.lo, hi); left; left &= left - 1) {
                     const int src = __ffs(left) - 1;
                     attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), b.head, own.lo, __shfl_sync(0xFFFFFFFFu, hi, src));
                 }
@@ -815,7 +888,8 @@ extern "C" int ragrt_enc_packed_attention(const void* d_q, const void* d_k, cons
     RAGRT_REQUIRE(q_stride >= qw && out_stride >= qw && k_stride >= kw && v_stride >= kw &&
                       (q_stride | k_stride | v_stride | out_stride) % 8 == 0,
                   "row strides must hold all heads and be multiples of 8 elements");
-    RAGRT_REQUIRE(scale > 0.f && scale <= 3.0e38f, "scale must be positive and finite");
+    // the kernel's scores are powers of two: scale times log2 e is finite too
+    RAGRT_REQUIRE(scale > 0.f && scale <= 2.3e38f, "scale must be positive and at most 2.3e38");
     if (T == 0 || B == 0) return RAGRT_OK;
     RAGRT_REQUIRE(d_q && d_k && d_v && d_cu_seqlens && d_out, "null argument");
     RAGRT_REQUIRE((((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_out) & 15) == 0 &&

@@ -73,3 +73,76 @@ def test_attention_reference_moves_twice_in_a_block(D, causal):
     want, bound = L.attention64(q, k, v, cu, causal, scale=scale)
     for _ in range(20):
         L.check(encoder.packed_attention(q, k, v, cu, causal=causal, scale=scale), want, bound)
+
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("T,D", [(700, 64), (700, 128), (2500, 64), (2500, 128), (700, 40)])
+def test_attention_what_is_seen_and_not_finite(T, D, causal, dtype):
+    """NaN and infinities that rows do see: all of a row whose scores they are in, one column of the rows that see
+    them in V.  Nothing else changes."""
+    H, KV = 4, 2
+    q, k, v = (torch.randn(T, h, D, generator=gen(h + i), device="cuda").to(dtype) for i, h in enumerate((H, KV, KV)))
+    cu = L.cu_of([T], "cuda")
+    want, bound = L.attention64(q, k, v, cu, causal)
+    seen = lambda row: slice(row if causal else 0, None)
+    q[100, 1, 5] = math.nan
+    want[100, 1] = math.nan
+    v[10, 0, 3], v[20, 0, 3], v[20, 0, 4], v[300, 0, 8] = math.inf, -math.inf, -math.inf, math.nan
+    want[seen(10), :2, 3] = math.inf
+    want[seen(20), :2, 3] = math.nan
+    want[seen(20), :2, 4] = -math.inf
+    want[seen(300), :2, 8] = math.nan
+    want[100, 1] = math.nan
+    k[400, 1, 0] = math.nan
+    want[seen(400), 2:] = math.nan
+    got = encoder.packed_attention(q, k, v, cu, causal=causal)
+    inf = want.isinf()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[inf].double(), want[inf]) and torch.equal(got.isinf(), inf)
+    want[inf] = math.nan                                   # looked at
+    L.check(got, want, bound)
+    assert flag() == 0
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_infinity_under_a_weight_that_rounds_to_nothing(causal):
+    """A weight far below fp16's smallest times an infinity is an infinity."""
+    n = 200
+    scores = torch.full((n,), -40.0, device="cuda")
+    scores[0] = 0.0
+    v = torch.randn(n, 1, 64, generator=gen(4), device="cuda")
+    v[50, 0, 2], v[60, 0, 3] = math.inf, -math.inf
+    q, k, v = by_scores(scores, v, 64, torch.float16)
+    got = encoder.packed_attention(q, k, v, L.cu_of([n], "cuda"), causal=causal, scale=math.log(2.0))
+    for col, row, value in ((2, 50, math.inf), (3, 60, -math.inf)):
+        sees = slice(row if causal else 0, None)
+        assert (got[sees, 0, col] == value).all()
+        got[sees, 0, col] = 0
+    assert torch.isfinite(got).all()
+
+
+def test_attention_rows_that_are_not_finite_by_the_formula_are_not_computed_again():
+    """They cost a look at V at most (measured: 5 times the time of finite inputs; computed again, 500 times)."""
+    T, H, KV, D = 8192, 8, 2, 128
+    q, k, v = (torch.randn(T, h, D, generator=gen(h), device="cuda").half() for h in (H, KV, KV))
+    cu = L.cu_of([T], "cuda")
+
+    def ms(q, k, v):
+        times = []
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            encoder.packed_attention(q, k, v, cu, causal=True)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    clean = ms(q, k, v)
+    for at, what in ((0, slice(None)), (1, 3), (2, 3), (2, slice(T // 2, None))):
+        odd = [q, k, v]
+        odd[at] = odd[at].clone()
+        odd[at][what] = math.nan
+        assert ms(*odd) < 25 * clean, (at, what)
