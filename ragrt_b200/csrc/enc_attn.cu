@@ -212,7 +212,9 @@ __device__ __noinline__ unsigned attn_odd_rows(const AttnParams& p, int h, int r
 constexpr int kAFirst = 4;                     // first softmax warp: TMA, MMA and search warp before them, one idle
 constexpr int kAItems = 2;                     // items whose tiles are in shared memory
 // The reference maximum of a row moves only when it is exceeded by a factor of 2^8: until then the weights are
-// at most 256, well inside either type, and the accumulator is not rescaled.
+// at most 256, well inside either type, and the accumulator is not rescaled.  It is a whole number at or below a
+// maximum of the row: the row's largest weight is at least 1, and what fp16 rounds off the smallest ones at most
+// 2^-25 of it.
 constexpr float kARescale = 8.0f;
 
 // CTAs of one tile, several to an SM, so that the many short steps of short sequences (loads, products,
@@ -683,7 +685,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
                     const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale2;
                     float alpha = 1.0f;
                     if (__any_sync(0xFFFFFFFFu, bm > m + kARescale)) {
-                        const float mn = fmaxf(m, ceilf(bm));
+                        const float mn = fmaxf(m, floorf(bm));
                         alpha = m == -INFINITY ? 0.f : ex2(m - mn);
                         l *= alpha;
                         m = mn;

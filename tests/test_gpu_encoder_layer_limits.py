@@ -146,3 +146,17 @@ def test_attention_rows_that_are_not_finite_by_the_formula_are_not_computed_agai
         odd[at] = odd[at].clone()
         odd[at][what] = math.nan
         assert ms(*odd) < 25 * clean, (at, what)
+
+
+def test_attention_many_small_weights_beside_a_large_one():
+    """2000 keys whose weights are just under fp16's smallest step relative to the row's largest: each is off by at
+    most half that step, as the bound says, so that together they are not lost."""
+    n = 2001
+    scores = torch.full((n,), -24.03125, device="cuda")
+    scores[0] = 0.0078125                                   # 2^-7: both are exact in fp16
+    v = torch.ones(n, 1, 64, device="cuda")
+    v[0] = 0
+    q, k, v = by_scores(scores, v, 64, torch.float16)
+    cu, scale = L.cu_of([n], "cuda"), math.log(2.0)
+    want, bound = L.attention64(q, k, v, cu, False, scale=scale)
+    L.check(encoder.packed_attention(q, k, v, cu, scale=scale), want, bound)
