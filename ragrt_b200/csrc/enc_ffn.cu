@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(256) ffn_join(const __grid_constant__ FfnParam
 template <typename T, int kRows, int kCols>
 __global__ void __launch_bounds__(256) ffn_rows(const T* __restrict__ x, const T* __restrict__ wg,
                                                 const T* __restrict__ wu, const __grid_constant__ FfnParams p) {
-    const int f0 = (int)((blockIdx.x * 256 + threadIdx.x) >> 5) * kCols, lane = threadIdx.x & 31;
+    const int f0 = (int)(blockIdx.x * 8 + (threadIdx.x >> 5)) * kCols, lane = threadIdx.x & 31;
     pdl_wait_then_release();
     if (f0 >= p.F) return;                           // F is a multiple of 8
     const T* w[2] = {wg + (int64_t)f0 * p.K, wu + (int64_t)f0 * p.K};

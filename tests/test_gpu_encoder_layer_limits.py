@@ -160,3 +160,21 @@ def test_attention_many_small_weights_beside_a_large_one():
     cu, scale = L.cu_of([n], "cuda"), math.log(2.0)
     want, bound = L.attention64(q, k, v, cu, False, scale=scale)
     L.check(encoder.packed_attention(q, k, v, cu, scale=scale), want, bound)
+
+
+# ------------------------------------------------------------------------------------ gated feed-forward
+@pytest.mark.parametrize("keep", [False, True])
+def test_gated_ffn_of_one_row_and_many_columns(keep):
+    """More columns than 2^27: a warp per column."""
+    room_for(12)
+    F, K = (1 << 27) + 64, 8
+    x = torch.randn(1, K, generator=gen(1), device="cuda").half()
+    part = torch.randn(2, 1 << 20, K, generator=gen(2), device="cuda").half()
+    wg, wu = (t.repeat(129, 1)[:F] for t in part)
+    h, *kept = (lambda r: r if keep else (r,))(encoder.gated_ffn(x, wg, wu, keep=keep))
+    want = encoder.gated_ffn(x, part[0], part[1], keep=keep)
+    for got, one in zip((h, *kept), want if keep else (want,)):
+        for at in range(0, F, 1 << 20):
+            n = min(1 << 20, F - at)
+            assert torch.equal(got[0, at:at + n], one[0, :n]), at
+    assert flag() == 0
