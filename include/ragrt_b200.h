@@ -407,7 +407,8 @@ int ragrt_enc_qk_norm_rope(const void* d_q, const void* d_k, const void* d_q_wei
  * d_h [M, F] = act(d_x . d_w_gate^T) * (d_x . d_w_up^T), d_x [M, K], weights [F, K] (the halves of a
  * stacked [2 F, K] matrix will do): both projections, the activation and the product in one
  * kernel.  act 0: silu, 1: gelu (erf form), 2: gelu (tanh form).  d_gate / d_up f32 [M, F] (or both
- * NULL) keep the two products for ragrt_enc_gated_ffn_backward.  F and K multiples of 8.
+ * NULL) keep the two products for ragrt_enc_gated_ffn_backward.  F and K multiples of 8.  Sums, here and in the
+ * gradients, of up to 2^26 values (one row: of any length).
  */
 int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const void* d_w_up, void* d_h, float* d_gate,
                         float* d_up, int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype, void* stream);

@@ -50,6 +50,8 @@ constexpr int kFOut = 32 * 64 * 2;             // an epilogue warp's 32 rows x 6
 constexpr int kFSmem = 1024 + kFStages * (kFTileA + kFTileB) + 8 * kFOut + 256;
 constexpr int kFThreads = 320;                 // TMA warp, MMA warp, 8 epilogue warps
 constexpr uint32_t kFWaitLimit = 1u << 26;
+// Chunks of a contraction at most: at a microsecond each, far more than any takes, half of what a wait allows.
+constexpr int64_t kFLongest = 1 << 20;
 
 enum FfnMode : int { kForward = 0, kBackward = 1 };
 enum FfnAct : int { kSilu = 0, kGelu = 1, kGeluTanh = 2 };
@@ -893,6 +895,11 @@ int ffn_launch(int dtype, FfnParams p, int width, const void* x, const void* wg,
         pair = p.split == 1 && p.split_dw == 1 && 5 * sum >= pairs * std::max(p.dx ? of_dx : 0, p.dw ? of_dw : 0);
     }
     if (std::max(large, small) > 0x3FFFFFFF) return fail(RAGRT_ERR_CAPACITY, "too many tiles");
+    const int64_t longest = kMode == kForward ? ceil_div(p.K, kFK)
+                                              : std::max(p.dx ? 2 * ceil_div(p.F, kFK) / p.split : 0,
+                                                         p.dw ? ceil_div(p.M, kFK) / p.split_dw : 0);
+    if (longest > kFLongest)
+        return fail(RAGRT_ERR_CAPACITY, "gated_ffn: a sum over %lld values is too long", (long long)longest * kFK);
     // few rows: a load brings no more of them than there are (one row of 2048 -> 5504 10.6 us; with
     // 128-row boxes, most of them outside the tensor, 30)
     p.a_rows = std::min(kFM / 2, (int)ceil_div(p.M, 8) * 8);
@@ -940,6 +947,8 @@ int ffn_check(int32_t M, int32_t F, int32_t K, int32_t act, int32_t dtype) {
     RAGRT_REQUIRE(act >= kSilu && act <= kGeluTanh, "unknown activation %d", (int)act);
     RAGRT_REQUIRE(M >= 0 && F >= 8 && F % 8 == 0 && K >= 8 && K % 8 == 0,
                   "gated_ffn needs M >= 0 and F, K multiples of 8 (M=%d F=%d K=%d)", (int)M, (int)F, (int)K);
+    RAGRT_REQUIRE(std::max({M, F, K}) <= 0x7FFFFFFF - 4096, "gated_ffn: sizes up to 2^31 - 4097 (M=%d F=%d K=%d)",
+                  (int)M, (int)F, (int)K);          // positions past the last tile stay in 32 bits
     return RAGRT_OK;
 }
 

@@ -177,3 +177,13 @@ def test_python_checks_of_gated_ffn(on_host):
     square = torch.zeros(128, 64, dtype=H16)
     with pytest.raises(RuntimeError, match="overlaps"):
         encoder.gated_ffn(square, torch.zeros(64, 64, dtype=H16), torch.zeros(64, 64, dtype=H16), out=square)
+
+
+def test_gated_ffn_sizes_past_32_bits_are_refused():
+    big = 0x7FFFFFF8
+    f, b = _lib.lib().ragrt_enc_gated_ffn, _lib.lib().ragrt_enc_gated_ffn_backward
+    for M, F, K in ((big, 64, 64), (4, big, 64), (4, 64, big)):
+        assert f(P, P, P, P, None, None, M, F, K, 0, 0, None) == -1
+        assert b"2^31" in _lib.lib().ragrt_last_error()
+        assert b(*(P,) * 11, M, F, K, 0, 0, None, 0, None) == -1
+        assert b"2^31" in _lib.lib().ragrt_last_error()

@@ -178,3 +178,26 @@ def test_gated_ffn_of_one_row_and_many_columns(keep):
             n = min(1 << 20, F - at)
             assert torch.equal(got[0, at:at + n], one[0, :n]), at
     assert flag() == 0
+
+
+def test_gated_ffn_of_the_longest_sums():
+    """2^26 values a sum: as the formula has it and far inside the waits' limit; eight more are refused."""
+    room_for(16)
+    M, F, K = 8, 8, 1 << 26
+    x, w = (torch.zeros(8, K + 8, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    at = torch.tensor([0, 100, K // 2 + 63, K - 1], device="cuda")
+    x[:, at] = torch.randn(M, 4, generator=gen(1), device="cuda").bfloat16()
+    w[:, at] = torch.randn(F, 4, generator=gen(2), device="cuda").bfloat16()
+    want, _, _, bound, _, _ = L.ffn64(x[:, at], w[:, at], w[:, at], "silu")
+    L.check(encoder.gated_ffn(x[:, :K].contiguous(), w[:, :K].contiguous(), w[:, :K].contiguous()), want, bound)
+    assert flag() == 0
+    with pytest.raises(RuntimeError, match="too long"):
+        encoder.gated_ffn(x, w, w)
+    dh, kept = torch.zeros(M, K + 8, dtype=torch.bfloat16, device="cuda"), torch.zeros(M, K + 8, device="cuda")
+    tall = torch.zeros(K + 8, 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="too long"):
+        # dx's parts are no more than 16 tiles' worth: without scratch it is one sum
+        _lib.check(_lib.lib().ragrt_enc_gated_ffn_backward(
+            dh.data_ptr(), x[:, :8].contiguous().data_ptr(), tall.data_ptr(), tall.data_ptr(), kept.data_ptr(),
+            kept.data_ptr(), dh.data_ptr(), dh.data_ptr(), torch.zeros_like(x[:, :8]).data_ptr(), None, None, M, K + 8,
+            8, 0, 1, None, 0, torch.cuda.current_stream().cuda_stream))
