@@ -158,7 +158,8 @@ __device__ __forceinline__ void ffn_act_grad(float x, int act, float& a, float& 
     } else {
         const float s = sigmoid(1.5957691216057308f * (x + 0.044715f * x * x * x));
         a = x * s;
-        d = s + x * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * x * x));
+        const float y = fminf(fabsf(x), 1e4f);       // the square of more could be infinite, where 1 - s or s is 0
+        d = s + x * s * (1.0f - s) * (1.5957691216057308f * (1.0f + 0.134145f * y * y));
     }
 }
 

@@ -201,3 +201,37 @@ def test_gated_ffn_of_the_longest_sums():
             dh.data_ptr(), x[:, :8].contiguous().data_ptr(), tall.data_ptr(), tall.data_ptr(), kept.data_ptr(),
             kept.data_ptr(), dh.data_ptr(), dh.data_ptr(), torch.zeros_like(x[:, :8]).data_ptr(), None, None, M, K + 8,
             8, 0, 1, None, 0, torch.cuda.current_stream().cuda_stream))
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_gated_ffn_of_huge_and_infinite_values(act, rows):
+    """Pre-activations up to 1e30, whose cubes are beyond fp32, and infinite ones: what the 64-bit formula has."""
+    K, F = 64, 128
+    values = torch.tensor([1e20, -1e20, 1e30, -1e30, math.inf, -math.inf, math.nan, 3.0], device="cuda")
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, device="cuda")
+    x[:, 0], x[:, 1] = 1.0, 1.0
+    wg = torch.zeros(F, K, dtype=torch.bfloat16, device="cuda")
+    wg[:, 0] = values.repeat(F // 8)
+    wu = torch.zeros(F, K, dtype=torch.bfloat16, device="cuda")
+    wu[:, 1] = 0.5
+    h, gate, up = encoder.gated_ffn(x, wg, wu, act=act, keep=True)
+    g = wg[:, 0].double()
+    a, d = L.act64(g, act)
+    room = 1.02 * L.EPS[torch.bfloat16]
+    for got, want in ((gate, g), (h, 0.5 * a)):
+        want = want.expand(rows, F)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        ok = want.isfinite()
+        assert ((got.double() - want)[ok].abs() <= room * want[ok].abs()).all()
+        assert torch.equal(got[want.isinf()].double(), want[want.isinf()])
+    # gradients of the finite columns, the others out of them
+    fine = g.isfinite()
+    w1, w2 = wg.clone(), wu.clone()
+    w1[~fine], gate[:, ~fine], up[:, ~fine] = 0, 0, 0
+    dh = torch.ones(rows, F, dtype=torch.bfloat16, device="cuda")
+    dh[:, ~fine] = 0
+    dx, dwg, dwu = encoder.gated_ffn_backward(dh, x, w1, w2, gate, up, act=act)
+    for got, (want, bound), what in zip((dwg, dwu), L.ffn_backward64(dh, x, w1, w2, gate, up, act)[1:], ("dwg", "dwu")):
+        assert torch.isfinite(got).all()
+        L.check(got, want, bound, what)
