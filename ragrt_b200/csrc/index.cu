@@ -12,6 +12,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <mutex>
 #include <vector>
 
 #include "index.cuh"
@@ -39,17 +40,36 @@ int fail(int code, const char* fmt, ...) {
 static std::atomic<unsigned long long> g_launches{0};
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
+// A zeroed int on the current device.  A call that is being captured into a graph may be the first to need it: the
+// allocation and its clearing stand outside of any capture.
+static int* new_flag() {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+    int* f = nullptr;
+    cudaStream_t own = nullptr;
+    bool ok = cudaMalloc(&f, sizeof(int)) == cudaSuccess &&
+              cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess &&
+              cudaMemsetAsync(f, 0, sizeof(int), own) == cudaSuccess && cudaStreamSynchronize(own) == cudaSuccess;
+    if (own) cudaStreamDestroy(own);
+    if (!ok) {
+        cudaGetLastError();
+        if (f) cudaFree(f);
+        f = nullptr;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return f;
+}
+
 int* device_error_flag() {
-    static int* flags[64] = {nullptr};
+    static std::atomic<int*> flags[64];
+    static std::mutex making;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-    if (!flags[dev]) {
-        int* f = nullptr;
-        if (cudaMalloc(&f, sizeof(int)) != cudaSuccess) { cudaGetLastError(); return nullptr; }
-        cudaMemset(f, 0, sizeof(int));
-        flags[dev] = f;
-    }
-    return flags[dev];
+    int* f = flags[dev].load();
+    if (f) return f;
+    std::lock_guard<std::mutex> lock(making);
+    if (!(f = flags[dev].load())) flags[dev].store(f = new_flag());
+    return f;
 }
 
 int num_sms() {

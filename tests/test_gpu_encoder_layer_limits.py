@@ -1,6 +1,9 @@
 """The encoder's layer operators at the ends of their ranges: the largest sizes, values that are not
 finite, steps that follow one another closely.  Bounds: layer_helpers.py."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -235,3 +238,40 @@ def test_gated_ffn_of_huge_and_infinite_values(act, rows):
     for got, (want, bound), what in zip((dwg, dwu), L.ffn_backward64(dh, x, w1, w2, gate, up, act)[1:], ("dwg", "dwu")):
         assert torch.isfinite(got).all()
         L.check(got, want, bound, what)
+
+
+# ------------------------------------------------------------------------------------ captured first calls
+FIRST = """
+import sys
+import torch
+sys.path.insert(0, {repo!r})
+from ragrt_b200 import encoder
+q = torch.randn(70, 2, 64, device="cuda").half()
+cu = torch.tensor([0, 30, 70], dtype=torch.int32, device="cuda")
+cos = torch.rand(80, 32, device="cuda")
+pos = torch.arange(70, device="cuda")
+x, w = torch.randn(70, 64, device="cuda").half(), torch.randn(136, 64, device="cuda").half()
+dh, kept = torch.randn(70, 136, device="cuda").half(), torch.randn(70, 136, device="cuda")
+calls = dict(attention=lambda: encoder.packed_attention(q, q, q, cu), rope=lambda: encoder.qk_norm_rope(q, q, cos, cos, pos),
+             ffn=lambda: encoder.gated_ffn(x, w, w), backward=lambda: encoder.gated_ffn_backward(dh, x, w, w, kept, kept))
+call = calls[{name!r}]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = call()
+graph.replay()
+want = call()
+torch.cuda.synchronize()
+as_tuple = lambda r: r if isinstance(r, tuple) else (r,)
+assert all(torch.equal(a, b) for a, b in zip(as_tuple(got), as_tuple(want)))
+print("equal")
+"""
+
+
+@pytest.mark.parametrize("name", ["attention", "rope", "ffn", "backward"])
+def test_first_call_of_a_process_in_a_graph(name):
+    """Nothing has to be called once outside of a capture first."""
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST.format(repo=repo, name=name)], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-3000:]
