@@ -1,8 +1,9 @@
 """
 Build recipe of the product library: every CUDA source in ragrt_b200/csrc compiled for
 sm_100a into ragrt_b200/libragrt_b200.so (in-tree, so it travels with the repository
-snapshot).  Exposes the C ABI declared in include/ragrt_b200.h.  Beside it the host binding of the
-encoder's layer operators (csrc/enc_bind.cpp, against torch's headers): ragrt_b200/_enc_bind.so.
+snapshot).  Exposes the C ABI declared in include/ragrt_b200.h.  Beside it, where torch and a C++
+compiler are there, the host binding of the encoder's layer operators (csrc/enc_bind.cpp, against
+torch's headers): ragrt_b200/_enc_bind.so.
 
     python -m ragrt_b200.build [--force] [-j N]
 """
@@ -61,18 +62,20 @@ def _build_bind(force):
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")]
+    made = os.path.join(OBJ_DIR, os.path.basename(BIND))
     cmd = [CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + ["-I" + i for i in inc] + [
-        BIND_SRC, "-o", BIND, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+        BIND_SRC, "-o", made, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
         "-ltorch", "-ltorch_python"]
     h = hashlib.sha256(open(BIND_SRC, "rb").read() + _headers_digest().encode() + torch.__version__.encode() +
                        " ".join(cmd).encode()).hexdigest()
     stamp = os.path.join(OBJ_DIR, "_enc_bind.stamp")
     if force or not os.path.exists(BIND) or not os.path.exists(stamp) or open(stamp).read() != h:
+        os.makedirs(OBJ_DIR, exist_ok=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"{CXX} failed for {BIND_SRC}:\n{r.stdout}\n{r.stderr}")
-        os.makedirs(OBJ_DIR, exist_ok=True)
+        os.replace(made, BIND)
         with open(stamp, "w") as f:
             f.write(h)
 
@@ -82,7 +85,6 @@ def build(force=False, jobs=None, verbose=False):
     with cf.ThreadPoolExecutor(max_workers=jobs or min(8, os.cpu_count() or 1)) as ex:
         bind = ex.submit(_build_bind, force)
         objs = list(ex.map(lambda s: _compile(s, force, verbose), srcs))
-        bind.result()
     # Objects are cached by content, so a source put back to an earlier state reuses an older
     # object: relink whenever the set of objects differs from the one the library was linked from.
     stamp = os.path.join(OBJ_DIR, "libragrt_b200.objs")
@@ -95,6 +97,15 @@ def build(force=False, jobs=None, verbose=False):
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         with open(stamp, "w") as f:
             f.write(want)
+    # The library needs nvcc alone.  The binding needs torch, its and Python's headers and a C++ compiler, and only
+    # shortens the calls from Python: without one of these the library is all there is, and no binding of an earlier
+    # interface stays beside it.
+    try:
+        bind.result()
+    except (ImportError, OSError, RuntimeError) as e:
+        if os.path.exists(BIND):
+            os.remove(BIND)
+        print(f"ragrt_b200: built without its host binding: {e}", file=sys.stderr)
     return LIB
 
 
