@@ -1,8 +1,12 @@
 """Refusals of the encoder's layer operators, without a GPU: the C entry points check their arguments
 before any CUDA call, the Python entry points every tensor, and outputs apart from inputs."""
+import sys
+import warnings
+
 import pytest
 import torch
 
+import ragrt_b200
 from ragrt_b200 import _lib, encoder
 
 P = 0x1000                                              # 16-byte aligned, never touched
@@ -187,3 +191,41 @@ def test_gated_ffn_sizes_past_32_bits_are_refused():
         assert b"2^31" in _lib.lib().ragrt_last_error()
         assert b(*(P,) * 11, M, F, K, 0, 0, None, 0, None) == -1
         assert b"2^31" in _lib.lib().ragrt_last_error()
+
+
+def test_binding_is_built_and_loads():
+    from ragrt_b200 import _enc_bind
+    assert encoder._bind() is _enc_bind
+
+
+def test_without_the_binding_calls_take_the_way_through_python(monkeypatch):
+    """A missing binding is said once; refusals stay what they are."""
+    monkeypatch.setattr(encoder, "_bound", None)
+    monkeypatch.setitem(sys.modules, "ragrt_b200._enc_bind", None)
+    monkeypatch.delattr(ragrt_b200, "_enc_bind", raising=False)
+    q, cu = torch.zeros(4, 2, 64, dtype=H16), torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.warns(RuntimeWarning, match="without their host binding"):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            encoder.packed_attention(q, q, q, cu)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with pytest.raises(RuntimeError, match="CUDA"):
+            encoder.gated_ffn(torch.zeros(4, 64, dtype=H16), q[:, 0], q[:, 1])
+    x, w, h = torch.zeros(4, 64, dtype=H16), torch.zeros(128, 64, dtype=H16), torch.zeros(4, 128, dtype=H16)
+    cos = torch.zeros(4, 32)
+    monkeypatch.setattr(encoder, "_need_cuda", lambda *ts: None)
+    reached = []
+
+    class Library:
+        def __getattr__(self, name):
+            reached.append(name)
+            return lambda *args: 0
+
+    monkeypatch.setattr(_lib, "lib", lambda: Library())
+    monkeypatch.setattr(encoder, "_raw_stream", lambda t: 0)
+    assert encoder.packed_attention(q, q, q, cu).shape == q.shape
+    assert encoder.qk_norm_rope(q, q, cos, cos, torch.arange(4))[1].shape == q.shape
+    assert len(encoder.gated_ffn(x, w, w, keep=True)) == 3
+    assert encoder.gated_ffn_backward(h, x, w, w, h.float(), h.float())[2].shape == w.shape
+    assert reached == ["ragrt_enc_packed_attention", "ragrt_enc_qk_norm_rope", "ragrt_enc_gated_ffn",
+                       "ragrt_enc_gated_ffn_workspace", "ragrt_enc_gated_ffn_backward"]

@@ -275,3 +275,23 @@ def test_first_call_of_a_process_in_a_graph(name):
     r = subprocess.run([sys.executable, "-c", FIRST.format(repo=repo, name=name)], capture_output=True, text=True,
                        timeout=300)
     assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-3000:]
+
+
+# ------------------------------------------------------------------------------------ the host's two ways
+def test_operators_with_and_without_the_host_binding(monkeypatch):
+    q, k, v = (torch.randn(90, h, 64, generator=gen(h), device="cuda").half() for h in (4, 2, 2))
+    cu = L.cu_of([33, 57], "cuda")
+    cos = torch.rand(90, 32, generator=gen(5), device="cuda")
+    x, w = torch.randn(90, 64, generator=gen(6), device="cuda").half(), torch.randn(272, 64, generator=gen(7), device="cuda").half()
+    dh = torch.randn(90, 136, generator=gen(8), device="cuda").half()
+
+    def all_of_them():
+        h, gate, up = encoder.gated_ffn(x, w[:136], w[136:], act="gelu", keep=True)
+        return (encoder.packed_attention(q, k, v, cu, causal=True), *encoder.qk_norm_rope(q, k, cos, cos, torch.arange(90, device="cuda")),
+                h, gate, up, *encoder.gated_ffn_backward(dh, x, w[:136], w[136:], gate, up, act="gelu"))
+
+    want = all_of_them()
+    assert encoder._bound is not encoder._NoBinding
+    monkeypatch.setattr(encoder, "_bound", encoder._NoBinding)
+    for a, b in zip(all_of_them(), want):
+        assert torch.equal(a, b)
