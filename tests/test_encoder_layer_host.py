@@ -1,5 +1,7 @@
 """Refusals of the encoder's layer operators, without a GPU: the C entry points check their arguments
 before any CUDA call, the Python entry points every tensor, and outputs apart from inputs."""
+import math
+import random
 import sys
 import warnings
 
@@ -229,3 +231,19 @@ def test_without_the_binding_calls_take_the_way_through_python(monkeypatch):
     assert encoder.gated_ffn_backward(h, x, w, w, h.float(), h.float())[2].shape == w.shape
     assert reached == ["ragrt_enc_packed_attention", "ragrt_enc_qk_norm_rope", "ragrt_enc_gated_ffn",
                        "ragrt_enc_gated_ffn_workspace", "ragrt_enc_gated_ffn_backward"]
+
+
+def test_gated_ffn_workspace_is_bounded():
+    """Three parts of 64 KiB per SM at most, whatever the sizes; the bound is nearly reached."""
+    rng = random.Random(5)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count if torch.cuda.is_available() else 148
+    size = lambda high: min(high, int(math.exp(rng.uniform(math.log(8), math.log(high + 1)))))
+    ws, most = _lib.lib().ragrt_enc_gated_ffn_workspace, 0
+    for _ in range(30000):
+        M, F, K = size(1 << 20), size(1 << 15) // 8 * 8, size(1 << 14) // 8 * 8
+        for dx, dw in ((1, 0), (0, 1), (1, 1)):
+            n = ws(M, F, K, dx, dw)
+            assert 0 <= n <= 3 * sms * 65536 and n % 16 == 0, (M, F, K, dx, dw, n)
+            most = max(most, n)
+    assert most > 1.8 * sms * 65536
+    assert ws(0, 64, 64, 1, 1) == 0 and ws(100, 64, 64, 0, 0) == 0
