@@ -295,3 +295,22 @@ def test_operators_with_and_without_the_host_binding(monkeypatch):
     monkeypatch.setattr(encoder, "_bound", encoder._NoBinding)
     for a, b in zip(all_of_them(), want):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------ one launch for all gradients
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,F,K", [(3000, 2600, 1000), (6000, 1400, 1000), (5000, 2600, 1496), (9000, 2712, 776)])
+def test_gated_ffn_gradients_of_several_rounds_of_pairs(M, F, K, dtype):
+    """Tiles of dx and of the weight gradients in one list of large tiles, more than a round of the 74 pairs, the last
+    round in part: 48 + 88, 96 + 48, 120 + 132 and 144 + 88 tiles, the border in the first round or the second."""
+    x = torch.randn(M, K, generator=gen(M), device="cuda").to(dtype)
+    w = (torch.randn(2 * F, K, generator=gen(F), device="cuda") * 1.5 / math.sqrt(K)).to(dtype)
+    dh = torch.randn(M, F, generator=gen(K), device="cuda").to(dtype)
+    assert _lib.lib().ragrt_enc_gated_ffn_workspace(M, F, K, 1, 1) == 0             # nothing in parts
+    _, gate, up = encoder.gated_ffn(x, w[:F], w[F:], keep=True)
+    grads = encoder.gated_ffn_backward(dh, x, w[:F], w[F:], gate, up)
+    for got, (want, bound), what in zip(grads, L.ffn_backward64(dh, x, w[:F], w[F:], gate, up, "silu"), ("dx", "dwg", "dwu")):
+        L.check(got, want, bound, what)
+    for a, b in zip(grads, encoder.gated_ffn_backward(dh, x, w[:F], w[F:], gate, up)):
+        assert torch.equal(a, b)
+    assert flag() == 0
