@@ -478,7 +478,7 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             constexpr uint32_t idO = tc::idesc_f16_f32(kAM, DP) | idesc_type<T>() | kIdescBMn;
             const uint32_t lead = tc::elect_one();
             AttnWalk<Cfg> walk;                                    // of the scores; the products with V are
-            int vj = 0, vjb[kTiles], vje[kTiles];                 // one block behind it, at vj
+            int vj = 0, vjb[kTiles] = {}, vje[kTiles] = {};                 // one block behind it, at vj
             walk.lead = lead != 0;
             uint32_t np[kTiles] = {};                             // products of each tile
             int nk = 0, nv = 0, nq = 0;
