@@ -379,8 +379,11 @@ int ragrt_enc_attention(const void* d_qkv, const int64_t* d_mask, void* d_ctx, i
  * up to t of its sequence, else all of it.  d_out [T, heads, head_dim] = softmax(scale q k^T) v.
  * A sequence may be empty; rows outside every sequence are not read as queries and not written.
  * What no row may see (other sequences, later rows) does not reach its output, NaN and infinities
- * included; a row that sees a score that is NaN or +infinite (2.3e38 or more after scaling) is all NaN.  A table that is not ascending within [0, T] sets the device error flag to 6 and
- * leaves the rows it cannot place unwritten.  head_dim a multiple of 8 up to 128.
+ * included; a row that sees a score that is NaN or +infinite (2.3e38 or more after scaling) is all NaN.
+ * Where values of d_v that are not finite lie within 127 rows of what a row may see, it may be computed again,
+ * slowly: a full sequence of 8000 rows before such rows takes 100 times as long.  A table that is not ascending
+ * within [0, T] sets the device error flag to 6 and leaves the rows it cannot place unwritten.  head_dim a multiple
+ * of 8 up to 128.
  */
 int ragrt_enc_packed_attention(const void* d_q, const void* d_k, const void* d_v, const int32_t* d_cu_seqlens,
                                void* d_out, int32_t T, int32_t B, int32_t heads, int32_t kv_heads, int32_t head_dim,

@@ -24,7 +24,7 @@
 //   attn_odd_rows      A weight of zero does not keep a NaN or an infinity in a masked row of V out of a
 //                      matrix product.  Of the rows that come out of it not finite this finds those that
 //                      are so by the formula, and what they are;
-//   attn_row           computes the others once more, over their own keys alone: one row of one head by
+//   attn_rows          computes the others once more, over their own keys alone: four rows of one head by
 //                      a warp, in fp32.
 #include <algorithm>
 
@@ -88,56 +88,90 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnParams& p, int64_t slot,
 // bits below n of a word, n of any size
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 
-// One row of one head by one warp.
-template <typename T>
-__device__ __noinline__ void attn_row(const AttnParams& p, int t, int h, int lo, int hi) {
-    const int lane = threadIdx.x & 31;
-    const int g = h / (p.heads / p.kv_heads);
-    const T* q = static_cast<const T*>(p.q) + t * p.q_stride + (int64_t)h * p.dim;
+// The first R of a warp's rows of one head (bit i of `rows`: row row0 + i, with the keys [lo, end), causal
+// [lo, row0 + i]), by the warp: a lane per key for the scores, per four columns for the sums.  Returns the other rows.
+// They share what is loaded of K and V, kScores and kSums loads ahead: it is their latency that counts.  8192 rows,
+// 8 heads of 128, causal, with a NaN in V in the middle (84 rows before it in its tile): 5.8 ms in all, a row by itself
+// and load by load 38; two full sequences of 8000 and 192 rows, V of the second NaN, so that all of the first is
+// computed again: 29 ms (165), 0.27 where all is finite.  Tried and dropped: zeros over the rest of the last block of V
+// in shared memory before the products read it: 0.36 ms for that call, but 1024 passages 195 -> 229 us.
+template <typename T, int R, int kScores, int kSums>
+__device__ __noinline__ unsigned attn_rows(const AttnParams& p, int h, int row0, unsigned rows, int lo, int end) {
+    const int lane = threadIdx.x & 31, g = h / (p.heads / p.kv_heads);
+    const T* q = static_cast<const T*>(p.q) + (int64_t)h * p.dim;
     const T* k = static_cast<const T*>(p.k) + (int64_t)g * p.dim;
-    const T* v = static_cast<const T*>(p.v) + (int64_t)g * p.dim;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};         // dims lane, lane + 32, ...
-    for (int base = lo; base < hi; base += 32) {
+    const bool there = 4 * lane < p.dim;
+    const T* v = static_cast<const T*>(p.v) + (int64_t)g * p.dim + (there ? 4 * lane : 0);
+    int row[R], n = 0, last = end;                   // behind the last one: the first again, not stored
+    float m[R], l[R], o[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        row[r] = rows ? row0 + __ffs(rows) - 1 : row[0];
+        if (p.causal && rows) last = row[r] + 1;
+        n += rows ? 1 : 0;
+        rows &= rows - 1;
+        m[r] = -INFINITY;
+        l[r] = o[r][0] = o[r][1] = o[r][2] = o[r][3] = 0.f;
+    }
+#pragma unroll 1
+    for (int base = lo; base < last; base += 32) {
         const int j = base + lane;
-        float s = -INFINITY;
-        if (j < hi) {
-            const T* kr = k + j * p.k_stride;
-            s = 0.f;
-            for (int c = 0; c < p.dim; c += 8) {
-                float f[8], a[8];
-                up8<T>(__ldg(reinterpret_cast<const uint4*>(kr + c)), f);
-                up8<T>(__ldg(reinterpret_cast<const uint4*>(q + c)), a);
+        float s[R] = {};
+        const T* kr = k + min(j, last - 1) * p.k_stride;
+#pragma unroll kScores
+        for (int c = 0; c < p.dim; c += 8) {
+            float f[8], a[8];
+            up8<T>(__ldg(reinterpret_cast<const uint4*>(kr + c)), f);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s = fmaf(f[e], a[e], s);
+            for (int r = 0; r < R; ++r) {
+                up8<T>(__ldg(reinterpret_cast<const uint4*>(q + row[r] * p.q_stride + c)), a);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[r] = fmaf(f[e], a[e], s[r]);
             }
-            s *= p.scale;
         }
-        float mx = s;
 #pragma unroll
-        for (int x = 16; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, x));
-        mx = fmaxf(mx, m);
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        const float e = __expf(s - ref), alpha = __expf(m - ref);
-        float sum = e;
+        for (int r = 0; r < R; ++r) {
+            s[r] = j < (p.causal ? row[r] + 1 : end) ? s[r] * p.scale : -INFINITY;
+            float mx = s[r];
 #pragma unroll
-        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
-        l = l * alpha + sum;
-        m = mx;
+            for (int x = 16; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, x));
+            mx = fmaxf(mx, m[r]);
+            const float ref = mx == -INFINITY ? 0.f : mx, alpha = __expf(m[r] - ref);
+            s[r] = __expf(s[r] - ref);               // the weight
+            float sum = s[r];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= alpha;
-        const int n = min(32, hi - base);
-        for (int i = 0; i < n; ++i) {
-            const float pj = __shfl_sync(0xFFFFFFFFu, e, i);
-            const T* vr = v + (int64_t)(base + i) * p.v_stride;
+            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+            l[r] = l[r] * alpha + sum;
+            m[r] = mx;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (lane + 32 * c < p.dim) o[c] = fmaf(pj, (float)vr[lane + 32 * c], o[c]);
+            for (int c = 0; c < 4; ++c) o[r][c] *= alpha;
+        }
+        const int keys = min(32, last - base);
+#pragma unroll kSums
+        for (int i = 0; i < keys; ++i) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(v + (base + i) * p.v_stride));
+            const float2 f = Pair16<T>::up(*reinterpret_cast<const typename Pair16<T>::type*>(&u.x));
+            const float2 e = Pair16<T>::up(*reinterpret_cast<const typename Pair16<T>::type*>(&u.y));
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float w = __shfl_sync(0xFFFFFFFFu, s[r], i);
+                const bool sees = base + i < (p.causal ? row[r] + 1 : end);      // not a matter of its weight: V may be NaN
+                o[r][0] = sees ? fmaf(w, f.x, o[r][0]) : o[r][0];
+                o[r][1] = sees ? fmaf(w, f.y, o[r][1]) : o[r][1];
+                o[r][2] = sees ? fmaf(w, e.x, o[r][2]) : o[r][2];
+                o[r][3] = sees ? fmaf(w, e.y, o[r][3]) : o[r][3];
+            }
         }
     }
-    T* dst = static_cast<T*>(p.out) + t * p.out_stride + (int64_t)h * p.dim;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (lane + 32 * c < p.dim) dst[lane + 32 * c] = (T)(o[c] / l);
+    for (int r = 0; r < R; ++r) {
+        if (r >= n || !there) break;
+        typename Pair16<T>::type y[2] = {Pair16<T>::down(o[r][0] / l[r], o[r][1] / l[r]),
+                                         Pair16<T>::down(o[r][2] / l[r], o[r][3] / l[r])};
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + row[r] * p.out_stride + (int64_t)h * p.dim + 4 * lane) =
+            *reinterpret_cast<const uint2*>(y);
+    }
+    return rows;
 }
 
 // Rows of one head, of a warp, whose output is not finite although the sum of their weights is: bit i of `rows` is
@@ -146,7 +180,7 @@ __device__ __noinline__ void attn_row(const AttnParams& p, int t, int h, int lo,
 // a row of V that may not be seen, through a weight of zero: the rows returned, which are to be computed again.  A
 // row of V that is not finite does that to the rows before it in its tile alone, and there only in columns in which
 // no row before it was: few rows of a causal sequence.  It does it to all rows of a full sequence that ends less than
-// a block of keys before it.  The warp looks at each seen row of V once.  8192 rows, 8 heads of 128, causal, 0.19 ms
+// a block of keys before it (attn_rows has what that costs).  The warp looks at each seen row of V once.  8192 rows, 8 heads of 128, causal, 0.19 ms
 // when all is finite: one NaN in an early row of V 0.69 ms, the later half of V NaN 0.89 (all such rows computed
 // again: 105 and 81).  No branch but the whole warp's and no vote: those made the kernel hold a convergence barrier's
 // state in memory across the call (1024 passages 194 -> 203 us).
@@ -239,6 +273,8 @@ struct AttnCfg {
     static constexpr int kRegs = kTiles == 2 ? 168 : DP == 128 ? 128 : 64;
     static constexpr int kRegsFew = kTiles == 2 ? 88 : DP == 128 ? 80 : 40;
     static constexpr int kRegsMany = kTiles == 2 ? 208 : DP == 128 ? 176 : 88;
+    // rows at a time, and loads ahead, that attn_rows has the registers for
+    static constexpr int kAgain = kTiles == 2 || DP == 128 ? 4 : 2, kAgainAhead = kAgain == 4 ? 8 : 2;
     static_assert(128 * kRegsFew + (kThreads - 128) * kRegsMany <= kThreads * kRegs, "more registers than the launch holds");
 };
 
@@ -246,7 +282,7 @@ struct AttnMaps {
     CUtensorMap q, k, v;
 };
 
-// Bounded wait: 2 s, not counting the time that a warp of the CTA spends in attn_odd_rows and attn_row (abort[1]:
+// Bounded wait: 2 s, not counting the time that a warp of the CTA spends in attn_odd_rows and attn_rows (abort[1]:
 // how many do), or until another role gave up (abort[0]).  In few instructions: the roles' code shares the
 // instruction cache, and this is in it some twenty times.
 __device__ __forceinline__ bool attn_wait(uint64_t* m, uint32_t parity, volatile int* abort) {
@@ -823,10 +859,9 @@ packed_attn_mma(const __grid_constant__ AttnMaps maps, const __grid_constant__ A
             unsigned left = __ballot_sync(0xFFFFFFFFu, bad && inv < INFINITY);
             if (left) {
                 if (lane == 0) atomicAdd(&sh->abort[1], 1);
-                for (left = attn_odd_rows<T>(p, b.head, row - lane, left, own.lo, hi); left; left &= left - 1) {
-                    const int src = __ffs(left) - 1;
-                    attn_row<T>(p, __shfl_sync(0xFFFFFFFFu, row, src), b.head, own.lo, __shfl_sync(0xFFFFFFFFu, hi, src));
-                }
+                left = attn_odd_rows<T>(p, b.head, row - lane, left, own.lo, hi);
+                while (left)
+                    left = attn_rows<T, Cfg::kAgain, Cfg::kAgainAhead, 2 * Cfg::kAgainAhead>(p, b.head, row - lane, left, own.lo, hi);
                 if (lane == 0) atomicAdd(&sh->abort[1], -1);
             }
         }
