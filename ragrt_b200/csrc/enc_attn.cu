@@ -13,19 +13,23 @@
 //                      softmax (two warps share an exponential unit that needs 1,024 for each), then P V and
 //                      the next Q K^T (16 products of about 95 cycles; a 128-row operand from shared memory
 //                      takes that long whatever the width of the other).  One sequence of 16,384 rows, 16
-//                      heads of 128, causal: 0.92 ms, 1,190 TFLOP/s.  CTAs of one tile, for short sequences,
-//                      are bound by instruction issue and fetch: 1,024 passages of 20-180 rows, 12 heads:
-//                      195 us, 3.2 TB/s.  Tried and dropped: tiles over the rows as they lie, several sequences
-//                      in one (masks cost more than the rows saved: 263 us); 64-key blocks with two score
-//                      buffers for wide heads (1.59 ms: twice the products at the same 95 cycles); a quarter
-//                      of the exponentials as polynomials on the FMA units (0.97 ms: issue, not that unit,
-//                      is short); two tiles of one CTA with an issuing warp each (1.20 ms: they fall into
-//                      step and want the same units at the same time).
+//                      heads of 128, causal: 1.03 ms, 1,070 TFLOP/s, the tensor pipe at work 57 % of its
+//                      cycles (12 prompts of 1-4,096, 46 %: the turns end with each item).  CTAs of one tile, for
+//                      short sequences, wait: an item is one chain of load, product, softmax, product, store, and
+//                      of the 17 warps that share an issued instruction 6.6 wait for memory or tensor memory, with
+//                      47 % of the issue slots, 19 % of the tensor pipe and 36 % of the memory's rate used.  1,024
+//                      passages of 20-180 rows, 12 heads: 195 us, 3.2 TB/s (218 in a long run).  Tried and
+//                      dropped: tiles over the rows as they lie, several sequences in one (masks cost more than
+//                      the rows saved: 263 us); 64-key blocks with two score buffers for wide heads
+//                      (1.59 ms for the long sequence: twice the products at the same 95 cycles); a quarter of
+//                      the exponentials as polynomials on the FMA units (0.97 ms, no gain); two tiles of one
+//                      CTA with an issuing warp each (1.20 ms: they fall into step and want the same units at
+//                      the same time).
 //   attn_odd_rows      A weight of zero does not keep a NaN or an infinity in a masked row of V out of a
 //                      matrix product.  Of the rows that come out of it not finite this finds those that
 //                      are so by the formula, and what they are;
-//   attn_rows          computes the others once more, over their own keys alone: four rows of one head by
-//                      a warp, in fp32.
+//   attn_rows          computes the others once more, over their own keys alone: a few rows of one head at
+//                      a time by a warp, in fp32.
 #include <algorithm>
 
 #include "enc_common.cuh"
@@ -385,8 +389,8 @@ __device__ __forceinline__ void add_pair(uint32_t w, float& a, float& b) {
 // w = 2^(s scale + ref) of 32 scores, rounded and packed in pairs; returns their sum.  Summing the rounded weights
 // (kRounded) makes the division take out the rounding of a weight that dominates its row: a row of one key is that
 // key's v exactly, and the error of 8 to 64 keys is 1.25 to 1.37 times that of the output's own rounding
-// instead of 1.42.  It costs one more instruction per pair (1024 passages 194 -> 198 us).  Blocks of 128 keys that all
-// rows see sum the weights as they come: rounded, 16384 tokens 917 -> 967 us, 12 prompts 802 -> 919.
+// instead of 1.42.  It costs one more instruction per pair (1024 passages 193 -> 195 us).  Blocks of 128 keys that all
+// rows see sum the weights as they come: rounded, 16384 tokens 1,040 -> 1,070 us, 12 prompts 850 -> 935.
 template <typename T, bool kRounded>
 __device__ __forceinline__ float attn_weights(const float* s, uint64_t scale, uint64_t ref, uint32_t* w) {
     float sum[4] = {};

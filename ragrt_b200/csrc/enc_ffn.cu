@@ -19,10 +19,11 @@
 //                           cores, bound by the weights' bytes.
 //   ffn_act_backward        dg and du, elementwise; at memory speed (8192 x 5504: 97 us, 6.5 TB/s).
 //
-// Measured: 16384 x 2048 -> 8192 forward 688 us in a burst (1,600 TFLOP/s; 810 us, 1,360 TFLOP/s, under the
-// power cap); a training step of 8192 x 2048 -> 5504 236 us forward, 36 more for keeping g and u, 645
-// backward, 99 of them elementwise (cuBLAS for the three products alone: 248, 202 and 226 us; one behind the other for
-// longer, at the power cap, 301, 286 and 306, and the backward pass here 694).
+// Measured: 16384 x 2048 -> 8192 forward 688 us in a burst (1,600 TFLOP/s, the tensor pipe at work 98 % of its
+// cycles; 805 us, 1,370 TFLOP/s, under the power cap); a training step of 8192 x 2048 -> 5504 236 us forward, 36 more
+// for keeping g and u, 645 backward, 99 of them elementwise, the tensor pipe at work 87 % of the rest (cuBLAS for the
+// three products alone: 248, 202 and 226 us; one behind the other for longer, at the power cap, 301, 286 and 306, and
+// the backward pass here 694).
 //
 // The weight matrices and x are read as they lie: an operand whose contraction index is the row of
 // its matrix is fed to the tensor cores MN-major.  Accumulators are fp32.  g and u are kept in fp32: in 16
@@ -783,7 +784,8 @@ int64_t ffn_part_bytes(int width) { return (int64_t)(kFM / 2) * width * 4; }
 // of of_dw chunks, dealt out to two CTAs per SM in turn.  A tile of the weight gradients takes 16 chunks at least, its
 // epilogue; a part 4 more; every entry of the list costs the SM 2; the joining kernel 8 and one per 64 parts.  Parts of
 // 8 chunks or more, at most two per SM in all (and 16 of a tile).  Against all counts, measured for 20 shapes from 25 x
-// 768 -> 2048 to 256 x 4096 -> 8192: within 5 % of the best for dx, 13 % for all gradients.
+// 768 -> 2048 to 256 x 4096 -> 8192 with the same inputs again and again (in L2, but for the largest): within 5 % of
+// the best for dx, 13 % for all gradients.
 int ffn_parts(int tiles, int nk, int per, int of_dw) {
     const int sms = num_sms(), ctas = 2 * sms;
     int best = 1, least = 0;
@@ -806,8 +808,8 @@ int ffn_parts(int tiles, int nk, int per, int of_dw) {
 // Whether the weight gradients' contraction, over the rows, is cut: where many rows meet small matrices, so that even
 // the 128 x 128 tiles are no more than the SMs.  An SM takes 0.41 us for a chunk of those, a pair as long for one of 256 x
 // 256 (so twice the rate); the former are spread evenly by the cut and pay 8 us for it, the latter's longest share counts.
-// All gradients whole and cut: 16000 rows 256 -> 256 87 and 25.5 us, 16384 rows 384 -> 1536 187 and 153, 4000 rows 512 ->
-// 512 32 and 25; not cut by this rule: 8192 rows 512 -> 2048 110, 3000 rows 512 -> 1024 26.
+// All gradients whole and cut, inputs from memory: 16000 rows 256 -> 256 94 and 30 us, 16384 rows 384 -> 1536 190 and
+// 150, 4000 rows 512 -> 512 32 and 25; not cut by this rule: 8192 rows 512 -> 2048 129, 3000 rows 512 -> 1024 30.
 bool ffn_cut_dw(int M, int F, int K, bool dx) {
     const int64_t sms = num_sms(), pairs = sms / 2, nk = 2 * ceil_div(F, kFK), of_dw = ceil_div(M, kFK);
     const int64_t per = ffn_dw_tiles(F, K, 128);
@@ -826,12 +828,12 @@ bool ffn_cut_dw(int M, int F, int K, bool dx) {
 // dx is cut where it has fewer tiles than there are SMs: its time is that of the 2 F steps of one tile then, 0.3 us
 // a chunk.  Not under 32 chunks (60 rows 512 -> 512 in two parts 10.1 us, whole 8.2).  The weight gradients join its
 // launch while they are 27 chunks per SM or fewer; else dx runs apart if its chain shrinks by 64 chunks, or is left
-// whole (1500 rows 768 -> 2048: large tiles for all 32 us, dx apart 36).  With their elementwise kernel, whole and in
-// parts, dx / all gradients: 25 rows 768 -> 2048 20.8 / 22.0 and 9.9 / 11.5 us, 128 rows 2048 -> 5504 50 / 68 and 16.5 /
-// 32, 300 rows 63 / 77 and 30 / 54, 25 rows 4096 -> 8192 86 / 124 and 34 / 76, 1000 rows 768 -> 2048 24 / 30 and 20 / 24
-// (cuBLAS's dx: 9.3, 17, 18.5, 26, 10.7).
+// whole (1500 rows 768 -> 2048: large tiles for all 36 us, dx apart 40).  With their elementwise kernel, inputs from
+// memory, whole and in parts, dx / all gradients: 25 rows 768 -> 2048 24 / 26 and 10.9 / 14.4 us, 128 rows 2048 -> 5504
+// 59 / 72 and 21 / 35, 300 rows 65 / 78 and 32 / 55, 25 rows 4096 -> 8192 87 / 123 and 34 / 76, 1000 rows 768 -> 2048
+// 29 / 33 and 23 / 30 (cuBLAS's dx, operands in L2: 9.3, 17, 18.5, 26, 10.7; here then 9.5, 17, 30, 33, 20).
 // Tiles of 64 columns where those are one round of CTAs and 64 chunks per SM; else of 128, whose products take no
-// longer (100 cycles: the 128-row operand comes from shared memory at that rate): all gradients of 1000 rows 768 ->
+// longer (100 cycles: the 128-row operand comes from shared memory at that rate).  In L2: all gradients of 1000 rows 768 ->
 // 2048 by 64 27.8 us, by 128 24.4; 128 rows 2048 -> 5504 39.2 and 32.0; 1200 rows 384 -> 1536 17.4 and 18.9; dx alone
 // of 25 rows 768 -> 2048 9.9 and 10.4, of 256 rows 4096 -> 8192 60 and 52.
 FfnPlan ffn_plan(int M, int F, int K, bool dx, bool dw) {
@@ -881,15 +883,15 @@ int ffn_launch(int dtype, FfnParams p, int width, const void* x, const void* wg,
     if (p.dw) small += (p.split_dw - 1) * ffn_dw_tiles(p.F, p.K, width);
     bool pair;
     if (kMode == kForward) {
-        // small tiles while they are one round of two CTAs per SM: 128 rows 2048 -> 5504 (172 tiles) 12.9 us
-        // against 16.2, 512 rows 768 -> 2048 (256) 7.2 against 9.3; 256 rows 2048 -> 5504 (344) 19.9
-        // against 16.5, 1000 rows 768 -> 2048 (512) 11.5 against 10.3
+        // small tiles while they are one round of two CTAs per SM.  Weights from memory: 128 rows 2048 -> 5504 (172
+        // tiles) 15.6 us against 17.6, 512 rows 768 -> 2048 (256) 7.7 against 10.4; 256 rows 2048 -> 5504 (344) 23.9
+        // against 18.2, 1000 rows 768 -> 2048 (512) 11.9 against 11.0
         pair = small > 2 * sms;
     } else {
         // small tiles where the large ones' longest contraction is far above their average per pair of SMs
-        // (five times): all gradients of 512 rows 768 -> 2048 (6.4 times) 25.8 us against 27.5, 128 rows
-        // 2048 -> 5504 (6.1) 67.7 against 70.8; 1000 rows (3.1) 29.2 against 28.9, 256 rows (4.6) 82.3
-        // against 73.1
+        // (five times).  Calls that got no scratch, inputs in L2: all gradients of 512 rows 768 -> 2048 (6.4 times)
+        // 27.4 us against 28.7; 1000 rows (3.1) 30.3 against 31.4, 256 rows 2048 -> 5504 (4.6) 93.9 against 74.2.
+        // From memory the large tiles gain: 36.0 against 30.7, 37.6 and 33.5, 95.4 and 74.9.
         const int64_t of_dx = 2 * ceil_div(p.F, kFK), of_dw = ceil_div(p.M, kFK);
         const int64_t n_dx = p.dx ? ceil_div(p.M, kFM) * ceil_div(p.K, kFN) : 0;
         const int64_t sum = n_dx * of_dx + (large - n_dx) * of_dw;
@@ -901,7 +903,7 @@ int ffn_launch(int dtype, FfnParams p, int width, const void* x, const void* wg,
                                                          p.dw ? ceil_div(p.M, kFK) / p.split_dw : 0);
     if (longest > kFLongest)
         return fail(RAGRT_ERR_CAPACITY, "gated_ffn: a sum over %lld values is too long", (long long)longest * kFK);
-    // few rows: a load brings no more of them than there are (one row of 2048 -> 5504 10.6 us; with
+    // few rows: a load brings no more of them than there are (one row of 2048 -> 5504, weights in L2, 11.2 us; with
     // 128-row boxes, most of them outside the tensor, 30)
     p.a_rows = std::min(kFM / 2, (int)ceil_div(p.M, 8) * 8);
     if ((rc = ffn_maps(m, kMode, pair, dtype, p, x, wg, wu, dg, du))) return rc;
@@ -973,8 +975,9 @@ extern "C" int ragrt_enc_gated_ffn(const void* d_x, const void* d_w_gate, const 
     if (!err) return fail(RAGRT_ERR_CUDA, "device error flag unavailable");
     cudaStream_t stream = (cudaStream_t)stream_;
     FfnParams p{M, F, K, act, d_gate != nullptr, 0, 0, 0, 1, 1, nullptr, {d_h, d_gate, d_up}, err};
-    // One row at any size: 2048 -> 5504 5.8 us, on the tensor cores 11.0.  Up to four where the weights are few: 4
-    // rows 768 -> 2048 4.4 us against 5.2, 2048 -> 4096 9.1 against 10.2; 2048 -> 5504 12.8 against 11.0.
+    // One row at any size: 2048 -> 5504 9.2 us with the weights from memory, 6.9 us of bytes, on the tensor cores 14.4.
+    // Up to four where the weights are few: 4 rows 768 -> 2048 5.7 us against 6.5, 2048 -> 4096 12.6 against 13.3; 2 rows
+    // 2048 -> 5504 17.4 against 14.5.
     if (M == 1 || (M <= kFewRows && (int64_t)F * K <= (1 << 23))) {
         return dtype == RAGRT_BF16 ? ffn_rows_launch<__nv_bfloat16>(d_x, d_w_gate, d_w_up, p, stream)
                                    : ffn_rows_launch<__half>(d_x, d_w_gate, d_w_up, p, stream);

@@ -8,8 +8,10 @@
 // chunks of a head that rotate with one another, so that a head is ceil(dim / 16) lanes, the
 // rotation needs no exchange, the mean a few shuffles, and a lane's cos / sin stay in registers
 // while its warp walks the heads of one token.  Measured: 102,411 tokens of 24 heads of 64 (32 values
-// turned) 125 us, 5.0 TB/s; 32,768 tokens of 40 heads of 128 125 us, 5.5 TB/s.  What is left of the way to
-// a copy's 6.5 is issue: about 230 instructions per warp for 512 values.
+// turned) 127 us in a burst, 137 in a long run, 4.6 TB/s; 32,768 tokens of 40 heads of 128 133 us, 5.2 TB/s.
+// What is left of the way to a copy's 6.5 is latency: 64 to 66 % of the issue slots are used (about 230
+// instructions per warp for 512 values) and 53 to 60 % of the memory's rate, by 5.5 warps of a scheduler's 16, each
+// of which loads, computes, stores and ends with nothing of the next token in flight.
 #include <algorithm>
 
 #include "enc_common.cuh"
