@@ -361,3 +361,58 @@ def test_attention_rows_computed_again_share_their_loads():
     odd = v.clone()
     odd[4180] = math.nan
     assert ms(odd) < 90 * ms(v)
+
+
+THREADS = """
+import sys, threading
+import torch
+sys.path.insert(0, {repo!r})
+from ragrt_b200 import _lib, encoder
+if {python}:
+    encoder._bound = encoder._NoBinding                   # ctypes lets go of the interpreter during a call
+cu = torch.tensor([0, 30, 700], dtype=torch.int32, device="cuda")
+cos = torch.rand(700, 32, device="cuda")
+pos = torch.arange(700, device="cuda")
+sets = []
+for i in range(8):
+    g = torch.Generator(device="cuda").manual_seed(i)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda").half()
+    sets.append((n(700, 4, 64), n(700, 2, 64), n(700, 2, 64), n(700, 128), n(272, 128), n(700, 136)))
+
+
+def work(q, k, v, x, w, dh):
+    a, b = encoder.qk_norm_rope(q, k, cos, cos, pos)
+    h, gate, up = encoder.gated_ffn(x, w[:136], w[136:], keep=True)
+    return (a, b, encoder.packed_attention(a, b, v, cu, causal=True), h,
+            *encoder.gated_ffn_backward(dh, x, w[:136], w[136:], gate, up))
+
+
+torch.cuda.synchronize()
+start, got = threading.Barrier(8), [None] * 8
+
+
+def run(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        for _ in range(20):
+            got[i] = work(*sets[i])
+        torch.cuda.current_stream().synchronize()
+
+
+threads = [threading.Thread(target=run, args=(i,)) for i in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+for s, r in zip(sets, got):
+    assert all(torch.equal(a, b) for a, b in zip(work(*s), r))
+torch.cuda.synchronize()
+assert _lib.lib().ragrt_device_error(0) == 0
+print("equal")
+"""
+
+
+@pytest.mark.parametrize("python", [False, True], ids=["binding", "ctypes"])
+def test_threads_that_all_make_their_first_calls_at_once(python):
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", THREADS.format(repo=repo, python=python)], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "equal" in r.stdout, r.stderr[-3000:]
