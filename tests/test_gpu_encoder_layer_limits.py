@@ -51,6 +51,14 @@ def test_norm_rope_of_one_token_with_a_million_heads():
 
 
 # ------------------------------------------------------------------------------------ attention
+def attention64(q, k, v, cu, causal, scale=None):
+    """layer_helpers.attention64 with the bound of a divisor that sums the rounded weights: with weights w (1 + d),
+    |d| <= e, sum w (1 + d) v / sum w (1 + d) is off from o = sum p v by sum p d (v - o) to first order, which is
+    e (sum p |v| + |o|) at most; there it is e sum p |v|, that of the unrounded sum."""
+    want, bound = L.attention64(q, k, v, cu, causal, scale)
+    return want, bound + 1.02 * L.EPS[q.dtype] * want.abs()
+
+
 def by_scores(scores, v, D, dtype):
     """q, k, v of one head whose row 0 onwards have score `scores[j]` (in powers of two) for key j."""
     n = scores.shape[0]
@@ -73,7 +81,7 @@ def test_attention_reference_moves_twice_in_a_block(D, causal):
     q, k, v = by_scores(scores, v, D, torch.bfloat16)
     cu = L.cu_of([n], "cuda")
     scale = math.log(2.0)
-    want, bound = L.attention64(q, k, v, cu, causal, scale=scale)
+    want, bound = attention64(q, k, v, cu, causal, scale=scale)
     for _ in range(20):
         L.check(encoder.packed_attention(q, k, v, cu, causal=causal, scale=scale), want, bound)
 
@@ -88,7 +96,7 @@ def test_attention_what_is_seen_and_not_finite(T, D, causal, dtype):
     H, KV = 4, 2
     q, k, v = (torch.randn(T, h, D, generator=gen(h + i), device="cuda").to(dtype) for i, h in enumerate((H, KV, KV)))
     cu = L.cu_of([T], "cuda")
-    want, bound = L.attention64(q, k, v, cu, causal)
+    want, bound = attention64(q, k, v, cu, causal)
     seen = lambda row: slice(row if causal else 0, None)
     q[100, 1, 5] = math.nan
     want[100, 1] = math.nan
@@ -161,7 +169,7 @@ def test_attention_many_small_weights_beside_a_large_one():
     v[0] = 0
     q, k, v = by_scores(scores, v, 64, torch.float16)
     cu, scale = L.cu_of([n], "cuda"), math.log(2.0)
-    want, bound = L.attention64(q, k, v, cu, False, scale=scale)
+    want, bound = attention64(q, k, v, cu, False, scale=scale)
     L.check(encoder.packed_attention(q, k, v, cu, scale=scale), want, bound)
 
 
@@ -324,7 +332,7 @@ def test_attention_rows_before_values_that_are_not_finite(T, D, dtype):
     H, KV = 4, 2
     q, k, v = (torch.randn(T, h, D, generator=gen(h + i), device="cuda").to(dtype) for i, h in enumerate((H, KV, KV)))
     cu = L.cu_of([T - 7], "cuda")
-    want, bound = L.attention64(q, k, v, cu, True)
+    want, bound = attention64(q, k, v, cu, True)
     for i, at in enumerate((37, 38, 200, 301, 511, 640, 700, T - 9)):
         v[at, 1, i], v[at, 1, i + 8] = math.nan, math.inf
         want[at:T - 7, 2:, i], want[at:T - 7, 2:, i + 8] = math.nan, math.inf
